@@ -11,9 +11,12 @@ LIB_PATH = os.path.join(_HERE, "libquamba_amd.so")
 
 QA_OK = 0
 ABI_VERSION = 3          # what qa_abi_version() of a matching library returns
+LM_ABI_VERSION = 1       # and qa_lm_abi_version()
 QA_OUT_I8, QA_OUT_F16, QA_OUT_BF16 = 0, 1, 2
 QA_ROUND_RNE, QA_ROUND_HALF_AWAY = 0, 1
 QA_IN_F16, QA_IN_F32 = 0, 1
+QA_LM_I8, QA_LM_F16, QA_LM_BF16, QA_LM_F32 = 0, 1, 2, 3
+QA_GATE_PLAIN, QA_GATE_SIGMOID, QA_GATE_SILU = 0, 1, 2
 
 i32, i64, f32, vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
 
@@ -207,6 +210,44 @@ class QaMamba2Params(C.Structure):
     ] + _CALL_FIELDS
 
 
+class QaAddNormParams(C.Structure):
+    _fields_ = [
+        ("rows", i32), ("dim", i32), ("x_type", i32), ("param_type", i32), ("residual_type", i32), ("out_type", i32),
+        ("gate_act", i32), ("dynamic_scale", i32), ("eps", f32), ("scale", f32), ("out_scale", f32), ("reserved0", i32),
+        ("x_row_stride", i64), ("gate_row_stride", i64), ("residual_row_stride", i64), ("residual_out_row_stride", i64),
+        ("out_row_stride", i64),
+        ("x", vp), ("weight", vp), ("post_weight", vp), ("gate", vp), ("scale_vector", vp), ("residual", vp),
+        ("residual_out", vp), ("out", vp), ("scales", vp),
+    ]
+
+
+class QaTokenLogprobsParams(C.Structure):
+    _fields_ = [
+        ("rows", i32), ("vocab", i32), ("logits_type", i32), ("token_bytes", i32), ("top", i32), ("reserved0", i32),
+        ("row_stride", i64), ("logits", vp), ("tokens", vp), ("logprobs", vp), ("entropy", vp), ("top_logprobs", vp),
+        ("top_tokens", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class QaMmTokenLogprobsParams(C.Structure):
+    _fields_ = [
+        ("rows", i32), ("vocab", i32), ("k", i32), ("a_scale_numel", i32), ("w_scale_numel", i32), ("token_bytes", i32),
+        ("top", i32), ("reserved0", i32), ("lda", i64), ("ldw", i64),
+        ("a", vp), ("w", vp), ("a_scale", vp), ("w_scale", vp), ("tokens", vp), ("logprobs", vp), ("entropy", vp),
+        ("top_logprobs", vp), ("top_tokens", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+# name -> (restype, argtypes); every symbol declared in include/quamba_amd_lm.h
+LM_SYMBOLS = {
+    "qa_lm_abi_version": (C.c_int, []),
+    "qa_add_rmsnorm": (C.c_int, [C.POINTER(QaAddNormParams), vp]),
+    "qa_token_logprobs_workspace_bytes": (C.c_int64, [C.POINTER(QaTokenLogprobsParams)]),
+    "qa_token_logprobs": (C.c_int, [C.POINTER(QaTokenLogprobsParams), vp]),
+    "qa_mm_token_logprobs_workspace_bytes": (C.c_int64, [C.POINTER(QaMmTokenLogprobsParams)]),
+    "qa_mm_token_logprobs": (C.c_int, [C.POINTER(QaMmTokenLogprobsParams), vp]),
+}
+
 # name -> (restype, argtypes); every symbol declared in include/quamba_amd.h
 SYMBOLS = {
     "qa_status_string": (C.c_char_p, [C.c_int]),
@@ -248,13 +289,14 @@ def lib():
                 f"{LIB_PATH} is missing: build it with `python -m quamba_amd.build` "
                 "(quamba_amd has no CPU or PyTorch fallback)")
         handle = C.CDLL(LIB_PATH)
-        for name, (res, args) in SYMBOLS.items():
+        for name, (res, args) in (*SYMBOLS.items(), *LM_SYMBOLS.items()):
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
-        if handle.qa_abi_version() != ABI_VERSION:
-            raise RuntimeError(f"{LIB_PATH} has ABI version {handle.qa_abi_version()}, this binding expects "
-                               f"{ABI_VERSION}: rebuild it with `python -m quamba_amd.build --force`")
+        found = handle.qa_abi_version(), handle.qa_lm_abi_version()
+        if found != (ABI_VERSION, LM_ABI_VERSION):
+            raise RuntimeError(f"{LIB_PATH} has ABI versions {found}, this binding expects {(ABI_VERSION, LM_ABI_VERSION)}: "
+                               "rebuild it with `python -m quamba_amd.build --force`")
         _lib = handle
     return _lib
 

@@ -16,6 +16,7 @@ BUILD = os.path.join(HERE, "csrc", "build")
 LIB = os.path.join(HERE, "libquamba_amd.so")
 HOST = os.path.join(HERE, "_host.so")
 HOST_SRC = os.path.join(HERE, "host", "layer_call.cpp")
+HEADERS = [os.path.join(HERE, "..", "include", h) for h in ("quamba_amd.h", "quamba_amd_lm.h")]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
@@ -40,7 +41,7 @@ def _newer(a, b):
 def _compile(src, force):
     obj = os.path.join(BUILD, src[:-4] + ".o")
     path = os.path.join(CSRC, src)
-    deps = [path, os.path.join(CSRC, "qa_common.hpp"), os.path.join(HERE, "..", "include", "quamba_amd.h")]
+    deps = [path, os.path.join(CSRC, "qa_common.hpp"), *HEADERS]
     deps += [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hpp")]
     if force or any(_newer(d, obj) for d in deps):
         cmd = [HIPCC, *FLAGS, "-c", path, "-o", obj]

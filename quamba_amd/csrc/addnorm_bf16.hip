@@ -1,0 +1,8 @@
+// The residual sum with its norms, of bf16 rows (addnorm.hpp).
+#include "addnorm.hpp"
+
+namespace qa {
+namespace lm {
+int add_rmsnorm_bf16(const QaAddNormParams& p, const AddNormShape& s, bool wide, hipStream_t stream) { return add_rmsnorm_of_type<__bf16>(p, s, wide, stream); }
+}  // namespace lm
+}  // namespace qa

@@ -1,0 +1,327 @@
+// Log probabilities of given tokens of the head's int8 product (qa_mm_token_logprobs): the tiles of gemm_core.hpp with a softmax's
+// statistics in the place of the stores.
+//
+//   l[m, n] = s_a[m|0] * (s_w[n|0] * float(sum_k a[m, k] w[n, k]))       (the products' sum is exact, the scales are those of qa_gemm_w8a8)
+//
+// rows x vocabulary logits would be the largest tensor of an evaluation by far (16384 x 50280: 1.6 GB in 16 bits, written and read again).
+// Here a workgroup reduces its tile to a RowStats and a best column per row: 16 bytes for each row and tile of columns go to the
+// workspace, and with them the logit of the row's given token from the one lane that holds it.  A second launch joins them.
+#include "gemm_core.hpp"
+#include "row_stats.hpp"
+
+namespace qa {
+namespace lm {
+namespace {
+
+using namespace gemm;
+
+struct TilePart {
+    float m, s, t;
+    int best;              // the lowest column with the value m
+};
+
+// v of the lanes that hold other columns of the same row (ROWS rows: lane l has row l % ROWS), by op, in every one of them
+template <int ROWS, class Op>
+__device__ __forceinline__ uint32_t over_columns(uint32_t v, Op op) {
+    const auto halves = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(halves[0], halves[1]);
+    if constexpr (ROWS == 16) {
+        const auto rows = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = op(rows[0], rows[1]);
+    }
+    return v;
+}
+template <int ROWS>
+__device__ __forceinline__ float most_over_columns(float v) {
+    return __uint_as_float(over_columns<ROWS>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+template <int ROWS>
+__device__ __forceinline__ float sum_over_columns(float v) {
+    return __uint_as_float(over_columns<ROWS>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+
+// A wave's TM x TN blocks: the statistics of each of its rows to parts[row_at + row], the given tokens' logits to `given`.
+// s_lds: column scales, row scales, and the low words of the tokens, of the workgroup's tile.
+template <int TM, int TN, int BM, int BN, class V, int NI, int NJ>
+__device__ __forceinline__ void tile_stats(const QaMmTokenLogprobsParams& p, V (&acc)[NI][NJ], const float* s_lds, int row_at, int col_at, int m0, int n0, int lane,
+                                           TilePart* parts, float* given) {
+    using Q = QuadView<V>;
+    constexpr int kQuads = TN * 32 / (256 / Q::kRows), kRowBlocks = TM * 32 / Q::kRows;
+    static_assert(NI * Q::kQuadsPer == kQuads && NJ == kRowBlocks, "accumulators of another tile");
+    const bool whole = n0 + col_at + TN * 32 <= p.vocab;
+    float s_col[kQuads][4];
+#pragma unroll
+    for (int u = 0; u < kQuads; ++u) {
+        const float4 v = *reinterpret_cast<const float4*>(s_lds + col_at + Q::column_of(u, lane));
+        s_col[u][0] = v.x; s_col[u][1] = v.y; s_col[u][2] = v.z; s_col[u][3] = v.w;
+    }
+#pragma unroll
+    for (int b = 0; b < kRowBlocks; ++b) {
+        const int row = row_at + b * Q::kRows + Q::row_of(lane);
+        const float s_row = s_lds[BN + row];
+        const int token = reinterpret_cast<const int*>(s_lds)[BN + BM + row] - (n0 + col_at);      // its column among the wave's
+        float v[kQuads][4], most = kLowest;
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                v[u][t] = s_row * (s_col[u][t] * Q::value(acc, u, b, t));
+                if (!whole && n0 + col_at + Q::column_of(u, lane) + t >= p.vocab) v[u][t] = -__builtin_inff();
+                most = fmaxf(most, v[u][t]);
+            }
+        most = most_over_columns<Q::kRows>(most);
+        RowStats r = {most, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) r.add(v[u][t]);
+        r.s = sum_over_columns<Q::kRows>(r.s);
+        r.t = sum_over_columns<Q::kRows>(r.t);
+        uint32_t best = 0xffffffffu;
+        if (p.top) {
+#pragma unroll
+            for (int u = kQuads - 1; u >= 0; --u)
+#pragma unroll
+                for (int t = 3; t >= 0; --t)
+                    if (v[u][t] == most) best = Q::column_of(u, lane) + t;
+            best = over_columns<Q::kRows>(best, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+        }
+        // (a row of NaNs has no such column)
+        if (lane < Q::kRows) parts[row] = {r.m, r.s, r.t, static_cast<int>(n0 + col_at + (best == 0xffffffffu ? 0 : best))};
+        if (__builtin_amdgcn_ballot_w64(token >= 0 && token < TN * 32)) {
+#pragma unroll
+            for (int u = 0; u < kQuads; ++u)
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    if (token == Q::column_of(u, lane) + t && m0 + row < p.rows && n0 + col_at + token < p.vocab) given[m0 + row] = v[u][t];
+        }
+    }
+}
+
+template <int TM, int TN, int WGM, int WGN, int STAGES>
+__global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmTokenLogprobsParams p) {
+    using C = Cfg<TM, TN, WGM, WGN, STAGES>;
+    constexpr int BM = C::kBM, BN = C::kBN, WAVES = C::kWaves;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    static_assert(WGN * BM * static_cast<int>(sizeof(TilePart)) <= C::kLdsBytes, "the waves' statistics take the place of the operands");
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave % WGM, wn = wave / WGM;
+    const int tiles_m = (p.rows + BM - 1) / BM, tiles_n = (p.vocab + BN - 1) / BN;
+    int tile_m, tile_n;
+    tile_of_workgroup<BM, BN>(blockIdx.x, tiles_m, tiles_n, tile_m, tile_n);
+    const int m0 = tile_m * BM, n0 = tile_n * BN;
+    const v4i rsrc_a = make_rsrc(p.a, static_cast<int>((static_cast<int64_t>(p.rows) - 1) * p.lda + p.k));
+    const v4i rsrc_w = make_rsrc(p.w, static_cast<int>((static_cast<int64_t>(p.vocab) - 1) * p.ldw + p.k));
+    const uint32_t lds_base = lds_offset_of(lds);
+
+    using Scales = TileScales<BM, BN, WAVES>;
+    Scales::request(lds_base + C::kLdsBytes, p.a_scale, p.a_scale_numel, p.rows, m0, p.w_scale, p.w_scale_numel, p.vocab, n0, wave, lane);
+    const v4i rsrc_t = make_rsrc(p.tokens, static_cast<int>(min(static_cast<int64_t>(p.rows) * p.token_bytes, static_cast<int64_t>(0x7fffffff))));
+#pragma unroll
+    for (int i = 0; i < BM / 64; ++i)
+        if (i % WAVES == wave) buffer_load_lds_b32(rsrc_t, lds_base + C::kLdsBytes + Scales::kBytes + i * 256, (m0 + i * 64 + lane) * p.token_bytes);
+    TileLoader<C::kAInstr> load_a;
+    TileLoader<C::kWInstr> load_w;
+    load_a.template init<WAVES>(m0, p.rows, p.lda, wave, lane);
+    load_w.template init<WAVES>(n0, p.vocab, p.ldw, wave, lane);
+    const int k_tiles = (p.k + kBK - 1) / kBK;
+
+    TilePart* const parts = reinterpret_cast<TilePart*>(lds);
+    TilePart* const out = static_cast<TilePart*>(p.workspace);
+    auto finish = [&](auto& acc) {
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        __syncthreads();
+        tile_stats<TM, TN, BM, BN>(p, acc, reinterpret_cast<const float*>(lds + C::kLdsBytes), wm * TM * 32, wn * TN * 32, m0, n0, lane, parts + wn * BM,
+                                   reinterpret_cast<float*>(out + static_cast<int64_t>(p.rows) * tiles_n));
+        __syncthreads();
+        for (int row = tid; row < BM; row += C::kThreads) {
+            if (m0 + row >= p.rows) break;
+            TilePart best = parts[row];
+            RowStats r = {best.m, best.s, best.t};
+#pragma unroll
+            for (int i = 1; i < WGN; ++i) {
+                const TilePart o = parts[i * BM + row];
+                if (o.m > best.m) best = o;
+                r.join({o.m, o.s, o.t});
+            }
+            out[static_cast<int64_t>(tile_n) * p.rows + m0 + row] = {r.m, r.s, r.t, best.best};
+        }
+    };
+    if constexpr (TM * TN > 1) {
+        // (requests as in the product's own kernel: one per kPace multiplications, counted from the barrier)
+        using Mma = RotatedMma<TM, TN>;
+        constexpr int kReq = C::kAInstr + C::kWInstr, kPace = kReq <= Mma::kPerTile / 4 ? 4 : Mma::kPerTile / kReq;
+        constexpr int kEarly = Mma::kBehindBarrier / kPace < kReq ? Mma::kBehindBarrier / kPace : kReq;
+        auto request = [&](int r, int k0, uint32_t stage) {
+            if (r < C::kAInstr) load_a.template issue_one<WAVES>(r, rsrc_a, k0, p.k, lds_base + stage, wave);
+            else if (r < kReq) load_w.template issue_one<WAVES>(r - C::kAInstr, rsrc_w, k0, p.k, lds_base + stage + BM * kBK, wave);
+        };
+        auto request_whole = [&](int r, int k0, uint32_t stage) {
+            if (r < C::kAInstr) load_a.template issue_whole<WAVES>(r, rsrc_a, k0, lds_base + stage, wave);
+            else if (r < kReq) load_w.template issue_whole<WAVES>(r - C::kAInstr, rsrc_w, k0, lds_base + stage + BM * kBK, wave);
+        };
+#pragma unroll
+        for (int t = 0; t < STAGES - 1; ++t)
+#pragma unroll
+            for (int r = 0; r < kReq; ++r) request(r, t * kBK, t * C::kStageBytes);
+#pragma unroll
+        for (int r = 0; r < kEarly; ++r) request(r, (STAGES - 1) * kBK, (STAGES - 1) * C::kStageBytes);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((STAGES - 2) * kReq + kEarly));
+        __syncthreads();
+        const uint8_t* my_a = lds + (wm * TM * 32) * kBK;
+        const uint8_t* my_w = lds + BM * kBK + (wn * TN * 32) * kBK;
+        Mma mma;
+        mma.init(lane);
+        mma.start(my_a, my_w);
+        uint32_t cur = 0, late = (STAGES - 1) * C::kStageBytes;
+        auto multiply = [&](int kt, auto&& req) {
+            const uint32_t nxt = cur + C::kStageBytes == C::kLdsBytes ? 0 : cur + C::kStageBytes;
+            mma.template tile<(STAGES - 2) * kReq>(my_a + cur, my_w + cur, my_a + nxt, my_w + nxt, [&](int idx) {
+                if (idx % kPace != kPace - 1) return;
+                const int r = idx / kPace;
+                if (r < kEarly) req(r, (kt + STAGES) * kBK, cur);
+                else req(r, (kt + STAGES - 1) * kBK, late);
+            });
+            late = cur;
+            cur = nxt;
+        };
+        int kt = 0;
+        for (const int whole = p.k / kBK - STAGES; kt < whole; ++kt) multiply(kt, request_whole);
+        for (; kt < k_tiles; ++kt) multiply(kt, request);
+        finish(mma.acc);
+    } else {
+        const int frow = lane & 31, fhalf = lane >> 5;
+        v16i acc[1][1];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[0][0][r] = 0;
+        auto issue = [&](int tile) {
+            const uint32_t base = lds_base + (tile % STAGES) * C::kStageBytes;
+            load_a.template issue<WAVES>(rsrc_a, tile * kBK, p.k, base, wave);
+            load_w.template issue<WAVES>(rsrc_w, tile * kBK, p.k, base + BM * kBK, wave);
+        };
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) issue(s);
+        for (int kt = 0; kt < k_tiles; ++kt) {
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm((STAGES - 2) * (C::kAInstr + C::kWInstr)));
+            __syncthreads();
+            const uint8_t* stage = lds + (kt % STAGES) * C::kStageBytes;
+            const int nt = kt + STAGES - 1;
+            const uint32_t nbase = lds_base + (nt % STAGES) * C::kStageBytes;
+            static_assert(C::kAInstr + C::kWInstr <= 4, "a request behind each of four multiplications");
+            mma_tile_paced(stage + wm * 32 * kBK, stage + BM * kBK + wn * 32 * kBK, frow, fhalf, acc[0][0], [&](int r) {
+                if (r < C::kAInstr) load_a.template issue_one<WAVES>(r, rsrc_a, nt * kBK, p.k, nbase, wave);
+                else if (r < C::kAInstr + C::kWInstr) load_w.template issue_one<WAVES>(r - C::kAInstr, rsrc_w, nt * kBK, p.k, nbase + BM * kBK, wave);
+            });
+        }
+        finish(acc);
+    }
+}
+
+// Rows' parts, tiles_n of them each: kThreads / at_once threads share a row, at_once rows a workgroup.
+constexpr int kJoinThreads = 256;
+__global__ __launch_bounds__(kJoinThreads) void mm_token_logprobs_join_kernel(QaMmTokenLogprobsParams p, int tiles_n, int at_once) {
+    __shared__ TilePart s_part[kJoinThreads];
+    const int r = threadIdx.x % at_once, first = threadIdx.x / at_once, step = kJoinThreads / at_once;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * at_once + r;
+    const TilePart* const parts = static_cast<const TilePart*>(p.workspace);
+    RowStats all;
+    all.clear();
+    TilePart best = {-__builtin_inff(), 0.0f, 0.0f, 0x7fffffff};
+    auto take = [&](const TilePart& o) {
+        if (o.m > best.m || (o.m == best.m && o.best < best.best)) best = o;
+        all.join({o.m, o.s, o.t});
+    };
+    if (row < p.rows)
+        for (int i = first; i < tiles_n; i += step) take(parts[i * static_cast<int64_t>(p.rows) + row]);
+    for (int half = step / 2; half > 0; half /= 2) {
+        __syncthreads();
+        s_part[threadIdx.x] = {all.m, all.s, all.t, best.best};
+        __syncthreads();
+        if (first < half) {
+            const TilePart o = s_part[threadIdx.x + half * at_once];
+            best.m = all.m;                                // (an empty side has the lowest number and no column)
+            take(o);
+        }
+    }
+    if (first != 0 || row >= p.rows) return;
+    const int64_t token = token_of(p.tokens, p.token_bytes, row);
+    float lp = token < 0 ? 0.0f : __builtin_nanf("");
+    if (token >= 0 && token < p.vocab) lp = all.logprob(reinterpret_cast<const float*>(parts + static_cast<int64_t>(p.rows) * tiles_n)[row]);
+    p.logprobs[row] = lp;
+    p.entropy[row] = all.s > 0.0f ? all.entropy() : __builtin_nanf("");
+    if (p.top) {
+        p.top_logprobs[row] = all.logprob(all.m);
+        p.top_tokens[row] = best.best;
+    }
+}
+
+// Rows and columns of a tile.
+struct Tile {
+    int bm, bn;
+};
+Tile tile_of(int rows, int vocab) {
+    if (rows <= 64) return {64, 64};
+    if (rows <= 128) return {128, 128};
+    return {256, 256};
+}
+
+int check(const QaMmTokenLogprobsParams& p) {
+    if (p.rows < 0 || p.vocab < 1 || p.k < 1) return QA_ERR_SHAPE;
+    if (p.token_bytes != 4 && p.token_bytes != 8) return QA_ERR_UNSUPPORTED;
+    if (p.top != 0 && p.top != 1) return QA_ERR_UNSUPPORTED;
+    return QA_OK;
+}
+
+int64_t workspace_bytes(const QaMmTokenLogprobsParams& p) {
+    const Tile tile = tile_of(p.rows, p.vocab);
+    const int64_t tiles_n = (p.vocab + tile.bn - 1) / tile.bn;
+    return p.rows * (tiles_n * static_cast<int64_t>(sizeof(TilePart)) + static_cast<int64_t>(sizeof(float)));
+}
+
+template <int TM, int TN, int WGM, int WGN, int STAGES>
+int launch(const QaMmTokenLogprobsParams& p, hipStream_t stream) {
+    using C = Cfg<TM, TN, WGM, WGN, STAGES>;
+    const int tiles_n = (p.vocab + C::kBN - 1) / C::kBN;
+    const int64_t tiles = static_cast<int64_t>((p.rows + C::kBM - 1) / C::kBM) * tiles_n;
+    if (tiles > 0x7fffffffLL) return QA_ERR_SHAPE;
+    auto kernel = mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES>;
+    constexpr int kLds = C::kLdsBytes + TileScales<C::kBM, C::kBN, C::kWaves>::kBytes + C::kBM * 4;
+    static_assert(kLds <= 160 * 1024, "LDS of a CU");
+    if (kLds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) return check_launch();
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(C::kThreads), kLds, stream, p);
+    if (const int status = check_launch()) return status;
+    const int at_once = p.rows >= 4096 ? 16 : 1;
+    hipLaunchKernelGGL(mm_token_logprobs_join_kernel, dim3(static_cast<unsigned>((p.rows + at_once - 1) / at_once)), dim3(kJoinThreads), 0, stream, p, tiles_n, at_once);
+    return check_launch();
+}
+
+}  // namespace
+}  // namespace lm
+}  // namespace qa
+
+extern "C" int64_t qa_mm_token_logprobs_workspace_bytes(const QaMmTokenLogprobsParams* p) {
+    using namespace qa::lm;
+    return p && check(*p) == QA_OK && p->rows > 0 ? workspace_bytes(*p) : 0;
+}
+
+extern "C" int qa_mm_token_logprobs(const QaMmTokenLogprobsParams* p, void* stream_) {
+    using namespace qa;
+    using namespace qa::lm;
+    if (!p) return QA_ERR_NULL;
+    if (const int status = check(*p)) return status;
+    if (p->rows == 0) return QA_OK;
+    if (!p->a || !p->w || !p->a_scale || !p->w_scale || !p->tokens || !p->logprobs || !p->entropy || !p->workspace) return QA_ERR_NULL;
+    if (p->top && (!p->top_logprobs || !p->top_tokens)) return QA_ERR_NULL;
+    if ((p->a_scale_numel != 1 && p->a_scale_numel != p->rows) || (p->w_scale_numel != 1 && p->w_scale_numel < p->vocab)) return QA_ERR_SHAPE;
+    if (p->k % 16 != 0 || p->lda % 16 != 0 || p->ldw % 16 != 0 || !aligned16(p->a) || !aligned16(p->w) || p->lda < p->k || p->ldw < p->k) return QA_ERR_STRIDE;
+    if (!aligned4(p->a_scale) || !aligned4(p->w_scale) || reinterpret_cast<uintptr_t>(p->tokens) % p->token_bytes != 0) return QA_ERR_STRIDE;
+    // operands are addressed with 32-bit byte offsets inside a buffer descriptor
+    if (static_cast<int64_t>(p->rows) * p->lda >= 0x70000000LL || static_cast<int64_t>(p->vocab) * p->ldw >= 0x70000000LL) return QA_ERR_SHAPE;
+    if (!aligned16(p->workspace) || p->workspace_bytes < workspace_bytes(*p)) return QA_ERR_SCRATCH;
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    const Tile tile = tile_of(p->rows, p->vocab);
+    if (tile.bm == 64) return launch<1, 1, 2, 2, 4>(*p, stream);
+    if (tile.bm == 128) return launch<2, 1, 2, 4, 4>(*p, stream);
+    return launch<4, 2, 2, 4, 2>(*p, stream);
+}

@@ -1,0 +1,154 @@
+// Running statistics of a softmax over a part of a row, the best entries of a row in order, and how both are joined.
+//
+// Stats: the largest value m, s = sum e^(l - m) and t = sum (l - m) e^(l - m), in fp32.  Two parts join at the larger m:
+//   s = sum s_i f_i,   t = sum (t_i + (m_i - m) s_i) f_i,   f_i = e^(m_i - m)
+// and at the end  log sum exp = m + ln s,  entropy = ln s - t / s.  Masked values (-inf) add nothing; m starts at the lowest
+// finite number, so a part without a value has s = 0.  A NaN or +inf leaves a NaN in s, which joins keep.
+#pragma once
+
+#include "lm_common.hpp"
+#include "normgated_core.hpp"
+
+namespace qa {
+namespace lm {
+
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLowest = -3.402823466e38f;
+
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+struct RowStats {
+    float m, s, t;
+    __device__ __forceinline__ void clear() { m = kLowest; s = 0.0f; t = 0.0f; }
+    // the statistics as seen from `most` >= m
+    __device__ __forceinline__ void raise(float most) {
+        const float d = fmaxf(m - most, -1e30f), f = exp_fast(d);          // (0 * -inf has no place here)
+        t = f * __builtin_fmaf(d, s, t);
+        s *= f;
+        m = most;
+    }
+    // one value, m no smaller than it
+    __device__ __forceinline__ void add(float value) {
+        const float d = value - m, e = exp_fast(d);
+        s += e;
+        t = __builtin_fmaf(fmaxf(d, -200.0f), e, t);                       // (e is 0 from -104 on)
+    }
+    __device__ __forceinline__ void join(RowStats o) {
+        const float most = fmaxf(m, o.m);
+        raise(most);
+        o.raise(most);
+        s += o.s;
+        t += o.t;
+    }
+    __device__ __forceinline__ float entropy() const { return logf(s) - t / s; }
+    // log probability of a value; NaN where the row has no distribution
+    __device__ __forceinline__ float logprob(float value) const { return s > 0.0f ? (value - m) - logf(s) : __builtin_nanf(""); }
+};
+
+// over the wave, in every lane
+__device__ __forceinline__ RowStats wave_stats(RowStats r) {
+    r.raise(wave_max(r.m));
+    r.s = wave_sum(r.s);
+    r.t = wave_sum(r.t);
+    return r;
+}
+
+// An entry of a row as one number: larger values first, of equal ones (-0 and 0 are equal) the lower index.  0: no entry.  A NaN ranks with -inf.
+typedef uint64_t Entry;
+__device__ __forceinline__ Entry entry_of(float value, uint32_t index) {
+    const float v = value == value ? value + 0.0f : -__builtin_inff();
+    const uint32_t u = __float_as_uint(v), key = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+    return static_cast<uint64_t>(key) << 32 | ~index;
+}
+__device__ __forceinline__ float value_of(Entry e) {
+    const uint32_t key = static_cast<uint32_t>(e >> 32);
+    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+__device__ __forceinline__ uint32_t index_of(Entry e) { return ~static_cast<uint32_t>(e); }
+
+__device__ __forceinline__ Entry entry_of_lane(Entry e, int lane) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(e >> 32), lane))) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(e)), lane));
+}
+
+// the entry of lane ^ MASK, MASK + 1 a power of two (a mirror) or MASK a power of two
+template <int MASK>
+__device__ __forceinline__ uint32_t word_across(uint32_t v, int lane) {
+    auto dpp = [](uint32_t a, auto ctrl) { return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(a), decltype(ctrl)::value, 0xf, 0xf, true)); };
+    if constexpr (MASK == 1) return dpp(v, std::integral_constant<int, 0xb1>{});
+    else if constexpr (MASK == 2) return dpp(v, std::integral_constant<int, 0x4e>{});
+    else if constexpr (MASK == 3) return dpp(v, std::integral_constant<int, 0x1b>{});
+    else if constexpr (MASK == 7) return dpp(v, std::integral_constant<int, 0x141>{});
+    else if constexpr (MASK == 15) return dpp(v, std::integral_constant<int, 0x140>{});
+    else if constexpr (MASK == 4) return word_across<3>(word_across<7>(v, lane), lane);
+    else if constexpr (MASK == 8) return dpp(v, std::integral_constant<int, 0x128>{});
+    else if constexpr (MASK == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return lane & 16 ? r[0] : r[1];
+    } else if constexpr (MASK == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return lane & 32 ? r[0] : r[1];
+    } else if constexpr (MASK == 31) return word_across<16>(word_across<15>(v, lane), lane);
+    else return word_across<32>(word_across<31>(v, lane), lane);
+}
+template <int MASK>
+__device__ __forceinline__ Entry across(Entry e, int lane) {
+    return static_cast<uint64_t>(word_across<MASK>(static_cast<uint32_t>(e >> 32), lane)) << 32 | word_across<MASK>(static_cast<uint32_t>(e), lane);
+}
+// lane l and lane l ^ MASK in descending order: the lower lane of the two gets the larger entry
+template <int MASK>
+__device__ __forceinline__ Entry order(Entry e, int lane) {
+    constexpr int kTop = (MASK + 1) & MASK ? MASK : (MASK + 1) / 2;        // the highest bit of MASK
+    const Entry o = across<MASK>(e, lane);
+    return ((e > o) == !(lane & kTop)) ? e : o;
+}
+template <int HALF>
+__device__ __forceinline__ Entry order_from(Entry e, int lane) {           // a sequence that rises and falls, in blocks of 2 HALF
+    if constexpr (HALF == 0) return e;
+    else return order_from<HALF / 2>(order<HALF>(e, lane), lane);
+}
+// the wave's entries in descending order: sorted runs of 2, 4 .. 64, each of two halves met as mirror images
+__device__ __forceinline__ Entry sort_wave(Entry e, int lane) {
+    e = order<1>(e, lane);
+    e = order_from<1>(order<3>(e, lane), lane);
+    e = order_from<2>(order<7>(e, lane), lane);
+    e = order_from<4>(order<15>(e, lane), lane);
+    e = order_from<8>(order<31>(e, lane), lane);
+    return order_from<16>(order<63>(e, lane), lane);
+}
+// the best 64 of two descending sequences, descending
+__device__ __forceinline__ Entry merge_waves(Entry a, Entry b, int lane) {
+    const Entry o = across<63>(b, lane);
+    return order_from<32>(a > o ? a : o, lane);
+}
+
+// The best entries of what a wave has seen, lane i the i-th best.
+struct BestEntries {
+    Entry mine;
+    Entry last;            // the top-th best (the same in every lane): what comes in has to be larger
+    __device__ __forceinline__ void clear() { mine = last = 0; }
+    __device__ __forceinline__ void settle(int top) { last = entry_of_lane(mine, top - 1); }
+    // one candidate per lane (0: none): a few go in one by one, many as a sorted run
+    __device__ __forceinline__ void offer(Entry e, int top, int lane) {
+        uint64_t wanting = __builtin_amdgcn_ballot_w64(e > last);
+        if (__popcll(wanting) > 6) {
+            mine = merge_waves(mine, sort_wave(e > last ? e : 0, lane), lane);
+            settle(top);
+            return;
+        }
+        while (wanting) {
+            const Entry c = entry_of_lane(e, __builtin_ctzll(wanting));
+            wanting &= wanting - 1;
+            if (c <= last) continue;
+            // lane l takes the entry of lane l - 1 behind the place where c belongs
+            const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(mine)), 0x138, 0xf, 0xf, false));
+            const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(mine >> 32), 0x138, 0xf, 0xf, false));
+            const Entry before = static_cast<uint64_t>(hi) << 32 | lo;
+            if (mine < c) mine = lane > 0 && before < c ? before : c;
+            settle(top);
+        }
+    }
+};
+
+}  // namespace lm
+}  // namespace qa

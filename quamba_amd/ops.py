@@ -865,29 +865,26 @@ def ssd_chunk_scan_combined_fwd(q_x, x_scale, q_dt, dt_scale, q_A_log, A_log_sca
 # ----------------------------------------------------------------------------------------------
 # The residual stream between two blocks
 # ----------------------------------------------------------------------------------------------
-_LM_TYPES = {torch.int8: _lib.QA_LM_I8, torch.float16: _lib.QA_LM_F16, torch.bfloat16: _lib.QA_LM_BF16, torch.float32: _lib.QA_LM_F32}
-_GATE_ACTS = {"none": _lib.QA_GATE_PLAIN, "sigmoid": _lib.QA_GATE_SIGMOID, "silu": _lib.QA_GATE_SILU}
+_lm_native = None
 
 
-def _rows_of(t, name, shape, dtypes, device):
-    _require(t.is_cuda and t.device == device, f"{name} must be on {device}")
-    _require(t.dtype in dtypes, f"{name} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
-    _require(tuple(t.shape) == shape, f"{name} must have shape {shape}, not {tuple(t.shape)}")
-    _require(t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} must be contiguous along the last dimension")
-    _require(len(shape) < 2 or shape[0] <= 1 or t.stride(0) >= shape[-1], f"the rows of {name} must not overlap")
-    return t
-
-
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _overlap(a, b):
-    """Whether the memory between the first and the last element of two row matrices meets."""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+def _lm():
+    """quamba_amd._lm_host, bound to the library; raises if it is not built (there is no fallback)."""
+    global _lm_native
+    if _lm_native is None:
+        try:
+            from . import _lm_host as native
+        except ImportError as e:
+            raise RuntimeError("quamba_amd/_lm_host.so is missing or does not load: build it with `python -m quamba_amd.build`") from e
+        if getattr(native, "LM_ABI_VERSION", None) != _lib.LM_ABI_VERSION:
+            raise RuntimeError("quamba_amd/_lm_host.so is built for another layout of the parameter blocks: rebuild it with "
+                               "`python -m quamba_amd.build --force`")
+        l = _lib.lib()
+        native.bind(tuple(ct.cast(getattr(l, n), ct.c_void_p).value for n in (
+            "qa_add_rmsnorm", "qa_token_logprobs_workspace_bytes", "qa_token_logprobs", "qa_mm_token_logprobs_workspace_bytes", "qa_mm_token_logprobs")),
+            (torch.cuda.current_device, torch.cuda.set_device, torch._C._cuda_getCurrentRawStream, torch.cuda.OutOfMemoryError, _lib.check))
+        _lm_native = native
+    return _lm_native
 
 
 def add_rmsnorm(x, weight, eps, residual=None, post_weight=None, gate=None, gate_act="none", residual_scale=1.0, prenorm=True,
@@ -908,69 +905,8 @@ def add_rmsnorm(x, weight, eps, residual=None, post_weight=None, gate=None, gate
 
     Returns (y, v, scales): v None with prenorm=False, else in the type of residual or residual_dtype, written to residual_out
     where that is given (it may be residual itself and must not overlap the other tensors); scales (rows,) fp32 or None."""
-    _require(x.dim() == 2, "x must be (rows, dim)")
-    _require_gpu(x, "x")
-    rows, dim = x.shape
-    dev, half = x.device, (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32)
-    _rows_of(x, "x", (rows, dim), (torch.float16, torch.bfloat16, torch.float32), dev)
-    if not 8 <= dim <= 32768:
-        raise NotImplementedError("add_rmsnorm: rows of 8 to 32768 values")
-    params = [("weight", weight), ("post_weight", post_weight)]
-    vector = torch.is_tensor(residual_scale) and residual_scale.dim() > 0
-    if vector:
-        params.append(("residual_scale", residual_scale))
-    for n, t in params:
-        if t is not None:
-            _rows_of(t, n, (dim,), half, dev)
-            _require(t.dtype == weight.dtype, f"{n} must be of the type of weight")
-    if residual is not None:
-        _rows_of(residual, "residual", (rows, dim), half, dev)
-        _require(residual_dtype in (None, residual.dtype), "residual_dtype differs from the type of residual")
-    if gate is not None:
-        _require(gate.dim() in (1, 2), "gate must be (rows, dim) or (dim,)")
-        if gate.dim() == 2 and (gate.shape[0] == 1 or gate.stride(0) == 0) and tuple(gate.shape) in ((1, dim), (rows, dim)):
-            gate = gate[0] if gate.shape[0] else gate.new_empty(dim)            # one row for all
-        _rows_of(gate, "gate", (dim,) if gate.dim() == 1 else (rows, dim), (x.dtype,), dev)
-    if gate_act not in _GATE_ACTS:
-        raise NotImplementedError(f"gate_act must be one of {tuple(_GATE_ACTS)}")
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in (x.dtype, torch.int8):
-        raise NotImplementedError("out_dtype must be that of x or int8")
-    _require(out_scale is None or out_dtype == torch.int8, "out_scale is for int8 output")
-    _require(out_scale is None or float(out_scale) > 0.0, "out_scale must be positive")
-    _require(prenorm or residual_out is None, "residual_out without prenorm")
-    rtype = residual.dtype if residual is not None else residual_dtype or x.dtype
-    if rtype not in half:
-        raise NotImplementedError("the stream is of the type of x or fp32")
-    y = torch.empty((rows, dim), dtype=out_dtype, device=dev)
-    if residual_out is not None:
-        _rows_of(residual_out, "residual_out", (rows, dim), (rtype,), dev)
-        for n, t in (("x", x), ("gate", gate), ("residual", residual), *params):
-            if t is not None and rows:
-                t2 = t if t.dim() == 2 else t[None]
-                same = n == "residual" and t.data_ptr() == residual_out.data_ptr() and t.stride() == residual_out.stride()
-                _require(same or not _overlap(t2, residual_out), f"residual_out overlaps {n}")
-    elif prenorm:
-        residual_out = torch.empty((rows, dim), dtype=rtype, device=dev)
-    dynamic = out_dtype == torch.int8 and out_scale is None
-    scales = torch.empty((rows,), dtype=torch.float32, device=dev) if dynamic else None
-    p = _lib.QaAddNormParams()
-    p.rows, p.dim = rows, dim
-    p.x_type, p.param_type, p.residual_type, p.out_type = (_LM_TYPES[t] for t in (x.dtype, weight.dtype, rtype, out_dtype))
-    p.gate_act, p.dynamic_scale, p.eps = _GATE_ACTS[gate_act], int(dynamic), float(eps)
-    p.scale = 1.0 if vector else float(residual_scale)
-    p.out_scale = 0.0 if out_scale is None else float(out_scale)
-    p.x_row_stride, p.out_row_stride = _row_stride(x), dim
-    p.gate_row_stride = _row_stride(gate) if gate is not None and gate.dim() == 2 else 0
-    p.residual_row_stride = _row_stride(residual) if residual is not None else 0
-    p.residual_out_row_stride = _row_stride(residual_out) if residual_out is not None else 0
-    p.x, p.weight, p.post_weight, p.gate = ptr(x), ptr(weight), ptr(post_weight), ptr(gate)
-    p.scale_vector = ptr(residual_scale) if vector else None
-    p.residual, p.residual_out, p.out, p.scales = ptr(residual), ptr(residual_out), ptr(y), ptr(scales)
-    with torch.cuda.device(dev):
-        st = _lib.lib().qa_add_rmsnorm(ct.byref(p), _lib.current_stream(dev))
-    _lib.check(st, "add_rmsnorm")
-    return y, residual_out, scales
+    return _lm().add_rmsnorm(x, weight, eps, residual, post_weight, gate, gate_act, residual_scale, prenorm, residual_dtype, residual_out,
+                             out_dtype, out_scale)
 
 
 # ----------------------------------------------------------------------------------------------
@@ -984,32 +920,6 @@ class TokenLogprobs(NamedTuple):
     top_tokens: torch.Tensor        # int64 (..., top): which they are, the lowest index first among equal logits
 
 
-def _tokens_of(tokens, shape, device):
-    _require(tokens.is_cuda and tokens.device == device, f"tokens must be on {device}")
-    _require(tokens.dtype in (torch.int32, torch.int64), "tokens must be int32 or int64")
-    _require(tuple(tokens.shape) == tuple(shape), f"tokens must have shape {tuple(shape)}, not {tuple(tokens.shape)}")
-    return tokens.contiguous()
-
-
-def _empty_logprobs(shape, top, device):
-    of = lambda t, *more: torch.empty((*shape, *more), dtype=t, device=device)  # noqa: E731
-    return TokenLogprobs(of(torch.float32), of(torch.float32), of(torch.float32, top), of(torch.int64, top))
-
-
-def _fill_logprobs(p, r, tokens, workspace_bytes, call, what):
-    """The answers' pointers, a workspace, the call."""
-    dev = tokens.device
-    p.token_bytes, p.tokens = tokens.element_size(), ptr(tokens)
-    p.logprobs, p.entropy, p.top_logprobs, p.top_tokens = (ptr(t) for t in r)
-    with torch.cuda.device(dev):
-        p.workspace_bytes = workspace_bytes(ct.byref(p))
-        workspace = torch.empty(p.workspace_bytes, dtype=torch.uint8, device=dev) if p.workspace_bytes else None
-        p.workspace = ptr(workspace)
-        st = call(ct.byref(p), _lib.current_stream(dev))
-    _lib.check(st, what)
-    return r
-
-
 def token_logprobs(logits, tokens, top=0):
     """Of each row of logits: the log probability of a given token, the entropy, and the `top` best alternatives, in one pass
     (qa_token_logprobs).  logits (..., vocab) fp16, bf16 or fp32, contiguous along the last dimension; tokens int32 or int64
@@ -1018,21 +928,7 @@ def token_logprobs(logits, tokens, top=0):
     A negative token asks for nothing and gets 0, so that padded positions add nothing to a sum; one beyond the vocabulary gets NaN.
     Logits of -inf are masked out.  A row whose logits are all -inf, or hold a NaN or +inf, has no distribution: its log
     probabilities and entropy are NaN, and its top_tokens are some indices of the row."""
-    _require(logits.dim() >= 1, "logits must be (..., vocab)")
-    _require_gpu(logits, "logits")
-    shape, vocab = logits.shape[:-1], logits.shape[-1]
-    _require(vocab >= 1, "logits without a vocabulary")
-    _require(0 <= top <= vocab, "top must be between 0 and the vocabulary's size")
-    rows = shape.numel()
-    # (dimensions in front are rows where they lie evenly apart, as logits[:, :-1] of one sequence do; else the call makes a copy)
-    flat = logits.reshape(rows, vocab) if rows else logits.new_empty((0, vocab))
-    _rows_of(flat, "logits", (rows, vocab), (torch.float16, torch.bfloat16, torch.float32), logits.device)
-    tokens = _tokens_of(tokens, shape, logits.device)
-    p = _lib.QaTokenLogprobsParams()
-    p.rows, p.vocab, p.logits_type, p.top = rows, vocab, _LM_TYPES[logits.dtype], int(top)
-    p.row_stride, p.logits = _row_stride(flat), ptr(flat)
-    l = _lib.lib()
-    return _fill_logprobs(p, _empty_logprobs(shape, top, logits.device), tokens, l.qa_token_logprobs_workspace_bytes, l.qa_token_logprobs, "token_logprobs")
+    return TokenLogprobs._make(_lm().token_logprobs(logits, tokens, top))
 
 
 def scaled_mm_token_logprobs(a, b, a_scales, b_scales, tokens, top=0, vocab=None):
@@ -1040,27 +936,4 @@ def scaled_mm_token_logprobs(a, b, a_scales, b_scales, tokens, top=0, vocab=None
     and never written (qa_mm_token_logprobs).  a int8 (M, K) row-major, b int8 (K, N) column-major, scales fp32 with 1 or M / 1 or N
     elements, tokens int32 or int64 (M,), top 0 or 1.  vocab: how many of b's columns are tokens (default all; the others are
     padding).  Returns TokenLogprobs."""
-    _require(a.dtype == torch.int8 and b.dtype == torch.int8, "a and b must be int8")
-    _require(a.dim() == 2 and b.dim() == 2 and a.shape[1] == b.shape[0], "shape mismatch: a (M,K) x b (K,N)")
-    _require_gpu(a, "a")
-    _require(b.device == a.device, "a and b must be on one device")
-    (M, K), N = a.shape, b.shape[1]
-    vocab = N if vocab is None else int(vocab)
-    _require(1 <= vocab <= N, "vocab must be between 1 and the columns of b")
-    _require(K >= 1 and K % 16 == 0, "K must be a multiple of 16")
-    _require(a.stride(1) == 1 and b.stride(0) == 1, "a must be row-major and b column-major")
-    lda, ldw = a.stride(0) if M > 1 else K, b.stride(1) if N > 1 else K
-    _require(lda % 16 == 0 and ldw % 16 == 0, "row strides of a and b must be multiples of 16")
-    for s, n, full in ((a_scales, "a_scales", M), (b_scales, "b_scales", N)):
-        _require(s.dtype == torch.float32 and s.device == a.device and s.is_contiguous(), f"{n} must be contiguous fp32 on {a.device}")
-        _require(s.numel() in (1, full), f"{n} must have 1 or {full} elements")
-    if top not in (0, 1):
-        raise NotImplementedError("scaled_mm_token_logprobs: top is 0 or 1 (more: token_logprobs of the written logits)")
-    tokens = _tokens_of(tokens, (M,), a.device)
-    p = _lib.QaMmTokenLogprobsParams()
-    p.rows, p.vocab, p.k, p.top = M, vocab, K, int(top)
-    p.a_scale_numel, p.w_scale_numel = a_scales.numel(), b_scales.numel()
-    p.lda, p.ldw = lda, ldw
-    p.a, p.w, p.a_scale, p.w_scale = ptr(a), ptr(b), ptr(a_scales), ptr(b_scales)
-    l = _lib.lib()
-    return _fill_logprobs(p, _empty_logprobs((M,), top, a.device), tokens, l.qa_mm_token_logprobs_workspace_bytes, l.qa_mm_token_logprobs, "scaled_mm_token_logprobs")
+    return TokenLogprobs._make(_lm().scaled_mm_token_logprobs(a, b, a_scales, b_scales, tokens, top, vocab))

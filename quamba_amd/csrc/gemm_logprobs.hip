@@ -15,6 +15,8 @@ namespace {
 
 using namespace gemm;
 
+constexpr float kLn2 = 0.693147180559945309f;
+
 struct TilePart {
     float m, s, t;
     int best;              // the lowest column with the value m
@@ -42,63 +44,80 @@ __device__ __forceinline__ float sum_over_columns(float v) {
 
 // A wave's TM x TN blocks: the statistics of each of its rows to parts[row_at + row], the given tokens' logits to `given`.
 // s_lds: column scales, row scales, and the low words of the tokens, of the workgroup's tile.
-template <int TM, int TN, int BM, int BN, class V, int NI, int NJ>
+//
+// All waves are in here at the same time, with nothing for the matrix cores to do: what counts is instructions a value.  With z = s_col * acc
+// (turned over where the row's scale is negative) and c = |s_row| log2(e) an exponent is one fused step, z c - r for r the rounded
+// z_max c; the rest of that rounding, z_max c - r, is exact in one number per row and corrects the sums.  s and t are sums of 2^d and of
+// d 2^d until they leave.  Ten instructions' time a value, four of it the exponential's (fifteen with a difference, a product, a clamp and
+// the best column each on its own).
+// PLAIN: all of the wave's columns are the vocabulary's and none of its rows has a negative scale.
+template <bool PLAIN, bool TOP, int TM, int TN, int BM, int BN, class V, int NI, int NJ>
 __device__ __forceinline__ void tile_stats(const QaMmTokenLogprobsParams& p, V (&acc)[NI][NJ], const float* s_lds, int row_at, int col_at, int m0, int n0, int lane,
                                            TilePart* parts, float* given) {
     using Q = QuadView<V>;
     constexpr int kQuads = TN * 32 / (256 / Q::kRows), kRowBlocks = TM * 32 / Q::kRows;
     static_assert(NI * Q::kQuadsPer == kQuads && NJ == kRowBlocks, "accumulators of another tile");
-    const bool whole = n0 + col_at + TN * 32 <= p.vocab;
-    float s_col[kQuads][4];
-#pragma unroll
-    for (int u = 0; u < kQuads; ++u) {
-        const float4 v = *reinterpret_cast<const float4*>(s_lds + col_at + Q::column_of(u, lane));
-        s_col[u][0] = v.x; s_col[u][1] = v.y; s_col[u][2] = v.z; s_col[u][3] = v.w;
-    }
+    const int columns = p.vocab - (n0 + col_at);           // of the vocabulary, from this wave's first one on
 #pragma unroll
     for (int b = 0; b < kRowBlocks; ++b) {
         const int row = row_at + b * Q::kRows + Q::row_of(lane);
-        const float s_row = s_lds[BN + row];
+        const float s_row = s_lds[BN + row], size = PLAIN ? s_row : fabsf(s_row), sign = s_row < 0.0f ? -1.0f : 1.0f;
         const int token = reinterpret_cast<const int*>(s_lds)[BN + BM + row] - (n0 + col_at);      // its column among the wave's
-        float v[kQuads][4], most = kLowest;
+        float z[kQuads][4], most = kLowest;
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u) {
+            const float4 s_quad = *reinterpret_cast<const float4*>(s_lds + col_at + Q::column_of(u, lane));
+            const float s_col[4] = {s_quad.x, s_quad.y, s_quad.z, s_quad.w};
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                z[u][t] = s_col[t] * Q::value(acc, u, b, t);
+                if constexpr (!PLAIN) z[u][t] = Q::column_of(u, lane) + t < columns ? sign * z[u][t] : -__builtin_inff();
+                most = fmaxf(most, z[u][t]);
+            }
+        }
+        most = most_over_columns<Q::kRows>(most);
+        if (!PLAIN && columns <= 0) most = 0.0f;
+        const float c = size * kLog2e, r = most * c, rest = __builtin_fmaf(most, c, -r);
+        float s = 0.0f, w = 0.0f;
 #pragma unroll
         for (int u = 0; u < kQuads; ++u)
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                v[u][t] = s_row * (s_col[u][t] * Q::value(acc, u, b, t));
-                if (!whole && n0 + col_at + Q::column_of(u, lane) + t >= p.vocab) v[u][t] = -__builtin_inff();
-                most = fmaxf(most, v[u][t]);
+                float d = __builtin_fmaf(z[u][t], c, -r);
+                if constexpr (!PLAIN) d = fmaxf(d, -200.0f);           // (its power is 0, and so is the product)
+                const float e = __builtin_amdgcn_exp2f(d);
+                s += e;
+                w = __builtin_fmaf(d, e, w);
             }
-        most = most_over_columns<Q::kRows>(most);
-        RowStats r = {most, 0.0f, 0.0f};
-#pragma unroll
-        for (int u = 0; u < kQuads; ++u)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) r.add(v[u][t]);
-        r.s = sum_over_columns<Q::kRows>(r.s);
-        r.t = sum_over_columns<Q::kRows>(r.t);
-        uint32_t best = 0xffffffffu;
-        if (p.top) {
+        s = sum_over_columns<Q::kRows>(s);
+        w = sum_over_columns<Q::kRows>(w);
+        const float f = __builtin_amdgcn_exp2f(-rest), m = PLAIN || columns > 0 ? fmaxf(size * most, kLowest) : kLowest;
+        uint32_t best = 0;
+        if constexpr (TOP) {
+            // (of the rounded logits, as they would be written)
+            best = 0xffffffffu;
 #pragma unroll
             for (int u = kQuads - 1; u >= 0; --u)
 #pragma unroll
                 for (int t = 3; t >= 0; --t)
-                    if (v[u][t] == most) best = Q::column_of(u, lane) + t;
-            best = over_columns<Q::kRows>(best, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+                    if (size * z[u][t] == m) best = Q::column_of(u, lane) + t;
+            best = over_columns<Q::kRows>(best, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+            if (best == 0xffffffffu) best = 0;             // (a row of NaNs)
         }
-        // (a row of NaNs has no such column)
-        if (lane < Q::kRows) parts[row] = {r.m, r.s, r.t, static_cast<int>(n0 + col_at + (best == 0xffffffffu ? 0 : best))};
+        if (lane < Q::kRows) parts[row] = {m, s * f, (w - rest * s) * f * kLn2, n0 + col_at + static_cast<int>(best)};
         if (__builtin_amdgcn_ballot_w64(token >= 0 && token < TN * 32)) {
+            float v = 0.0f;
 #pragma unroll
             for (int u = 0; u < kQuads; ++u)
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    if (token == Q::column_of(u, lane) + t && m0 + row < p.rows && n0 + col_at + token < p.vocab) given[m0 + row] = v[u][t];
+                for (int t = 0; t < 4; ++t) v = token == Q::column_of(u, lane) + t ? z[u][t] : v;
+            const int by = Q::kRows == 16 ? token >> 2 & 3 : token >> 2 & 1;                       // the lanes that hold it
+            if (token >= 0 && token < min(columns, TN * 32) && lane / Q::kRows == by && m0 + row < p.rows) given[m0 + row] = size * v;
         }
     }
 }
 
-template <int TM, int TN, int WGM, int WGN, int STAGES>
+template <int TM, int TN, int WGM, int WGN, int STAGES, bool TOP>
 __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmTokenLogprobsParams p) {
     using C = Cfg<TM, TN, WGM, WGN, STAGES>;
     constexpr int BM = C::kBM, BN = C::kBN, WAVES = C::kWaves;
@@ -132,8 +151,16 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmT
     auto finish = [&](auto& acc) {
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         __syncthreads();
-        tile_stats<TM, TN, BM, BN>(p, acc, reinterpret_cast<const float*>(lds + C::kLdsBytes), wm * TM * 32, wn * TN * 32, m0, n0, lane, parts + wn * BM,
-                                   reinterpret_cast<float*>(out + static_cast<int64_t>(p.rows) * tiles_n));
+        const float* const s_lds = reinterpret_cast<const float*>(lds + C::kLdsBytes);
+        float* const given = reinterpret_cast<float*>(out + static_cast<int64_t>(p.rows) * tiles_n);
+        bool negative = false;
+        for (int row = lane; row < TM * 32; row += 64) negative |= s_lds[BN + wm * TM * 32 + row] < 0.0f;
+        const bool plain = p.vocab - (n0 + wn * TN * 32) >= TN * 32 && !__builtin_amdgcn_ballot_w64(negative);
+        auto stats = [&](auto plain_c) __attribute__((always_inline)) {
+            tile_stats<decltype(plain_c)::value, TOP, TM, TN, BM, BN>(p, acc, s_lds, wm * TM * 32, wn * TN * 32, m0, n0, lane, parts + wn * BM, given);
+        };
+        if (plain) stats(std::true_type{});
+        else stats(std::false_type{});
         __syncthreads();
         for (int row = tid; row < BM; row += C::kThreads) {
             if (m0 + row >= p.rows) break;
@@ -218,33 +245,56 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmT
     }
 }
 
-// Rows' parts, tiles_n of them each: kThreads / at_once threads share a row, at_once rows a workgroup.
-constexpr int kJoinThreads = 256;
-__global__ __launch_bounds__(kJoinThreads) void mm_token_logprobs_join_kernel(QaMmTokenLogprobsParams p, int tiles_n, int at_once) {
-    __shared__ TilePart s_part[kJoinThreads];
-    const int r = threadIdx.x % at_once, first = threadIdx.x / at_once, step = kJoinThreads / at_once;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * at_once + r;
+// The parts of ROWS rows, tiles_n each, by one workgroup.  A part is 16 bytes and a row's parts lie p.rows of them apart, so the rows of a
+// workgroup are what its loads have in one piece; with few rows all threads go to one.  What a thread holds of a row meets through
+// lane exchanges (lane l has row l % ROWS), then over the waves.
+constexpr int kJoinThreads = 256, kJoinAhead = 4;
+template <int ROWS>
+__global__ __launch_bounds__(kJoinThreads) void mm_token_logprobs_join_kernel(QaMmTokenLogprobsParams p, int tiles_n) {
+    __shared__ TilePart s_part[kJoinThreads / 64][ROWS];
+    constexpr int kStep = kJoinThreads / ROWS;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = threadIdx.x % ROWS;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + r, from = min(row, static_cast<int64_t>(p.rows) - 1);
     const TilePart* const parts = static_cast<const TilePart*>(p.workspace);
     RowStats all;
     all.clear();
-    TilePart best = {-__builtin_inff(), 0.0f, 0.0f, 0x7fffffff};
-    auto take = [&](const TilePart& o) {
-        if (o.m > best.m || (o.m == best.m && o.best < best.best)) best = o;
-        all.join({o.m, o.s, o.t});
-    };
-    if (row < p.rows)
-        for (int i = first; i < tiles_n; i += step) take(parts[i * static_cast<int64_t>(p.rows) + row]);
-    for (int half = step / 2; half > 0; half /= 2) {
-        __syncthreads();
-        s_part[threadIdx.x] = {all.m, all.s, all.t, best.best};
-        __syncthreads();
-        if (first < half) {
-            const TilePart o = s_part[threadIdx.x + half * at_once];
-            best.m = all.m;                                // (an empty side has the lowest number and no column)
-            take(o);
+    float best_m = -__builtin_inff();
+    int best = 0x7fffffff;
+    auto take = [&](float m, float s, float t, int column) {
+        if (m > best_m || (m == best_m && column < best)) {
+            best_m = m;
+            best = column;
         }
+        all.join({m, s, t});
+    };
+    for (int i = threadIdx.x / ROWS; i < tiles_n; i += kJoinAhead * kStep) {
+        TilePart o[kJoinAhead];
+#pragma unroll
+        for (int j = 0; j < kJoinAhead; ++j) o[j] = parts[min(i + j * kStep, tiles_n - 1) * static_cast<int64_t>(p.rows) + from];
+#pragma unroll
+        for (int j = 0; j < kJoinAhead; ++j)
+            if (i + j * kStep < tiles_n) take(o[j].m, o[j].s, o[j].t, o[j].best);
     }
-    if (first != 0 || row >= p.rows) return;
+    auto meet = [&](auto mask_c) {
+        constexpr int MASK = decltype(mask_c)::value;
+        if constexpr (MASK >= ROWS) {
+            auto other = [&](float v) { return __uint_as_float(word_across<MASK>(__float_as_uint(v), lane)); };
+            // (an empty side has the lowest number and no column)
+            const float m = other(all.m), s = other(all.s), t = other(all.t);
+            take(m, s, t, static_cast<int>(word_across<MASK>(static_cast<uint32_t>(best), lane)));
+        }
+    };
+    meet(std::integral_constant<int, 32>{});
+    meet(std::integral_constant<int, 16>{});
+    meet(std::integral_constant<int, 8>{});
+    meet(std::integral_constant<int, 4>{});
+    meet(std::integral_constant<int, 2>{});
+    meet(std::integral_constant<int, 1>{});
+    if (lane < ROWS) s_part[wave][lane] = {all.m, all.s, all.t, best};
+    __syncthreads();
+    if (threadIdx.x >= ROWS || row >= p.rows) return;
+#pragma unroll
+    for (int w = 1; w < kJoinThreads / 64; ++w) take(s_part[w][r].m, s_part[w][r].s, s_part[w][r].t, s_part[w][r].best);
     const int64_t token = token_of(p.tokens, p.token_bytes, row);
     float lp = token < 0 ? 0.0f : __builtin_nanf("");
     if (token >= 0 && token < p.vocab) lp = all.logprob(reinterpret_cast<const float*>(parts + static_cast<int64_t>(p.rows) * tiles_n)[row]);
@@ -252,18 +302,37 @@ __global__ __launch_bounds__(kJoinThreads) void mm_token_logprobs_join_kernel(Qa
     p.entropy[row] = all.s > 0.0f ? all.entropy() : __builtin_nanf("");
     if (p.top) {
         p.top_logprobs[row] = all.logprob(all.m);
-        p.top_tokens[row] = best.best;
+        p.top_tokens[row] = best;
     }
 }
 
-// Rows and columns of a tile.
+// The tiles, and what a launch of them takes, in us with `units` of 128 codes of K: fixed and, for each round of one tile per CU,
+// per_round + per_unit x units (the launch of the join is in it).  The fastest by that is taken; up to 64 rows only tiles of 64, which
+// read the weights at the memory's rate and nothing for rows that are not there.  Measured over 1 .. 16384 rows, 1000 .. 256000 columns
+// and K from 768 to 4096 the choice is the fastest of the six but for 1.5 % of the time (rows x vocabulary x K, us by the tiles in the
+// order below): 64 x 16000 x 2560 13.1, 15.0, 16.0, 20.7, 32.5, 36.2; 64 x 50280 x 2560 34.4, 30.4, 40.5, 33.8, 44.9, 48.1; 1000 x 4000 x
+// 2560 25.3, 21.3, 18.2, 24.2, 34.4, 37.4; 128 x 50280 x 2560 (the third on) 43.7, 36.6, 45.3, 48.4; 256 x 50280 x 2560 70.9, 57.8, 49.1,
+// 51.0; 16000 x 16000 x 768 419, 349, 360, 281, 238, 227; 16384 x 50280 x 2560 (the last two) 1667, 1554.
 struct Tile {
     int bm, bn;
+    float fixed, per_round, per_unit;
 };
-Tile tile_of(int rows, int vocab) {
-    if (rows <= 64) return {64, 64};
-    if (rows <= 128) return {128, 128};
-    return {256, 256};
+constexpr Tile kTiles[] = {{64, 64, 6.0f, 0.3f, 0.2f},    {64, 128, 6.0f, 1.0f, 0.31f},  {128, 128, 4.0f, 1.6f, 0.56f},
+                           {128, 256, 4.0f, 2.6f, 0.84f}, {256, 256, 5.0f, 3.6f, 1.45f}, {256, 320, 5.0f, 4.2f, 1.75f}};
+int tile_of(const QaMmTokenLogprobsParams& p) {
+    const int cus = compute_units(), candidates = p.rows <= 64 ? 2 : 6, units = (p.k + kBK - 1) / kBK;
+    int best = 0;
+    float best_us = 1e30f;
+    for (int i = 0; i < candidates; ++i) {
+        const Tile& t = kTiles[i];
+        const int64_t tiles = static_cast<int64_t>((p.rows + t.bm - 1) / t.bm) * ((p.vocab + t.bn - 1) / t.bn);
+        const float us = t.fixed + static_cast<float>((tiles + cus - 1) / cus) * (t.per_round + t.per_unit * units);
+        if (us < best_us) {
+            best = i;
+            best_us = us;
+        }
+    }
+    return best;
 }
 
 int check(const QaMmTokenLogprobsParams& p) {
@@ -274,25 +343,27 @@ int check(const QaMmTokenLogprobsParams& p) {
 }
 
 int64_t workspace_bytes(const QaMmTokenLogprobsParams& p) {
-    const Tile tile = tile_of(p.rows, p.vocab);
-    const int64_t tiles_n = (p.vocab + tile.bn - 1) / tile.bn;
+    const int64_t bn = kTiles[tile_of(p)].bn, tiles_n = (p.vocab + bn - 1) / bn;
     return p.rows * (tiles_n * static_cast<int64_t>(sizeof(TilePart)) + static_cast<int64_t>(sizeof(float)));
 }
 
-template <int TM, int TN, int WGM, int WGN, int STAGES>
+template <int TILE, int TM, int TN, int WGM, int WGN, int STAGES>
 int launch(const QaMmTokenLogprobsParams& p, hipStream_t stream) {
     using C = Cfg<TM, TN, WGM, WGN, STAGES>;
+    static_assert(C::kBM == kTiles[TILE].bm && C::kBN == kTiles[TILE].bn, "the tile of the table");
     const int tiles_n = (p.vocab + C::kBN - 1) / C::kBN;
     const int64_t tiles = static_cast<int64_t>((p.rows + C::kBM - 1) / C::kBM) * tiles_n;
     if (tiles > 0x7fffffffLL) return QA_ERR_SHAPE;
-    auto kernel = mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES>;
+    auto kernel = p.top ? mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES, true> : mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES, false>;
     constexpr int kLds = C::kLdsBytes + TileScales<C::kBM, C::kBN, C::kWaves>::kBytes + C::kBM * 4;
     static_assert(kLds <= 160 * 1024, "LDS of a CU");
     if (kLds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) return check_launch();
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(C::kThreads), kLds, stream, p);
     if (const int status = check_launch()) return status;
-    const int at_once = p.rows >= 4096 ? 16 : 1;
-    hipLaunchKernelGGL(mm_token_logprobs_join_kernel, dim3(static_cast<unsigned>((p.rows + at_once - 1) / at_once)), dim3(kJoinThreads), 0, stream, p, tiles_n, at_once);
+    const int at_once = p.rows >= 4096 ? 16 : p.rows >= 512 ? 4 : 1;
+    const dim3 grid(static_cast<unsigned>((p.rows + at_once - 1) / at_once));
+    auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kJoinThreads), 0, stream, p, tiles_n); };
+    at_once == 16 ? join(mm_token_logprobs_join_kernel<16>) : at_once == 4 ? join(mm_token_logprobs_join_kernel<4>) : join(mm_token_logprobs_join_kernel<1>);
     return check_launch();
 }
 
@@ -320,8 +391,12 @@ extern "C" int qa_mm_token_logprobs(const QaMmTokenLogprobsParams* p, void* stre
     if (static_cast<int64_t>(p->rows) * p->lda >= 0x70000000LL || static_cast<int64_t>(p->vocab) * p->ldw >= 0x70000000LL) return QA_ERR_SHAPE;
     if (!aligned16(p->workspace) || p->workspace_bytes < workspace_bytes(*p)) return QA_ERR_SCRATCH;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
-    const Tile tile = tile_of(p->rows, p->vocab);
-    if (tile.bm == 64) return launch<1, 1, 2, 2, 4>(*p, stream);
-    if (tile.bm == 128) return launch<2, 1, 2, 4, 4>(*p, stream);
-    return launch<4, 2, 2, 4, 2>(*p, stream);
+    switch (tile_of(*p)) {
+        case 0: return launch<0, 1, 1, 2, 2, 3>(*p, stream);
+        case 1: return launch<1, 1, 2, 2, 2, 3>(*p, stream);
+        case 2: return launch<2, 2, 1, 2, 4, 4>(*p, stream);
+        case 3: return launch<3, 2, 2, 2, 4, 3>(*p, stream);
+        case 4: return launch<4, 4, 2, 2, 4, 2>(*p, stream);
+        default: return launch<5, 2, 5, 4, 2, 2>(*p, stream);
+    }
 }

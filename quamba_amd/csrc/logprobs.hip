@@ -1,12 +1,13 @@
 // Log probabilities of given tokens, entropies and the best alternatives of rows of logits (qa_token_logprobs).
 //
 // One pass over the logits, bound by memory while the vector units keep up: a value is converted, joins a maximum of a batch,
-// and costs an exponential and five operations more (RowStats); a lane raises its maximum once a batch of kUnroll loads, not
-// once a value.  The best entries stay sorted over the lanes of a wave, and a batch in which no value is above the last of them is
-// passed over with one comparison per lane.
+// and costs an exponential and five operations more (RowStats); a lane raises its maximum once a batch of loads, not
+// once a value.
 //
 // A workgroup of four waves takes a segment of a row, whole rows when there are many; the parts of a cut row go to the workspace
-// and a second launch joins them.
+// and a second launch joins them.  With few rows a segment is one batch, and what costs is not the bytes but what happens one after the
+// other: there the best entries are picked out of the registers by a bound (pick).  In a longer segment a wave keeps its own, and loads in
+// which no value is above the last of them are passed over with one comparison per lane (BestOfBatches).
 #include "row_stats.hpp"
 
 #include <algorithm>
@@ -17,21 +18,23 @@ namespace {
 
 constexpr int kWaves = 4, kUnroll = 4;
 constexpr int kMaxTop = 64, kMaxSegments = 64;
+constexpr int kCandidates = 256;
+constexpr uint32_t kNoIndex = 0xffffffffu;               // of a lane's place without a value
 
 struct Part {
     float m, s, t, reserved;
 };
 
-// values of a workgroup's batch
-int batch_values(int type) { return kWaves * 64 * kUnroll * (type == QA_LM_F32 ? 4 : 8); }
-
-// segments a row is cut into
-int segments_of(int rows, int vocab, int type) {
-    const int batches = (vocab + batch_values(type) - 1) / batch_values(type);
-    const int wanted = static_cast<int>((4LL * compute_units() + rows - 1) / rows);
-    const int segments = std::min(std::min(batches, wanted), kMaxSegments);
-    const int each = (batches + segments - 1) / segments;
-    return (batches + each - 1) / each;
+// How the rows are cut: segments of a row, batches of a segment, loads of a lane in a batch.
+struct Cut {
+    int segments, batches, loads;
+};
+Cut cut_of(int rows, int vocab, int type) {
+    const int load = kWaves * 64 * (type == QA_LM_F32 ? 4 : 8), short_batches = (vocab + load - 1) / load, batches = (vocab + load * kUnroll - 1) / (load * kUnroll);
+    const int wanted = static_cast<int>(std::min<int64_t>((4LL * compute_units() + rows - 1) / rows, kMaxSegments));
+    if (short_batches <= wanted) return {short_batches, 1, 1};
+    const int each = (batches + std::min(batches, wanted) - 1) / std::min(batches, wanted);
+    return {(batches + each - 1) / each, each, kUnroll};
 }
 
 __device__ __forceinline__ float logit_at(const QaTokenLogprobsParams& p, int64_t row, int64_t i) {
@@ -51,75 +54,158 @@ __device__ __forceinline__ void answer(const QaTokenLogprobsParams& p, int64_t r
         p.entropy[row] = r.s > 0.0f ? r.entropy() : __builtin_nanf("");
     }
     if (lane < p.top) {
+        // (a row with NaNs may have fewer entries than that)
         p.top_logprobs[row * p.top + lane] = r.logprob(value_of(best));
-        p.top_tokens[row * p.top + lane] = index_of(best);
+        p.top_tokens[row * p.top + lane] = best ? index_of(best) : 0;
     }
 }
 
-template <class T, bool WIDE, bool TOP>
+struct Candidates {
+    Entry at[kCandidates];
+    uint32_t keys[kWaves][64];
+    int count;
+};
+
+// The candidates that a workgroup has put together, by one wave.
+__device__ __forceinline__ void take_candidates(BestEntries& best, const Candidates& c, int count, int top, int lane) {
+    for (int i = 0; i < count; i += 64) best.offer(i + lane < count ? c.at[i + lane] : 0, top, lane);
+}
+
+// The best `top` of the workgroup's values: `visit(f)` calls f(value, index) for each value of a lane, `most` is the largest of them.
+// The top-th largest of the lanes' largest values is a bound that `top` values or more reach and hardly more than that do: those are put
+// together in LDS (in any order) and one wave sorts them.  Where more come than there is room for - equal values, or as many
+// alternatives as lanes - every wave keeps its own best instead and one wave merges them.  The result is wave 0's.
+template <class Visit>
+__device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, Candidates& c, Entry (&lists)[kWaves][64], int wave, int lane) {
+    if (threadIdx.x == 0) c.count = 0;
+    c.keys[wave][lane] = sort_wave(key_of(most), lane);
+    __syncthreads();
+    const uint32_t all = merge_waves(merge_waves(c.keys[0][lane], c.keys[1][lane], lane), merge_waves(c.keys[2][lane], c.keys[3][lane], lane), lane);
+    const float bound = value_of_key(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(all), top - 1)));
+    if (__builtin_amdgcn_ballot_w64(most >= bound)) {
+        visit([&](float v, uint32_t index) __attribute__((always_inline)) {
+            if (v >= bound && index != kNoIndex) {
+                const int at = atomicAdd(&c.count, 1);
+                if (at < kCandidates) c.at[at] = entry_of(v, index);
+            }
+        });
+    }
+    __syncthreads();
+    const int count = c.count;
+    BestEntries best;
+    best.clear();
+    // (a NaN reaches no bound: where nothing else is left, it is one of the waves' own best)
+    if (count <= kCandidates && count >= top) {
+        if (wave == 0) take_candidates(best, c, count, top, lane);
+        return best;
+    }
+    visit([&](float v, uint32_t index) __attribute__((always_inline)) { best.offer(index == kNoIndex ? 0 : entry_of(v, index), top, lane); });
+    lists[wave][lane] = best.mine;
+    __syncthreads();
+    if (wave == 0)
+        for (int w = 1; w < kWaves; ++w) best.mine = merge_waves(best.mine, lists[w][lane], lane);
+    return best;
+}
+
+// ONE: the segment is one batch
+template <class T, bool WIDE, bool TOP, bool ONE, int LOADS>
 __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogprobsParams p, int segments, int batches_each) {
     constexpr int V = 16 / sizeof(T);                      // values a load
     __shared__ Part s_part[kWaves];
     __shared__ Entry s_best[TOP ? kWaves : 1][64];
+    __shared__ std::conditional_t<TOP && ONE, Candidates, int> s_candidates;
+    __shared__ Entry s_waiting[TOP && !ONE ? kWaves : 1][128];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = blockIdx.x / segments;
     const int segment = blockIdx.x % segments;
     const T* const logits = static_cast<const T*>(p.logits) + row * p.row_stride;
     const int vectors = p.vocab / V, rest = p.vocab - vectors * V;
-    const int first = segment * batches_each, end = min(first + batches_each, (vectors + kWaves * 64 * kUnroll - 1) / (kWaves * 64 * kUnroll));
+    const int first = segment * batches_each, end = ONE ? first + 1 : min(first + batches_each, (vectors + kWaves * 64 * LOADS - 1) / (kWaves * 64 * LOADS));
     const float none = -__builtin_inff();
 
+    // fewer than V values behind the last whole load: one each in the first lanes of the last segment
+    const int rest_at = vectors * V + lane;
+    const bool has_rest = segment == segments - 1 && wave == 0 && lane < rest;
+    float rest_v = none;
+    if (has_rest) rest_v = static_cast<float>(logits[rest_at]);
     RowStats r;
     r.clear();
     BestEntries best;
     best.clear();
+    BestOfBatches run;
+    if constexpr (TOP && !ONE) run.clear(s_waiting[wave]);
     for (int b = first; b < end; ++b) {
-        Raw<T, V> raw[kUnroll];
-        int at[kUnroll];
+        Raw<T, V> raw[LOADS];
+        int at[LOADS];
+        float v[LOADS][V], most_of[LOADS], most = none;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            at[u] = ((b * kUnroll + u) * kWaves + wave) * 64 + lane;
-            raw[u].template load<WIDE>(logits + static_cast<int64_t>(min(at[u], vectors - 1)) * V);
+        for (int u = 0; u < LOADS; ++u) {
+            at[u] = ((b * LOADS + u) * kWaves + wave) * 64 + lane;
+            if (!ONE || vectors > 0) raw[u].template load<WIDE>(logits + static_cast<int64_t>(min(at[u], vectors - 1)) * V);
         }
-        float v[kUnroll][V], most = none;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
+        for (int u = 0; u < LOADS; ++u) {
+            most_of[u] = none;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 v[u][j] = at[u] < vectors ? raw[u].get(j) : none;
-                most = fmaxf(most, v[u][j]);
+                most_of[u] = fmaxf(most_of[u], v[u][j]);
             }
+            most = fmaxf(most, most_of[u]);
+        }
+        if constexpr (ONE) most = fmaxf(most, rest_v);
         r.raise(fmaxf(r.m, most));
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
+        for (int u = 0; u < LOADS; ++u)
 #pragma unroll
             for (int j = 0; j < V; ++j) r.add(v[u][j]);
-        if constexpr (TOP) {
-            // (what a wave has seen has lower indices than what comes: an equal value does not come in)
-            if (best.last == 0 || __builtin_amdgcn_ballot_w64(most > value_of(best.last))) {
+        if constexpr (TOP && ONE) {
+            best = pick([&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u)
+                for (int u = 0; u < LOADS; ++u)
 #pragma unroll
-                    for (int j = 0; j < V; ++j) best.offer(at[u] < vectors ? entry_of(v[u][j], at[u] * V + j) : 0, p.top, lane);
+                    for (int j = 0; j < V; ++j) f(v[u][j], at[u] < vectors ? static_cast<uint32_t>(at[u] * V + j) : kNoIndex);
+                f(rest_v, has_rest ? static_cast<uint32_t>(rest_at) : kNoIndex);
+            }, most, p.top, s_candidates, s_best, wave, lane);
+        } else if constexpr (TOP) {
+            auto each = [&](auto comes_in) __attribute__((always_inline)) {
+#pragma unroll
+                for (int u = 0; u < LOADS; ++u) {
+                    if (!__builtin_amdgcn_ballot_w64(comes_in(most_of[u]))) continue;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) run.put(comes_in(v[u][j]) && at[u] < vectors, v[u][j], at[u] * V + j, p.top, lane);
+                }
+            };
+            // (what a wave has seen has lower indices than what comes: later an equal value does not come in)
+            if (b == first) {
+                run.first(most, p.top, lane);
+                const float reach = run.bound;
+                each([&](float value) { return value >= reach; });
+            } else {
+                each([&](float value) { return value > run.bound; });
             }
         }
     }
-    if (segment == segments - 1 && wave == 0 && rest) {    // fewer than V values behind the last whole load
-        const int i = vectors * V + lane;
-        const float v = lane < rest ? static_cast<float>(logits[i]) : none;
-        r.raise(fmaxf(r.m, v));
-        r.add(v);
-        if constexpr (TOP) best.offer(lane < rest ? entry_of(v, i) : 0, p.top, lane);
+    if (ONE) {
+        r.add(rest_v);
+    } else if (segment == segments - 1 && wave == 0 && rest) {
+        r.raise(fmaxf(r.m, rest_v));
+        r.add(rest_v);
+        if constexpr (TOP) run.put(has_rest && rest_v > run.bound, rest_v, rest_at, p.top, lane);
+    }
+    if constexpr (TOP && !ONE) {
+        run.finish(p.top, lane);
+        best = run.best;
     }
     r = wave_stats(r);
     if (lane == 0) s_part[wave] = {r.m, r.s, r.t, 0.0f};
-    if constexpr (TOP) s_best[wave][lane] = best.mine;
+    if constexpr (TOP && !ONE) s_best[wave][lane] = best.mine;
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) {
         r.join({s_part[w].m, s_part[w].s, s_part[w].t});
-        if constexpr (TOP) best.mine = merge_waves(best.mine, s_best[w][lane], lane);
+        if constexpr (TOP && !ONE) best.mine = merge_waves(best.mine, s_best[w][lane], lane);
     }
     if (segments == 1) {
         answer(p, row, r, best.mine, lane);
@@ -130,26 +216,36 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
     if (TOP && lane < p.top) reinterpret_cast<Entry*>(parts + static_cast<int64_t>(p.rows) * segments)[static_cast<int64_t>(blockIdx.x) * p.top + lane] = best.mine;
 }
 
-// a row's segments, by one wave
-__global__ __launch_bounds__(64) void token_logprobs_join_kernel(QaTokenLogprobsParams p, int segments) {
+// A row's segments.  Their best entries, each segment's in order, are shared out among the waves: whole lists, merged as they are, or with
+// few alternatives 64 entries at a time, sorted first.
+template <bool TOP>
+__global__ __launch_bounds__(64 * kWaves) void token_logprobs_join_kernel(QaTokenLogprobsParams p, int segments) {
     static_assert(kMaxSegments <= 64, "a lane for each");
-    const int lane = threadIdx.x;
+    __shared__ Entry s_best[TOP ? kWaves : 1][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = blockIdx.x;
-    const Part* const parts = static_cast<const Part*>(p.workspace);
+    const Part* const parts = static_cast<const Part*>(p.workspace) + row * segments;
     RowStats r;
     r.clear();
-    if (lane < segments) {
-        const Part part = parts[row * segments + lane];
-        r = {part.m, part.s, part.t};
+    if (lane < segments) r = {parts[lane].m, parts[lane].s, parts[lane].t};
+    Entry best = 0;
+    if constexpr (TOP) {
+        const Entry* const from = reinterpret_cast<const Entry*>(static_cast<const Part*>(p.workspace) + static_cast<int64_t>(p.rows) * segments) + row * segments * p.top;
+        if (p.top >= 16) {
+            for (int i = wave; i < segments; i += kWaves) best = merge_waves(best, lane < p.top ? from[i * p.top + lane] : Entry(0), lane);
+        } else {
+            const int count = segments * p.top;
+            for (int i = wave * 64; i < count; i += kWaves * 64) best = merge_waves(best, sort_wave(i + lane < count ? from[i + lane] : Entry(0), lane), lane);
+        }
+        s_best[wave][lane] = best;
+        __syncthreads();
     }
-    r = wave_stats(r);
-    BestEntries best;
-    best.clear();
-    if (p.top) {
-        const Entry* const from = reinterpret_cast<const Entry*>(parts + static_cast<int64_t>(p.rows) * segments) + row * segments * p.top;
-        for (int i = 0; i < segments * p.top; i += 64) best.offer(i + lane < segments * p.top ? from[i + lane] : 0, p.top, lane);
+    if (wave != 0) return;
+    if constexpr (TOP) {
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) best = merge_waves(best, s_best[w][lane], lane);
     }
-    answer(p, row, r, best.mine, lane);
+    answer(p, row, wave_stats(r), best, lane);
 }
 
 int check(const QaTokenLogprobsParams& p) {
@@ -161,22 +257,27 @@ int check(const QaTokenLogprobsParams& p) {
 }
 
 int64_t workspace_bytes(const QaTokenLogprobsParams& p) {
-    const int segments = segments_of(p.rows, p.vocab, p.logits_type);
-    return segments == 1 ? 0 : static_cast<int64_t>(p.rows) * segments * (static_cast<int64_t>(sizeof(Part)) + p.top * static_cast<int64_t>(sizeof(Entry)));
+    const int64_t segments = cut_of(p.rows, p.vocab, p.logits_type).segments;
+    return segments == 1 ? 0 : p.rows * segments * (static_cast<int64_t>(sizeof(Part)) + p.top * static_cast<int64_t>(sizeof(Entry)));
 }
 
 template <class T>
 int launch(const QaTokenLogprobsParams& p, hipStream_t stream) {
-    const int segments = segments_of(p.rows, p.vocab, p.logits_type);
-    const int batches = (p.vocab + batch_values(p.logits_type) - 1) / batch_values(p.logits_type);
+    const Cut cut = cut_of(p.rows, p.vocab, p.logits_type);
     const bool wide = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.row_stride * static_cast<int64_t>(sizeof(T)) % 16 == 0;
-    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.rows) * segments)), block(64 * kWaves);
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, segments, (batches + segments - 1) / segments); };
-    if (wide) p.top ? go(token_logprobs_kernel<T, true, true>) : go(token_logprobs_kernel<T, true, false>);
-    else p.top ? go(token_logprobs_kernel<T, false, true>) : go(token_logprobs_kernel<T, false, false>);
-    if (segments > 1) {
+    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.rows) * cut.segments)), block(64 * kWaves);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, cut.segments, cut.batches); };
+    auto of_wide = [&](auto wide_c) {
+        constexpr bool WIDE = decltype(wide_c)::value;
+        if (cut.loads == 1) p.top ? go(token_logprobs_kernel<T, WIDE, true, true, 1>) : go(token_logprobs_kernel<T, WIDE, false, true, 1>);
+        else if (cut.batches == 1) p.top ? go(token_logprobs_kernel<T, WIDE, true, true, kUnroll>) : go(token_logprobs_kernel<T, WIDE, false, true, kUnroll>);
+        else p.top ? go(token_logprobs_kernel<T, WIDE, true, false, kUnroll>) : go(token_logprobs_kernel<T, WIDE, false, false, kUnroll>);
+    };
+    wide ? of_wide(std::true_type{}) : of_wide(std::false_type{});
+    if (cut.segments > 1) {
         if (const int status = check_launch()) return status;
-        hipLaunchKernelGGL(token_logprobs_join_kernel, dim3(p.rows), dim3(64), 0, stream, p, segments);
+        auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(p.rows), block, 0, stream, p, cut.segments); };
+        p.top ? join(token_logprobs_join_kernel<true>) : join(token_logprobs_join_kernel<false>);
     }
     return check_launch();
 }

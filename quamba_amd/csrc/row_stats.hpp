@@ -55,15 +55,14 @@ __device__ __forceinline__ RowStats wave_stats(RowStats r) {
 
 // An entry of a row as one number: larger values first, of equal ones (-0 and 0 are equal) the lower index.  0: no entry.  A NaN ranks with -inf.
 typedef uint64_t Entry;
-__device__ __forceinline__ Entry entry_of(float value, uint32_t index) {
+__device__ __forceinline__ uint32_t key_of(float value) {
     const float v = value == value ? value + 0.0f : -__builtin_inff();
-    const uint32_t u = __float_as_uint(v), key = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
-    return static_cast<uint64_t>(key) << 32 | ~index;
+    const uint32_t u = __float_as_uint(v);
+    return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float value_of(Entry e) {
-    const uint32_t key = static_cast<uint32_t>(e >> 32);
-    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
-}
+__device__ __forceinline__ float value_of_key(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+__device__ __forceinline__ Entry entry_of(float value, uint32_t index) { return static_cast<uint64_t>(key_of(value)) << 32 | ~index; }
+__device__ __forceinline__ float value_of(Entry e) { return value_of_key(static_cast<uint32_t>(e >> 32)); }
 __device__ __forceinline__ uint32_t index_of(Entry e) { return ~static_cast<uint32_t>(e); }
 
 __device__ __forceinline__ Entry entry_of_lane(Entry e, int lane) {
@@ -92,23 +91,26 @@ __device__ __forceinline__ uint32_t word_across(uint32_t v, int lane) {
     else return word_across<32>(word_across<31>(v, lane), lane);
 }
 template <int MASK>
+__device__ __forceinline__ uint32_t across(uint32_t v, int lane) { return word_across<MASK>(v, lane); }
+template <int MASK>
 __device__ __forceinline__ Entry across(Entry e, int lane) {
     return static_cast<uint64_t>(word_across<MASK>(static_cast<uint32_t>(e >> 32), lane)) << 32 | word_across<MASK>(static_cast<uint32_t>(e), lane);
 }
-// lane l and lane l ^ MASK in descending order: the lower lane of the two gets the larger entry
-template <int MASK>
-__device__ __forceinline__ Entry order(Entry e, int lane) {
+// lane l and lane l ^ MASK in descending order: the lower lane of the two gets the larger of them (entries, or keys alone)
+template <int MASK, class E>
+__device__ __forceinline__ E order(E e, int lane) {
     constexpr int kTop = (MASK + 1) & MASK ? MASK : (MASK + 1) / 2;        // the highest bit of MASK
-    const Entry o = across<MASK>(e, lane);
+    const E o = across<MASK>(e, lane);
     return ((e > o) == !(lane & kTop)) ? e : o;
 }
-template <int HALF>
-__device__ __forceinline__ Entry order_from(Entry e, int lane) {           // a sequence that rises and falls, in blocks of 2 HALF
+template <int HALF, class E>
+__device__ __forceinline__ E order_from(E e, int lane) {                   // a sequence that rises and falls, in blocks of 2 HALF
     if constexpr (HALF == 0) return e;
     else return order_from<HALF / 2>(order<HALF>(e, lane), lane);
 }
-// the wave's entries in descending order: sorted runs of 2, 4 .. 64, each of two halves met as mirror images
-__device__ __forceinline__ Entry sort_wave(Entry e, int lane) {
+// the wave's in descending order: sorted runs of 2, 4 .. 64, each of two halves met as mirror images
+template <class E>
+__device__ __forceinline__ E sort_wave(E e, int lane) {
     e = order<1>(e, lane);
     e = order_from<1>(order<3>(e, lane), lane);
     e = order_from<2>(order<7>(e, lane), lane);
@@ -117,8 +119,9 @@ __device__ __forceinline__ Entry sort_wave(Entry e, int lane) {
     return order_from<16>(order<63>(e, lane), lane);
 }
 // the best 64 of two descending sequences, descending
-__device__ __forceinline__ Entry merge_waves(Entry a, Entry b, int lane) {
-    const Entry o = across<63>(b, lane);
+template <class E>
+__device__ __forceinline__ E merge_waves(E a, E b, int lane) {
+    const E o = across<63>(b, lane);
     return order_from<32>(a > o ? a : o, lane);
 }
 
@@ -127,26 +130,57 @@ struct BestEntries {
     Entry mine;
     Entry last;            // the top-th best (the same in every lane): what comes in has to be larger
     __device__ __forceinline__ void clear() { mine = last = 0; }
-    __device__ __forceinline__ void settle(int top) { last = entry_of_lane(mine, top - 1); }
-    // one candidate per lane (0: none): a few go in one by one, many as a sorted run
+    // one candidate per lane (0: none)
+    __device__ __forceinline__ void take(Entry e, int top, int lane) {
+        mine = merge_waves(mine, sort_wave(e, lane), lane);
+        last = entry_of_lane(mine, top - 1);
+    }
+    // the same, skipped where none comes in
     __device__ __forceinline__ void offer(Entry e, int top, int lane) {
-        uint64_t wanting = __builtin_amdgcn_ballot_w64(e > last);
-        if (__popcll(wanting) > 6) {
-            mine = merge_waves(mine, sort_wave(e > last ? e : 0, lane), lane);
-            settle(top);
-            return;
-        }
-        while (wanting) {
-            const Entry c = entry_of_lane(e, __builtin_ctzll(wanting));
-            wanting &= wanting - 1;
-            if (c <= last) continue;
-            // lane l takes the entry of lane l - 1 behind the place where c belongs
-            const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(mine)), 0x138, 0xf, 0xf, false));
-            const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(mine >> 32), 0x138, 0xf, 0xf, false));
-            const Entry before = static_cast<uint64_t>(hi) << 32 | lo;
-            if (mine < c) mine = lane > 0 && before < c ? before : c;
-            settle(top);
-        }
+        if (__builtin_amdgcn_ballot_w64(e > last)) take(e > last ? e : 0, top, lane);
+    }
+};
+
+// The best entries of a long run of values, a batch at a time: what may come in is put down in LDS, and once 64 are together they
+// are sorted and merged.  Until then `bound` stands for the top-th best: that many values of the first batch reach it.
+struct BestOfBatches {
+    BestEntries best;
+    float bound;
+    int count;             // entries waiting, at most 64 between batches
+    Entry* waiting;        // 128, of this wave alone
+    __device__ __forceinline__ void clear(Entry* place) {
+        best.clear();
+        count = 0;
+        waiting = place;
+    }
+    __device__ __forceinline__ void first(float lane_most, int top, int lane) {
+        bound = value_of_key(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sort_wave(key_of(lane_most), lane)), top - 1)));
+    }
+    // the values of the lanes that say so
+    __device__ __forceinline__ void put(bool wanted, float value, uint32_t index, int top, int lane) {
+        const uint64_t which = __builtin_amdgcn_ballot_w64(wanted);
+        if (!which) return;
+        const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(which >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(which), 0));
+        if (wanted) waiting[count + before] = entry_of(value, index);
+        count += __popcll(which);
+        if (count <= 64) return;
+        wave_order();
+        best.take(waiting[lane], top, lane);
+        const Entry more = lane < count - 64 ? waiting[64 + lane] : 0;
+        wave_order();
+        waiting[lane] = more;
+        count -= 64;
+        bound = fmaxf(bound, value_of(best.last));
+    }
+    __device__ __forceinline__ void finish(int top, int lane) {
+        wave_order();
+        best.offer(lane < count ? waiting[lane] : 0, top, lane);
+    }
+    // the wave's own LDS accesses in the order of the program
+    static __device__ __forceinline__ void wave_order() {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 };
 

@@ -5,14 +5,6 @@ namespace qa {
 namespace lm {
 namespace {
 
-AddNormShape shape_of(const QaAddNormParams& p) {
-    const int runs = (p.dim + 511) / 512;                 // waves that one piece each would take
-    int pieces = 1;
-    while ((runs + pieces - 1) / pieces > kAddNormWaves) pieces *= 2;
-    const int waves = (runs + pieces - 1) / pieces;
-    return {pieces, waves, waves >= 4 ? 1 : 4 / waves};
-}
-
 // rows, when there are any, of `type` on 16 bytes (8 for codes)
 bool on_words(const void* base, int64_t row_stride, int type) {
     const int64_t bytes = bytes_of(type), unit = type == QA_LM_I8 ? 8 : 16;
@@ -51,7 +43,7 @@ extern "C" int qa_add_rmsnorm(const QaAddNormParams* p, void* stream_) {
                       on_words(p->out, p->out_row_stride, p->out_type) && on_words(p->weight, 0, p->param_type) &&
                       on_words(p->post_weight, 0, p->param_type) && on_words(p->scale_vector, 0, p->param_type);
     hipStream_t stream = static_cast<hipStream_t>(stream_);
-    const AddNormShape s = shape_of(*p);
+    const AddNormShape s = add_norm_shape(p->dim);
     if (p->x_type == QA_LM_F16) return add_rmsnorm_f16(*p, s, wide, stream);
     if (p->x_type == QA_LM_BF16) return add_rmsnorm_bf16(*p, s, wide, stream);
     return add_rmsnorm_launch<float, float, float>(*p, s, wide, stream);

@@ -21,13 +21,28 @@ namespace lm {
 constexpr int kAddNormWaves = 16;                        // of a workgroup, at most
 constexpr int kAddNormDim = kAddNormWaves * 4 * 512;     // widest row
 
-// waves that share a row, and rows of a workgroup
+// within 4 + |z| units of 2^-24 (an exponential and a reciprocal of two each, and the rounding of the exponent); exact divisions and
+// expf made the gate the larger part of the kernel's time
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f)); }
+
+// Pieces of a lane, waves that share a row, rows of a workgroup.  A run is what a wave loads at once, 512 columns.
 struct AddNormShape {
     int pieces, waves, rows;
 };
+constexpr int max_waves(int pieces) { return pieces == 3 ? 9 : kAddNormWaves; }
+// Two runs a wave: with one a row's barriers gather twice the waves, with more a wave holds so much that fewer of them are there
+// (everything on, us with 1, 2, 3, 4 of them a wave: 8192 x 4096 bf16 73, 64, 67, 65; 4096 x 8192 bf16 with an fp32 stream 108, 91, 102, 102;
+// 64 x 2560 4.6, 4.4, 4.9, 5.7).  Three where that leaves no wave without work and two would (6131 x 4099, nine runs: 95, 71, 62, 73); four
+// for rows that sixteen waves do not hold otherwise.
+inline AddNormShape add_norm_shape(int dim) {
+    const int runs = (dim + 511) / 512;
+    const int pieces = runs == 1 ? 1 : runs > 2 * kAddNormWaves ? 4 : runs % 2 != 0 && runs % 3 == 0 ? 3 : 2;
+    const int waves = (runs + pieces - 1) / pieces;
+    return {pieces, waves, waves >= 4 ? 1 : 4 / waves};
+}
 
 template <class X, class R, class P, int PIECES, bool WIDE, bool BLOCK>
-__global__ __launch_bounds__(64 * kAddNormWaves) void add_rmsnorm_kernel(QaAddNormParams p, int W) {
+__global__ __launch_bounds__(64 * max_waves(PIECES)) void add_rmsnorm_kernel(QaAddNormParams p, int W) {
     __shared__ float s_part[3][kAddNormWaves];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int sub = wave % W, first = wave - sub;
@@ -104,7 +119,7 @@ __global__ __launch_bounds__(64 * kAddNormWaves) void add_rmsnorm_kernel(QaAddNo
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float z = rg[c].get(j);
-                    v[c][j] *= p.gate_act == QA_GATE_PLAIN ? z : (p.gate_act == QA_GATE_SILU ? z : 1.0f) * (1.0f / (1.0f + expf(-z)));
+                    v[c][j] *= p.gate_act == QA_GATE_PLAIN ? z : (p.gate_act == QA_GATE_SILU ? z : 1.0f) * sigmoid(z);
                 }
         }
         if (p.scale_vector) {
@@ -209,6 +224,7 @@ int add_rmsnorm_launch(const QaAddNormParams& p, const AddNormShape& s, bool wid
     switch (s.pieces) {
         case 1: return go(std::integral_constant<int, 1>{});
         case 2: return go(std::integral_constant<int, 2>{});
+        case 3: return go(std::integral_constant<int, 3>{});
         default: return go(std::integral_constant<int, 4>{});
     }
 }

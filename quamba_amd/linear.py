@@ -53,6 +53,26 @@ class _W8A8Base(nn.Module):
         return y.view(*x_shape[:-1], -1)
 
 
+def _token_scales(x_scale, shape, otherwise):
+    """One scale per row of the flattened activations, or the layer's own"""
+    if x_scale is None:
+        return otherwise.reshape(-1)
+    if x_scale.shape != shape:
+        raise RuntimeError(f"x_scale must have shape {tuple(shape)}, not {tuple(x_scale.shape)}")
+    return x_scale.reshape(-1)
+
+
+def _tokens_like(tokens, shape):
+    if tokens.shape != shape:
+        raise RuntimeError(f"tokens must have shape {tuple(shape)}, not {tuple(tokens.shape)}")
+    return tokens.reshape(-1)
+
+
+def _shaped_logprobs(r, shape):
+    top = r.top_tokens.shape[-1]
+    return ops.TokenLogprobs(r.logprobs.view(shape), r.entropy.view(shape), r.top_logprobs.view(*shape, top), r.top_tokens.view(*shape, top))
+
+
 class _AlphaHooks:
     """``alpha`` (Python float used by the single-row path) travels through the state dict."""
 
@@ -188,6 +208,24 @@ class W8A8B16O16Linear(_W8A8Base, _AlphaHooks):
             y = self._mm(x2d, torch.float16)
         return self._finish(y, x_shape)
 
+    @torch.no_grad()
+    def token_logprobs(self, x, tokens, top=0, x_scale=None):
+        """As a model's head: log probabilities of ``tokens`` (...,) after the hidden states ``x`` int8 (..., in), entropies, and the
+        ``top`` best alternatives, an ops.TokenLogprobs.  ``x_scale`` fp32 (...,): one scale per token, as QRMSNorm gives them, in
+        place of the layer's input scale.
+
+        With ``top`` up to 1 the logits stay in fp32 and are never written (ops.scaled_mm_token_logprobs); with more they are
+        those of ``forward``, rounded to fp16."""
+        x2d, shape = x.reshape(-1, x.shape[-1]).contiguous(), x.shape[:-1]
+        a, flat = _token_scales(x_scale, shape, self.a), _tokens_like(tokens, shape)
+        if top <= 1:
+            r = ops.scaled_mm_token_logprobs(x2d, self.weight, a, self.b, flat, top, self.out_features)
+        else:
+            y = torch.empty((x2d.shape[0], self.out_features + self.pad_out), dtype=torch.float16, device=x.device)
+            ops.scaled_mm_dq(y, x2d, self.weight, a, self.b)
+            r = ops.token_logprobs(y[:, :self.out_features], flat, top)
+        return _shaped_logprobs(r, shape)
+
     def __repr__(self):
         return f"W8A8B16O16Linear(in_features={self.in_features}, out_features={self.out_features})"
 
@@ -292,6 +330,14 @@ class _W4A8Base(nn.Module):
 
 class W4A8B16O16Linear(_W4A8Base):
     _out_dtype = torch.float16
+
+    @torch.no_grad()
+    def token_logprobs(self, x, tokens, top=0, x_scale=None):
+        """As W8A8B16O16Linear.token_logprobs; the logits are those of ``forward``, in fp16, whatever ``top``."""
+        x2d, shape = x.reshape(-1, x.shape[-1]).contiguous(), x.shape[:-1]
+        a, flat = _token_scales(x_scale, shape, self.input_scale), _tokens_like(tokens, shape)
+        y = ops.w4a8o16_gemm(x2d, self.weight, a, self.s_channel, self.s_group, self.workspace, x2d.shape[0], self.size_n, self.size_k)
+        return _shaped_logprobs(ops.token_logprobs(y[:, :self.out_features], flat, top), shape)
 
     @classmethod
     def from_fp16(cls, originalLayer: nn.Linear, input_scale: torch.Tensor):

@@ -9,6 +9,8 @@
 #include "gemm_core.hpp"
 #include "row_stats.hpp"
 
+#include <algorithm>
+
 namespace qa {
 namespace lm {
 namespace {
@@ -52,12 +54,12 @@ __device__ __forceinline__ float sum_over_columns(float v) {
 // the best column each on its own).
 // PLAIN: all of the wave's columns are the vocabulary's and none of its rows has a negative scale.
 template <bool PLAIN, bool TOP, int TM, int TN, int BM, int BN, class V, int NI, int NJ>
-__device__ __forceinline__ void tile_stats(const QaMmTokenLogprobsParams& p, V (&acc)[NI][NJ], const float* s_lds, int row_at, int col_at, int m0, int n0, int lane,
+__device__ __forceinline__ void tile_stats(const QaMmTokenLogprobsParams& p, V (&acc)[NI][NJ], const float* s_lds, int row_at, int col_at, int m0, int n0, int n_end, int lane,
                                            TilePart* parts, float* given) {
     using Q = QuadView<V>;
     constexpr int kQuads = TN * 32 / (256 / Q::kRows), kRowBlocks = TM * 32 / Q::kRows;
     static_assert(NI * Q::kQuadsPer == kQuads && NJ == kRowBlocks, "accumulators of another tile");
-    const int columns = p.vocab - (n0 + col_at);           // of the vocabulary, from this wave's first one on
+    const int columns = n_end - (n0 + col_at);             // of the tile, from this wave's first one on
 #pragma unroll
     for (int b = 0; b < kRowBlocks; ++b) {
         const int row = row_at + b * Q::kRows + Q::row_of(lane);
@@ -117,19 +119,22 @@ __device__ __forceinline__ void tile_stats(const QaMmTokenLogprobsParams& p, V (
     }
 }
 
-template <int TM, int TN, int WGM, int WGN, int STAGES, bool TOP>
-__global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmTokenLogprobsParams p) {
+// A tile takes `columns` of its BN columns.  TURN: workgroups do not all start at K's beginning (in step, all of them ask for the same 128 bytes of
+// rows that lie K bytes apart, which few of the memory's channels hold: 64 x 50280 x 4096 56.7 -> 50.9 us, other K the same).
+template <int TM, int TN, int WGM, int WGN, int STAGES, bool TOP, bool TURN>
+__global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmTokenLogprobsParams p, int columns) {
     using C = Cfg<TM, TN, WGM, WGN, STAGES>;
     constexpr int BM = C::kBM, BN = C::kBN, WAVES = C::kWaves;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     static_assert(WGN * BM * static_cast<int>(sizeof(TilePart)) <= C::kLdsBytes, "the waves' statistics take the place of the operands");
+    static_assert(BM % 64 == 0 && BN % 64 == 0 && BM * kChunks % C::kThreads == 0 && BN * kChunks % C::kThreads == 0, "whole requests");
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WGM, wn = wave / WGM;
-    const int tiles_m = (p.rows + BM - 1) / BM, tiles_n = (p.vocab + BN - 1) / BN;
+    const int tiles_m = (p.rows + BM - 1) / BM, tiles_n = (p.vocab + columns - 1) / columns;
     int tile_m, tile_n;
     tile_of_workgroup<BM, BN>(blockIdx.x, tiles_m, tiles_n, tile_m, tile_n);
-    const int m0 = tile_m * BM, n0 = tile_n * BN;
+    const int m0 = tile_m * BM, n0 = tile_n * columns, n_end = min(n0 + columns, p.vocab);
     const v4i rsrc_a = make_rsrc(p.a, static_cast<int>((static_cast<int64_t>(p.rows) - 1) * p.lda + p.k));
     const v4i rsrc_w = make_rsrc(p.w, static_cast<int>((static_cast<int64_t>(p.vocab) - 1) * p.ldw + p.k));
     const uint32_t lds_base = lds_offset_of(lds);
@@ -143,8 +148,14 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmT
     TileLoader<C::kAInstr> load_a;
     TileLoader<C::kWInstr> load_w;
     load_a.template init<WAVES>(m0, p.rows, p.lda, wave, lane);
-    load_w.template init<WAVES>(n0, p.vocab, p.ldw, wave, lane);
+    load_w.template init<WAVES>(n0, n_end, p.ldw, wave, lane);
     const int k_tiles = (p.k + kBK - 1) / kBK;
+    const int turn = TURN ? static_cast<int>(static_cast<unsigned>(blockIdx.x * 7) % static_cast<unsigned>(k_tiles)) : 0;
+    auto k_of = [&](int tile) {
+        if constexpr (!TURN) return tile * kBK;
+        const int t = tile + turn;
+        return tile >= k_tiles ? k_tiles * kBK : (t >= k_tiles ? t - k_tiles : t) * kBK;
+    };
 
     TilePart* const parts = reinterpret_cast<TilePart*>(lds);
     TilePart* const out = static_cast<TilePart*>(p.workspace);
@@ -155,9 +166,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmT
         float* const given = reinterpret_cast<float*>(out + static_cast<int64_t>(p.rows) * tiles_n);
         bool negative = false;
         for (int row = lane; row < TM * 32; row += 64) negative |= s_lds[BN + wm * TM * 32 + row] < 0.0f;
-        const bool plain = p.vocab - (n0 + wn * TN * 32) >= TN * 32 && !__builtin_amdgcn_ballot_w64(negative);
+        const bool plain = n_end - (n0 + wn * TN * 32) >= TN * 32 && !__builtin_amdgcn_ballot_w64(negative);
         auto stats = [&](auto plain_c) __attribute__((always_inline)) {
-            tile_stats<decltype(plain_c)::value, TOP, TM, TN, BM, BN>(p, acc, s_lds, wm * TM * 32, wn * TN * 32, m0, n0, lane, parts + wn * BM, given);
+            tile_stats<decltype(plain_c)::value, TOP, TM, TN, BM, BN>(p, acc, s_lds, wm * TM * 32, wn * TN * 32, m0, n0, n_end, lane, parts + wn * BM, given);
         };
         if (plain) stats(std::true_type{});
         else stats(std::false_type{});
@@ -191,9 +202,10 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmT
 #pragma unroll
         for (int t = 0; t < STAGES - 1; ++t)
 #pragma unroll
-            for (int r = 0; r < kReq; ++r) request(r, t * kBK, t * C::kStageBytes);
+            for (int r = 0; r < kReq; ++r) request(r, k_of(t), t * C::kStageBytes);
+        int k_late = k_of(STAGES - 1);                                 // of the tile STAGES - 1 further than the one at hand
 #pragma unroll
-        for (int r = 0; r < kEarly; ++r) request(r, (STAGES - 1) * kBK, (STAGES - 1) * C::kStageBytes);
+        for (int r = 0; r < kEarly; ++r) request(r, k_late, (STAGES - 1) * C::kStageBytes);
         __builtin_amdgcn_s_waitcnt(vmcnt_imm((STAGES - 2) * kReq + kEarly));
         __syncthreads();
         const uint8_t* my_a = lds + (wm * TM * 32) * kBK;
@@ -204,12 +216,14 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmT
         uint32_t cur = 0, late = (STAGES - 1) * C::kStageBytes;
         auto multiply = [&](int kt, auto&& req) {
             const uint32_t nxt = cur + C::kStageBytes == C::kLdsBytes ? 0 : cur + C::kStageBytes;
+            const int k_early = k_of(kt + STAGES);
             mma.template tile<(STAGES - 2) * kReq>(my_a + cur, my_w + cur, my_a + nxt, my_w + nxt, [&](int idx) {
                 if (idx % kPace != kPace - 1) return;
                 const int r = idx / kPace;
-                if (r < kEarly) req(r, (kt + STAGES) * kBK, cur);
-                else req(r, (kt + STAGES - 1) * kBK, late);
+                if (r < kEarly) req(r, k_early, cur);
+                else req(r, k_late, late);
             });
+            k_late = k_early;
             late = cur;
             cur = nxt;
         };
@@ -224,8 +238,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmT
         for (int r = 0; r < 16; ++r) acc[0][0][r] = 0;
         auto issue = [&](int tile) {
             const uint32_t base = lds_base + (tile % STAGES) * C::kStageBytes;
-            load_a.template issue<WAVES>(rsrc_a, tile * kBK, p.k, base, wave);
-            load_w.template issue<WAVES>(rsrc_w, tile * kBK, p.k, base + BM * kBK, wave);
+            load_a.template issue<WAVES>(rsrc_a, k_of(tile), p.k, base, wave);
+            load_w.template issue<WAVES>(rsrc_w, k_of(tile), p.k, base + BM * kBK, wave);
         };
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) issue(s);
@@ -235,10 +249,11 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmT
             const uint8_t* stage = lds + (kt % STAGES) * C::kStageBytes;
             const int nt = kt + STAGES - 1;
             const uint32_t nbase = lds_base + (nt % STAGES) * C::kStageBytes;
+            const int nk = k_of(nt);
             static_assert(C::kAInstr + C::kWInstr <= 4, "a request behind each of four multiplications");
             mma_tile_paced(stage + wm * 32 * kBK, stage + BM * kBK + wn * 32 * kBK, frow, fhalf, acc[0][0], [&](int r) {
-                if (r < C::kAInstr) load_a.template issue_one<WAVES>(r, rsrc_a, nt * kBK, p.k, nbase, wave);
-                else if (r < C::kAInstr + C::kWInstr) load_w.template issue_one<WAVES>(r - C::kAInstr, rsrc_w, nt * kBK, p.k, nbase + BM * kBK, wave);
+                if (r < C::kAInstr) load_a.template issue_one<WAVES>(r, rsrc_a, nk, p.k, nbase, wave);
+                else if (r < C::kAInstr + C::kWInstr) load_w.template issue_one<WAVES>(r - C::kAInstr, rsrc_w, nk, p.k, nbase + BM * kBK, wave);
             });
         }
         finish(acc);
@@ -307,24 +322,44 @@ __global__ __launch_bounds__(kJoinThreads) void mm_token_logprobs_join_kernel(Qa
 }
 
 // The tiles, and what a launch of them takes, in us with `units` of 128 codes of K: fixed and, for each round of one tile per CU,
-// per_round + per_unit x units (the launch of the join is in it).  The fastest by that is taken; up to 64 rows only tiles of 64, which
-// read the weights at the memory's rate and nothing for rows that are not there.  Measured over 1 .. 16384 rows, 1000 .. 256000 columns
-// and K from 768 to 4096 the choice is the fastest of the six but for 1.5 % of the time (rows x vocabulary x K, us by the tiles in the
-// order below): 64 x 16000 x 2560 13.1, 15.0, 16.0, 20.7, 32.5, 36.2; 64 x 50280 x 2560 34.4, 30.4, 40.5, 33.8, 44.9, 48.1; 1000 x 4000 x
-// 2560 25.3, 21.3, 18.2, 24.2, 34.4, 37.4; 128 x 50280 x 2560 (the third on) 43.7, 36.6, 45.3, 48.4; 256 x 50280 x 2560 70.9, 57.8, 49.1,
-// 51.0; 16000 x 16000 x 768 419, 349, 360, 281, 238, 227; 16384 x 50280 x 2560 (the last two) 1667, 1554.
+// per_round + per_unit x units (the launch of the join is in it).  From 65 rows on the fastest by that is taken.  Measured over 1 .. 16384
+// rows, 1000 .. 256000 columns and K from 768 to 4096 the choice is the fastest of them but for 1.5 % of the time (rows x vocabulary x K,
+// us by the tiles in the order below, without the third): 1000 x 4000 x 2560 25.3, 21.3, 18.2, 24.2, 34.4, 37.4; 128 x 50280 x 2560 (from
+// 128 rows on) 43.7, 36.6, 45.3, 48.4; 256 x 50280 x 2560 70.9, 57.8, 49.1, 51.0; 16000 x 16000 x 768 419, 349, 360, 281, 238, 227; 16384 x
+// 50280 x 2560 (the last two) 1667, 1554.
 struct Tile {
     int bm, bn;
     float fixed, per_round, per_unit;
 };
-constexpr Tile kTiles[] = {{64, 64, 6.0f, 0.3f, 0.2f},    {64, 128, 6.0f, 1.0f, 0.31f},  {128, 128, 4.0f, 1.6f, 0.56f},
+constexpr Tile kTiles[] = {{64, 64, 6.0f, 0.3f, 0.2f},    {64, 128, 6.0f, 1.0f, 0.31f},   {64, 256, 0.0f, 0.0f, 0.0f},   {128, 128, 4.0f, 1.6f, 0.56f},
                            {128, 256, 4.0f, 2.6f, 0.84f}, {256, 256, 5.0f, 3.6f, 1.45f}, {256, 320, 5.0f, 4.2f, 1.75f}};
-int tile_of(const QaMmTokenLogprobsParams& p) {
-    const int cus = compute_units(), candidates = p.rows <= 64 ? 2 : 6, units = (p.k + kBK - 1) / kBK;
+constexpr int kNarrow = 0, kMiddle = 1, kWide = 2, kWideOf128 = 4;
+
+// The tile, and how many columns of the vocabulary one takes (the rest of its width reads nothing).
+//
+// One row of tiles is bound by the memory's rate, of which a CU alone takes a part: all of them have to be at it all the time, with the same
+// number of columns.  Those of 16 that make whole rounds, in the narrowest tile that holds them (64 rows, us with whole tiles of 128
+// and so): 50280 x 2560 37.2 -> 31.5, 50280 x 4096 51.0 -> 42.9, 40000 x 2560 33.9 -> 28.1, 98304 x 2560 58.4 -> 55.8.
+struct Plan {
+    int tile, columns;
+};
+Plan plan_of(const QaMmTokenLogprobsParams& p) {
+    const int cus = compute_units(), units = (p.k + kBK - 1) / kBK;
+    auto even = [&](int width) {
+        const int64_t places = static_cast<int64_t>((p.vocab + static_cast<int64_t>(cus) * width - 1) / (static_cast<int64_t>(cus) * width)) * cus;
+        return static_cast<int>((p.vocab + 16 * places - 1) / (16 * places) * 16);
+    };
+    if (p.rows <= 64) {
+        const int columns = std::max(even(256), 64);
+        // (a short K is over before the difference shows: 1 x 50280 x 768 13.4 by 128 columns, 13.8; 4 x 256000 x 768 47.9, 49.7)
+        if (columns > 128 && units <= 8) return {kMiddle, 128};
+        return {columns <= 64 ? kNarrow : columns <= 128 ? kMiddle : kWide, columns};
+    }
     int best = 0;
     float best_us = 1e30f;
-    for (int i = 0; i < candidates; ++i) {
+    for (int i = 0; i < static_cast<int>(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
         const Tile& t = kTiles[i];
+        if (i == kWide) continue;
         const int64_t tiles = static_cast<int64_t>((p.rows + t.bm - 1) / t.bm) * ((p.vocab + t.bn - 1) / t.bn);
         const float us = t.fixed + static_cast<float>((tiles + cus - 1) / cus) * (t.per_round + t.per_unit * units);
         if (us < best_us) {
@@ -332,7 +367,7 @@ int tile_of(const QaMmTokenLogprobsParams& p) {
             best_us = us;
         }
     }
-    return best;
+    return {best, best == kWideOf128 && p.rows <= 128 ? even(256) : kTiles[best].bn};
 }
 
 int check(const QaMmTokenLogprobsParams& p) {
@@ -343,22 +378,22 @@ int check(const QaMmTokenLogprobsParams& p) {
 }
 
 int64_t workspace_bytes(const QaMmTokenLogprobsParams& p) {
-    const int64_t bn = kTiles[tile_of(p)].bn, tiles_n = (p.vocab + bn - 1) / bn;
+    const int64_t columns = plan_of(p).columns, tiles_n = (p.vocab + columns - 1) / columns;
     return p.rows * (tiles_n * static_cast<int64_t>(sizeof(TilePart)) + static_cast<int64_t>(sizeof(float)));
 }
 
-template <int TILE, int TM, int TN, int WGM, int WGN, int STAGES>
-int launch(const QaMmTokenLogprobsParams& p, hipStream_t stream) {
+template <int TILE, int TM, int TN, int WGM, int WGN, int STAGES, bool TURN>
+int launch(const QaMmTokenLogprobsParams& p, int columns, hipStream_t stream) {
     using C = Cfg<TM, TN, WGM, WGN, STAGES>;
     static_assert(C::kBM == kTiles[TILE].bm && C::kBN == kTiles[TILE].bn, "the tile of the table");
-    const int tiles_n = (p.vocab + C::kBN - 1) / C::kBN;
+    const int tiles_n = (p.vocab + columns - 1) / columns;
     const int64_t tiles = static_cast<int64_t>((p.rows + C::kBM - 1) / C::kBM) * tiles_n;
     if (tiles > 0x7fffffffLL) return QA_ERR_SHAPE;
-    auto kernel = p.top ? mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES, true> : mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES, false>;
+    auto kernel = p.top ? mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES, true, TURN> : mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES, false, TURN>;
     constexpr int kLds = C::kLdsBytes + TileScales<C::kBM, C::kBN, C::kWaves>::kBytes + C::kBM * 4;
     static_assert(kLds <= 160 * 1024, "LDS of a CU");
     if (kLds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) return check_launch();
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(C::kThreads), kLds, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(C::kThreads), kLds, stream, p, columns);
     if (const int status = check_launch()) return status;
     const int at_once = p.rows >= 4096 ? 16 : p.rows >= 512 ? 4 : 1;
     const dim3 grid(static_cast<unsigned>((p.rows + at_once - 1) / at_once));
@@ -391,12 +426,15 @@ extern "C" int qa_mm_token_logprobs(const QaMmTokenLogprobsParams* p, void* stre
     if (static_cast<int64_t>(p->rows) * p->lda >= 0x70000000LL || static_cast<int64_t>(p->vocab) * p->ldw >= 0x70000000LL) return QA_ERR_SHAPE;
     if (!aligned16(p->workspace) || p->workspace_bytes < workspace_bytes(*p)) return QA_ERR_SCRATCH;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
-    switch (tile_of(*p)) {
-        case 0: return launch<0, 1, 1, 2, 2, 3>(*p, stream);
-        case 1: return launch<1, 1, 2, 2, 2, 3>(*p, stream);
-        case 2: return launch<2, 2, 1, 2, 4, 4>(*p, stream);
-        case 3: return launch<3, 2, 2, 2, 4, 3>(*p, stream);
-        case 4: return launch<4, 4, 2, 2, 4, 2>(*p, stream);
-        default: return launch<5, 2, 5, 4, 2, 2>(*p, stream);
+    const Plan plan = plan_of(*p);
+    const bool turned = p->k % kBK == 0;
+    switch (plan.tile) {
+        case 0: return turned ? launch<0, 1, 1, 2, 2, 3, true>(*p, plan.columns, stream) : launch<0, 1, 1, 2, 2, 3, false>(*p, plan.columns, stream);
+        case 1: return turned ? launch<1, 1, 2, 2, 2, 3, true>(*p, plan.columns, stream) : launch<1, 1, 2, 2, 2, 3, false>(*p, plan.columns, stream);
+        case 2: return turned ? launch<2, 1, 2, 2, 4, 3, true>(*p, plan.columns, stream) : launch<2, 1, 2, 2, 4, 3, false>(*p, plan.columns, stream);
+        case 3: return launch<3, 2, 1, 2, 4, 4, false>(*p, plan.columns, stream);
+        case 4: return launch<4, 2, 2, 2, 4, 3, false>(*p, plan.columns, stream);
+        case 5: return launch<5, 4, 2, 2, 4, 2, false>(*p, plan.columns, stream);
+        default: return launch<6, 2, 5, 4, 2, 2, false>(*p, plan.columns, stream);
     }
 }

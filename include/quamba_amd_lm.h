@@ -29,7 +29,7 @@ typedef enum QaGateAct { QA_GATE_PLAIN = 0, QA_GATE_SIGMOID = 1, QA_GATE_SILU = 
  *   v = residual + scale * u                                                       (residual null: scale * u)
  *   y = v / sqrt(mean(v^2) + eps) * weight
  * all in fp32; v is not rounded on its way into y.  residual_out (null: not wanted) gets v; it may be `residual` itself and
- * must not overlap an input otherwise.  out gets y, or with QA_LM_I8 the saturated rint(y / s): s is out_scale, or with
+ * must not overlap an input otherwise.  out gets y, or with QA_LM_I8 the saturated rint(y / s): s is out_scale (a normal number above 0), or with
  * dynamic_scale max(max|y|, 1e-5) / 127 of the row, written to scales.  A row with a NaN or an infinity, or whose
  * squares pass fp32 (values from some 1e18 on), is NaN as a whole: its y, or its scale.
  */
@@ -66,7 +66,7 @@ int qa_add_rmsnorm(const QaAddNormParams* p, void* stream);
  * its top_tokens are indices inside the row.
  */
 typedef struct QaTokenLogprobsParams {
-    int32_t rows, vocab;
+    int32_t rows, vocab;        /* vocab up to 2^30 */
     int32_t logits_type;        /* QaLmType, not I8 */
     int32_t token_bytes;        /* 4 or 8: tokens are int32 or int64 */
     int32_t top, reserved0;
@@ -91,11 +91,11 @@ int qa_token_logprobs(const QaTokenLogprobsParams* p, void* stream);
  * qa_gemm_w8a8, in fp32 and never written).  top is 0 or 1.
  */
 typedef struct QaMmTokenLogprobsParams {
-    int32_t rows, vocab, k;     /* k a multiple of 16 */
+    int32_t rows, vocab, k;     /* vocab up to 2^30, k a multiple of 16 */
     int32_t a_scale_numel, w_scale_numel;   /* 1 or rows, 1 or at least vocab */
     int32_t token_bytes;
     int32_t top, reserved0;
-    int64_t lda, ldw;           /* row pitches of a (rows, k) and w (vocab, k): multiples of 16 */
+    int64_t lda, ldw;           /* row pitches of a (rows, k) and w (vocab, k): multiples of 16, up to 2^22 */
     const int8_t* a;
     const int8_t* w;
     const float* a_scale;

@@ -30,6 +30,8 @@ extern "C" int qa_add_rmsnorm(const QaAddNormParams* p, void* stream_) {
     if (p->gate_act < QA_GATE_PLAIN || p->gate_act > QA_GATE_SILU) return QA_ERR_UNSUPPORTED;
     if (p->rows == 0) return QA_OK;
     const bool dynamic = p->out_type == QA_LM_I8 && p->dynamic_scale;
+    // (the reciprocal of a smaller scale is no number)
+    if (p->out_type == QA_LM_I8 && !dynamic && !(p->out_scale >= 1.17549435e-38f && p->out_scale <= 3.402823466e38f)) return QA_ERR_UNSUPPORTED;
     if (!p->x || !p->weight || !p->out || (dynamic && !p->scales)) return QA_ERR_NULL;
     auto row_ok = [&](const void* base, int64_t stride, int type) { return !base || (on_elements(base, type) && (stride >= p->dim || p->rows == 1)); };
     if (!row_ok(p->x, p->x_row_stride, p->x_type) || !row_ok(p->residual, p->residual_row_stride, p->residual_type) ||

@@ -135,20 +135,23 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmT
     int tile_m, tile_n;
     tile_of_workgroup<BM, BN>(blockIdx.x, tiles_m, tiles_n, tile_m, tile_n);
     const int m0 = tile_m * BM, n0 = tile_n * columns, n_end = min(n0 + columns, p.vocab);
-    const v4i rsrc_a = make_rsrc(p.a, static_cast<int>((static_cast<int64_t>(p.rows) - 1) * p.lda + p.k));
-    const v4i rsrc_w = make_rsrc(p.w, static_cast<int>((static_cast<int64_t>(p.vocab) - 1) * p.ldw + p.k));
+    // (from the tile's own first row and column on: 32-bit offsets then reach over operands of any size)
+    const int rows = min(BM, p.rows - m0), width = n_end - n0;
+    const v4i rsrc_a = make_rsrc(p.a + m0 * p.lda, static_cast<int>((rows - 1) * p.lda + p.k));
+    const v4i rsrc_w = make_rsrc(p.w + n0 * p.ldw, static_cast<int>((width - 1) * p.ldw + p.k));
     const uint32_t lds_base = lds_offset_of(lds);
 
     using Scales = TileScales<BM, BN, WAVES>;
-    Scales::request(lds_base + C::kLdsBytes, p.a_scale, p.a_scale_numel, p.rows, m0, p.w_scale, p.w_scale_numel, p.vocab, n0, wave, lane);
-    const v4i rsrc_t = make_rsrc(p.tokens, static_cast<int>(min(static_cast<int64_t>(p.rows) * p.token_bytes, static_cast<int64_t>(0x7fffffff))));
+    const bool one_a = p.a_scale_numel == 1, one_w = p.w_scale_numel == 1;
+    Scales::request(lds_base + C::kLdsBytes, one_a ? p.a_scale : p.a_scale + m0, one_a ? 1 : 2, rows, 0, one_w ? p.w_scale : p.w_scale + n0, one_w ? 1 : 2, width, 0, wave, lane);
+    const v4i rsrc_t = make_rsrc(static_cast<const uint8_t*>(p.tokens) + static_cast<int64_t>(m0) * p.token_bytes, rows * p.token_bytes);
 #pragma unroll
     for (int i = 0; i < BM / 64; ++i)
-        if (i % WAVES == wave) buffer_load_lds_b32(rsrc_t, lds_base + C::kLdsBytes + Scales::kBytes + i * 256, (m0 + i * 64 + lane) * p.token_bytes);
+        if (i % WAVES == wave) buffer_load_lds_b32(rsrc_t, lds_base + C::kLdsBytes + Scales::kBytes + i * 256, (i * 64 + lane) * p.token_bytes);
     TileLoader<C::kAInstr> load_a;
     TileLoader<C::kWInstr> load_w;
-    load_a.template init<WAVES>(m0, p.rows, p.lda, wave, lane);
-    load_w.template init<WAVES>(n0, n_end, p.ldw, wave, lane);
+    load_a.template init<WAVES>(0, rows, p.lda, wave, lane);
+    load_w.template init<WAVES>(0, width, p.ldw, wave, lane);
     const int k_tiles = (p.k + kBK - 1) / kBK;
     const int turn = TURN ? static_cast<int>(static_cast<unsigned>(blockIdx.x * 7) % static_cast<unsigned>(k_tiles)) : 0;
     auto k_of = [&](int tile) {
@@ -370,8 +373,13 @@ Plan plan_of(const QaMmTokenLogprobsParams& p) {
     return {best, best == kWideOf128 && p.rows <= 128 ? even(256) : kTiles[best].bn};
 }
 
+// a tile's operands are addressed with 32-bit byte offsets
+constexpr int64_t kWidestRow = 4 << 20;
+static_assert(320 * kWidestRow < 0x70000000LL, "the widest tile");
+constexpr int kMostColumns = 1 << 30;
+
 int check(const QaMmTokenLogprobsParams& p) {
-    if (p.rows < 0 || p.vocab < 1 || p.k < 1) return QA_ERR_SHAPE;
+    if (p.rows < 0 || p.vocab < 1 || p.vocab > kMostColumns || p.k < 1) return QA_ERR_SHAPE;
     if (p.token_bytes != 4 && p.token_bytes != 8) return QA_ERR_UNSUPPORTED;
     if (p.top != 0 && p.top != 1) return QA_ERR_UNSUPPORTED;
     return QA_OK;
@@ -422,8 +430,7 @@ extern "C" int qa_mm_token_logprobs(const QaMmTokenLogprobsParams* p, void* stre
     if ((p->a_scale_numel != 1 && p->a_scale_numel != p->rows) || (p->w_scale_numel != 1 && p->w_scale_numel < p->vocab)) return QA_ERR_SHAPE;
     if (p->k % 16 != 0 || p->lda % 16 != 0 || p->ldw % 16 != 0 || !aligned16(p->a) || !aligned16(p->w) || p->lda < p->k || p->ldw < p->k) return QA_ERR_STRIDE;
     if (!aligned4(p->a_scale) || !aligned4(p->w_scale) || reinterpret_cast<uintptr_t>(p->tokens) % p->token_bytes != 0) return QA_ERR_STRIDE;
-    // operands are addressed with 32-bit byte offsets inside a buffer descriptor
-    if (static_cast<int64_t>(p->rows) * p->lda >= 0x70000000LL || static_cast<int64_t>(p->vocab) * p->ldw >= 0x70000000LL) return QA_ERR_SHAPE;
+    if (p->lda > kWidestRow || p->ldw > kWidestRow) return QA_ERR_SHAPE;
     if (!aligned16(p->workspace) || p->workspace_bytes < workspace_bytes(*p)) return QA_ERR_SCRATCH;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     const Plan plan = plan_of(*p);

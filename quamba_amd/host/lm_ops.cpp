@@ -236,7 +236,8 @@ PyObject* add_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const bool fixed = a[12] != Py_None;
         const double out_scale = fixed ? number(a[12]) : 0.0;
         require(!fixed || out_type == at::kChar, "out_scale is for int8 output");
-        require(!fixed || (static_cast<float>(out_scale) > 0.0f && static_cast<float>(out_scale) < std::numeric_limits<float>::infinity()), "out_scale must be positive");
+        require(!fixed || (static_cast<float>(out_scale) >= std::numeric_limits<float>::min() && static_cast<float>(out_scale) <= std::numeric_limits<float>::max()),
+                "out_scale must be positive and no smaller than fp32's normal numbers");
         const bool dynamic = out_type == at::kChar && !fixed;
         const auto asked = dtype_or_none(a[9], "residual_dtype");
         require(!residual || !asked || *asked == residual->scalar_type(), "residual_dtype differs from the type of residual");

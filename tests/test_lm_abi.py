@@ -79,7 +79,8 @@ def test_add_rmsnorm_refusals():
     _codes(l.qa_add_rmsnorm, p, [
         (dict(rows=-1), -2), (dict(dim=0), -2), (dict(dim=7), -4), (dict(dim=32769), -4), (dict(x_type=0), -4), (dict(x_type=4), -4),
         (dict(param_type=2), -4), (dict(residual_type=2), -4), (dict(residual_type=0), -4), (dict(out_type=2), -4), (dict(out_type=3), -4),
-        (dict(gate_act=3), -4), (dict(gate_act=-1), -4), (dict(x=0), -1), (dict(weight=0), -1), (dict(out=0), -1),
+        (dict(gate_act=3), -4), (dict(gate_act=-1), -4), (dict(out_type=0, out_scale=0.0), -4), (dict(out_type=0, out_scale=1e-39), -4),
+        (dict(out_type=0, out_scale=float("inf")), -4), (dict(out_type=0, out_scale=float("nan")), -4), (dict(x=0), -1), (dict(weight=0), -1), (dict(out=0), -1),
         (dict(out_type=0, dynamic_scale=1, scales=0), -1), (dict(x=AT + 1), -3), (dict(weight=AT + 1), -3), (dict(post_weight=AT + 1), -3),
         (dict(scale_vector=AT + 1), -3), (dict(gate=AT + 1), -3), (dict(residual=AT + 1), -3), (dict(residual_out=AT + 1), -3), (dict(out=AT + 1), -3),
         (dict(residual_type=3, residual=AT + 2), -3), (dict(out_type=0, dynamic_scale=1, scales=AT + 2), -3), (dict(x_row_stride=63), -3),
@@ -96,7 +97,7 @@ def test_token_logprobs_refusals():
     p.workspace_bytes = need = l.qa_token_logprobs_workspace_bytes(C.byref(p))
     assert need > 0                                                # (one row is cut into segments)
     _codes(l.qa_token_logprobs, p, [
-        (dict(rows=-1), -2), (dict(vocab=0), -2), (dict(top=65), -4), (dict(top=-1), -4), (dict(vocab=4), -2), (dict(logits_type=0), -4),
+        (dict(rows=-1), -2), (dict(vocab=0), -2), (dict(vocab=(1 << 30) + 1), -2), (dict(top=65), -4), (dict(top=-1), -4), (dict(vocab=4), -2), (dict(logits_type=0), -4),
         (dict(logits_type=4), -4), (dict(token_bytes=2), -4), (dict(logits=0), -1), (dict(tokens=0), -1), (dict(logprobs=0), -1), (dict(entropy=0), -1),
         (dict(top_logprobs=0), -1), (dict(top_tokens=0), -1), (dict(logits=AT + 1), -3), (dict(tokens=AT + 4), -3), (dict(rows=2, row_stride=50279), -3),
         (dict(workspace=0), -1), (dict(workspace=AT + 8), -6), (dict(workspace_bytes=need - 1), -6), (dict(rows=0, logits=0, tokens=0, workspace=0), 0)])
@@ -121,8 +122,8 @@ def test_mm_token_logprobs_refusals():
         (dict(w=0), -1), (dict(a_scale=0), -1), (dict(w_scale=0), -1), (dict(tokens=0), -1), (dict(logprobs=0), -1), (dict(entropy=0), -1),
         (dict(top_logprobs=0), -1), (dict(top_tokens=0), -1), (dict(workspace=0), -1), (dict(a_scale_numel=3), -2), (dict(w_scale_numel=999), -2),
         (dict(k=250, lda=256), -3), (dict(lda=264), -3), (dict(ldw=264), -3), (dict(lda=240), -3), (dict(ldw=240), -3), (dict(a=AT + 8), -3), (dict(w=AT + 8), -3),
-        (dict(a_scale=AT + 2), -3), (dict(w_scale=AT + 2), -3), (dict(tokens=AT + 4), -3), (dict(vocab=1 << 23, w_scale_numel=1), -2),
-        (dict(rows=1 << 23, a_scale_numel=1), -2), (dict(workspace=AT + 8), -6), (dict(workspace_bytes=need - 1), -6),
+        (dict(a_scale=AT + 2), -3), (dict(w_scale=AT + 2), -3), (dict(tokens=AT + 4), -3), (dict(vocab=(1 << 30) + 1), -2), (dict(lda=(1 << 22) + 16), -2),
+        (dict(ldw=(1 << 22) + 16), -2), (dict(workspace=AT + 8), -6), (dict(workspace_bytes=need - 1), -6),
         (dict(rows=0, a=0, w=0, tokens=0, workspace=0), 0)])
     for bad in (dict(rows=0), dict(vocab=0), dict(k=0), dict(top=2)):
         q = _lib.QaMmTokenLogprobsParams.from_buffer_copy(p)

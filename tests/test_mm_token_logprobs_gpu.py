@@ -135,6 +135,24 @@ def test_rows_that_lie_apart(dev):
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+@pytest.mark.parametrize("rows,vocab", [(2, 70000), (70000, 130)])
+def test_operands_beyond_32_bits(dev, rows, vocab):
+    """Rows 32 KiB apart: the last ones lie more than 2^31 bytes behind the first."""
+    pitch, k = 32768, 64
+    c = make(rows, vocab, k, dev)
+    want = ops.scaled_mm_token_logprobs(**c, top=1, vocab=vocab)
+    large = "a" if rows > vocab else "b"
+    n = max(rows, c["b"].shape[1]) if large == "b" else rows
+    store = torch.empty(n * pitch, dtype=torch.int8, device=dev)
+    rows_apart = store.view(n, pitch)[:, :k]
+    rows_apart.copy_(c["a"] if large == "a" else c["b"].t())
+    got = ops.scaled_mm_token_logprobs(**{**c, large: rows_apart if large == "a" else rows_apart.t()}, top=1, vocab=vocab)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    few = min(rows, 300)
+    part = {k_: (v[:few] if k_ in ("a", "tokens") or (k_ == "a_scales" and v.numel() > 1) else v) for k_, v in c.items()}
+    check(ops.TokenLogprobs(*(t[:few] for t in got)), part, vocab, 1)
+
+
 def test_the_same_bits_again_and_no_rows(dev):
     c = make(300, 2000, 256, dev)
     want = ops.scaled_mm_token_logprobs(**c, top=1)

@@ -94,6 +94,19 @@ def test_orders_of_the_values(dev, shape, rows):
     check(ops.token_logprobs(logits, tokens, top=17), logits, tokens, 17)
 
 
+@pytest.mark.parametrize("dtype,vocab", [("fp16", 16387), ("bf16", 16391), ("fp32", 8195), ("fp16", 24581), ("fp32", 12291)])
+@pytest.mark.parametrize("rows", [512, 700, 1030])
+def test_values_behind_the_last_whole_load(dev, dtype, vocab, rows):
+    """They are all that is left for the last segment; the best value among them, or none that counts, or only NaNs."""
+    logits, tokens = make(rows, vocab, TYPES[dtype], dev)
+    logits[1::3, -1] = 30.0
+    logits[2::3, -3:] = float("-inf")
+    check(ops.token_logprobs(logits, tokens, top=5), logits, tokens, 5)
+    logits[0, -3:] = float("nan")
+    got = ops.token_logprobs(logits, tokens, top=5)
+    assert torch.isnan(got.entropy[0]) and ((got.top_tokens >= 0) & (got.top_tokens < vocab)).all()
+
+
 @pytest.mark.parametrize("rows", [2, 600])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_masked_logits(dev, dtype, rows):

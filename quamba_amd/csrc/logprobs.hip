@@ -19,7 +19,6 @@ namespace {
 constexpr int kWaves = 4, kUnroll = 4;
 constexpr int kMaxTop = 64, kMaxSegments = 64;
 constexpr int kCandidates = 256;
-constexpr uint32_t kNoIndex = 0xffffffffu;               // of a lane's place without a value
 
 struct Part {
     float m, s, t, reserved;
@@ -71,12 +70,12 @@ __device__ __forceinline__ void take_candidates(BestEntries& best, const Candida
     for (int i = 0; i < count; i += 64) best.offer(i + lane < count ? c.at[i + lane] : 0, top, lane);
 }
 
-// The best `top` of the workgroup's values: `visit(f)` calls f(value, index) for each value of a lane, `most` is the largest of them.
-// What the lanes' largest values say is a bound that `top` values or more reach and hardly more than that do: those are put together in
-// LDS (in any order) and one wave sorts them.  Where more come than there is room for - equal values, or as many
-// alternatives as lanes - every wave keeps its own best instead and one wave merges them.  The result is wave 0's.
-template <class Visit>
-__device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, Candidates& c, Entry (&lists)[kWaves][64], int wave, int lane) {
+// The best `top` of the workgroup's values: `visit(f)` calls f(values, the largest of them, whether they are there, index) for each load of a
+// lane, `most` is the largest of all.  What the lanes' largest values say is a bound that `top` values or more reach and hardly more than
+// that do: those are put together in LDS (in any order) and one wave sorts them.  Where more come than there is room for - equal values,
+// or as many alternatives as lanes - every wave keeps its own best instead and one wave merges them.  The result is wave 0's.
+template <int V, class Visit>
+__device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, Candidates& c, Entry (&lists)[kWaves][64], Entry* waiting, int wave, int lane) {
     if (threadIdx.x == 0) c.count = 0;
     c.keys[wave][lane] = sort_wave(key_of(most), lane);
     __syncthreads();
@@ -98,26 +97,33 @@ __device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, 
         reached = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(all), top - 1));
     }
     const float bound = value_of_key(reached);
-    if (__builtin_amdgcn_ballot_w64(most >= bound)) {
-        visit([&](float v, uint32_t index) __attribute__((always_inline)) {
-            if (v >= bound && index != kNoIndex) {
-                const int at = atomicAdd(&c.count, 1);
-                if (at < kCandidates) c.at[at] = entry_of(v, index);
-            }
-        });
-    }
+    visit([&](const auto& v, float most_of, bool valid, uint32_t index) __attribute__((always_inline)) {
+        if (!__builtin_amdgcn_ballot_w64(valid && most_of >= bound)) return;
+        constexpr int N = sizeof(v) / sizeof(v[0]);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (!valid || !(v[j] >= bound)) continue;
+            const int at = atomicAdd(&c.count, 1);
+            if (at < kCandidates) c.at[at] = entry_of(v[j], index + j);
+        }
+    });
     __syncthreads();
     const int count = c.count;
     BestEntries best;
     best.clear();
-    // (a NaN reaches no bound: where nothing else is left, it is one of the waves' own best)
-    if (count <= kCandidates && count >= top) {
+    // (a NaN reaches no bound)
+    if (count <= kCandidates) {
         if (wave == 0) take_candidates(best, c, count, top, lane);
         return best;
     }
-    visit([&](float v, uint32_t index) __attribute__((always_inline)) { best.offer(index == kNoIndex ? 0 : entry_of(v, index), top, lane); });
-    lists[wave][lane] = best.mine;
+    BestOfBatches<V> run;
+    run.clear(waiting);
+    run.first_batch(most, top, lane);
+    visit([&](const auto& v, float most_of, bool valid, uint32_t index) __attribute__((always_inline)) { run.take(v, most_of, valid, index, top, lane); });
+    run.finish(top, lane);
+    lists[wave][lane] = run.best.mine;
     __syncthreads();
+    best = run.best;
     if (wave == 0)
         for (int w = 1; w < kWaves; ++w) best.mine = merge_waves(best.mine, lists[w][lane], lane);
     return best;
@@ -130,7 +136,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
     __shared__ Part s_part[kWaves];
     __shared__ Entry s_best[TOP ? kWaves : 1][64];
     __shared__ std::conditional_t<TOP && ONE, Candidates, int> s_candidates;
-    __shared__ Entry s_waiting[TOP && !ONE ? kWaves : 1][128];
+    __shared__ Entry s_waiting[TOP ? kWaves : 1][BestOfBatches<V>::kWaiting];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = blockIdx.x / segments;
     const int segment = blockIdx.x % segments;
@@ -148,7 +154,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
     r.clear();
     BestEntries best;
     best.clear();
-    BestOfBatches run;
+    BestOfBatches<V> run;
     if constexpr (TOP && !ONE) run.clear(s_waiting[wave]);
     for (int b = first; b < end; ++b) {
         Raw<T, V> raw[LOADS];
@@ -176,30 +182,17 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
 #pragma unroll
             for (int j = 0; j < V; ++j) r.add(v[u][j]);
         if constexpr (TOP && ONE) {
-            best = pick([&](auto&& f) __attribute__((always_inline)) {
+            best = pick<V>([&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
-                for (int u = 0; u < LOADS; ++u)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) f(v[u][j], at[u] < vectors ? static_cast<uint32_t>(at[u] * V + j) : kNoIndex);
-                f(rest_v, has_rest ? static_cast<uint32_t>(rest_at) : kNoIndex);
-            }, most, p.top, s_candidates, s_best, wave, lane);
+                for (int u = 0; u < LOADS; ++u) f(v[u], most_of[u], at[u] < vectors, static_cast<uint32_t>(at[u] * V));
+                const float one[1] = {rest_v};
+                f(one, rest_v, has_rest, static_cast<uint32_t>(rest_at));
+            }, most, p.top, s_candidates, s_best, s_waiting[wave], wave, lane);
         } else if constexpr (TOP) {
-            auto each = [&](auto comes_in) __attribute__((always_inline)) {
+            if (b == first) run.first_batch(most, p.top, lane);
+            else run.next_batch();
 #pragma unroll
-                for (int u = 0; u < LOADS; ++u) {
-                    if (!__builtin_amdgcn_ballot_w64(comes_in(most_of[u]))) continue;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) run.put(comes_in(v[u][j]) && at[u] < vectors, v[u][j], at[u] * V + j, p.top, lane);
-                }
-            };
-            // (what a wave has seen has lower indices than what comes: later an equal value does not come in)
-            if (b == first) {
-                run.first(most, p.top, lane);
-                const float reach = run.bound;
-                each([&](float value) { return value >= reach; });
-            } else {
-                each([&](float value) { return value > run.bound; });
-            }
+            for (int u = 0; u < LOADS; ++u) run.take(v[u], most_of[u], at[u] < vectors, static_cast<uint32_t>(at[u] * V), p.top, lane);
         }
     }
     if (ONE) {
@@ -207,8 +200,12 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
     } else if (segment == segments - 1 && wave == 0 && rest) {
         r.raise(fmaxf(r.m, rest_v));
         r.add(rest_v);
-        // (it is all there is of a last segment that has no whole load)
-        if constexpr (TOP) run.put(has_rest && (first < end ? rest_v > run.bound : rest_v == rest_v), rest_v, rest_at, p.top, lane);
+        if constexpr (TOP) {
+            // (they are all there is of a last segment that has no whole load)
+            const float one[1] = {rest_v};
+            if (first < end) run.next_batch();
+            run.take(one, rest_v, has_rest, static_cast<uint32_t>(rest_at), p.top, lane);
+        }
     }
     if constexpr (TOP && !ONE) {
         run.finish(p.top, lane);

@@ -141,36 +141,46 @@ struct BestEntries {
     }
 };
 
-// The best entries of a long run of values, a batch at a time: what may come in is put down in LDS, and once 64 are together they
-// are sorted and merged.  Until then `bound` stands for the top-th best: that many values of the first batch reach it.
+// The best entries of a long run of values, a batch of loads at a time: what may come in is put down in LDS, and once more than 64 are
+// together they are sorted and merged.  Until then `bound` stands for the top-th best: that many values of the first batch reach it.
+// (The sorting stands behind a load of V values, not behind each of them: in 32 places its code does not stay in the instruction cache.)
+template <int V>
 struct BestOfBatches {
+    static constexpr int kWaiting = 64 + 64 * V;
     BestEntries best;
-    float bound;
-    int count;             // entries waiting, at most 64 between batches
-    Entry* waiting;        // 128, of this wave alone
+    float bound, reach;    // what comes in is no smaller than `reach`
+    int count;             // entries waiting, at most 64 between loads
+    Entry* waiting;        // kWaiting of them, of this wave alone
     __device__ __forceinline__ void clear(Entry* place) {
         best.clear();
+        bound = reach = -__builtin_inff();
         count = 0;
         waiting = place;
     }
-    __device__ __forceinline__ void first(float lane_most, int top, int lane) {
-        bound = value_of_key(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sort_wave(key_of(lane_most), lane)), top - 1)));
+    __device__ __forceinline__ void first_batch(float lane_most, int top, int lane) {
+        bound = reach = value_of_key(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sort_wave(key_of(lane_most), lane)), top - 1)));
     }
-    // the values of the lanes that say so
-    __device__ __forceinline__ void put(bool wanted, float value, uint32_t index, int top, int lane) {
-        const uint64_t which = __builtin_amdgcn_ballot_w64(wanted);
-        if (!which) return;
-        const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(which >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(which), 0));
-        if (wanted) waiting[count + before] = entry_of(value, index);
-        count += __popcll(which);
-        if (count <= 64) return;
-        wave_order();
-        best.take(waiting[lane], top, lane);
-        const Entry more = lane < count - 64 ? waiting[64 + lane] : 0;
-        wave_order();
-        waiting[lane] = more;
-        count -= 64;
-        bound = fmaxf(bound, value_of(best.last));
+    // what a wave has seen has lower indices than what comes: an equal value does not come in any more
+    __device__ __forceinline__ void next_batch() { reach = value_of_key(key_of(bound) + 1); }
+    // N values of each lane that says so, index and following
+    template <int N>
+    __device__ __forceinline__ void take(const float (&v)[N], float most, bool valid, uint32_t index, int top, int lane) {
+        if (!__builtin_amdgcn_ballot_w64(valid && most >= reach)) return;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const bool wanted = valid && v[j] >= reach;
+            const uint64_t which = __builtin_amdgcn_ballot_w64(wanted);
+            const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(which >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(which), 0));
+            if (wanted) waiting[count + before] = entry_of(v[j], index + j);
+            count += __popcll(which);
+        }
+        while (count > 64) {
+            count -= 64;
+            wave_order();
+            best.take(waiting[count + lane], top, lane);
+            bound = fmaxf(bound, value_of(best.last));
+            reach = fmaxf(reach, bound);
+        }
     }
     __device__ __forceinline__ void finish(int top, int lane) {
         wave_order();

@@ -17,8 +17,6 @@ namespace {
 
 using namespace gemm;
 
-constexpr float kLn2 = 0.693147180559945309f;
-
 struct TilePart {
     float m, s, t;
     int best;              // the lowest column with the value m

@@ -1,7 +1,7 @@
 // Log probabilities of given tokens, entropies and the best alternatives of rows of logits (qa_token_logprobs).
 //
 // One pass over the logits, bound by memory while the vector units keep up: a value is converted, joins a maximum of a batch,
-// and costs an exponential and five operations more (RowStats); a lane raises its maximum once a batch of loads, not
+// and costs an exponential and four operations more (RowStats); a lane raises its maximum once a batch of loads, not
 // once a value.
 //
 // A workgroup of four waves takes a segment of a row, whole rows when there are many; the parts of a cut row go to the workspace
@@ -21,7 +21,7 @@ constexpr int kMaxTop = 64, kMaxSegments = 64;
 constexpr int kCandidates = 256;
 
 struct Part {
-    float m, s, t, reserved;
+    float m, s, t, bound;      // (bound: within a workgroup)
 };
 
 // How the rows are cut: segments of a row, batches of a segment, loads of a lane in a batch.
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
     constexpr int V = 16 / sizeof(T);                      // values a load
     __shared__ Part s_part[kWaves];
     __shared__ Entry s_best[TOP ? kWaves : 1][64];
-    __shared__ std::conditional_t<TOP && ONE, Candidates, int> s_candidates;
+    __shared__ std::conditional_t<TOP, Candidates, int> s_candidates;
     __shared__ Entry s_waiting[TOP ? kWaves : 1][BestOfBatches<V>::kWaiting];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = blockIdx.x / segments;
@@ -156,31 +156,29 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
     best.clear();
     BestOfBatches<V> run;
     if constexpr (TOP && !ONE) run.clear(s_waiting[wave]);
-    for (int b = first; b < end; ++b) {
+    // WHOLE: every lane has its loads
+    auto batch = [&](int b, auto whole_c) __attribute__((always_inline)) {
+        constexpr bool WHOLE = decltype(whole_c)::value;
         Raw<T, V> raw[LOADS];
         int at[LOADS];
         float v[LOADS][V], most_of[LOADS], most = none;
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
             at[u] = ((b * LOADS + u) * kWaves + wave) * 64 + lane;
-            if (!ONE || vectors > 0) raw[u].template load<WIDE>(logits + static_cast<int64_t>(min(at[u], vectors - 1)) * V);
+            if (!ONE || vectors > 0) raw[u].template load<WIDE>(logits + static_cast<int64_t>(WHOLE ? at[u] : min(at[u], vectors - 1)) * V);
         }
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
             most_of[u] = none;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                v[u][j] = at[u] < vectors ? raw[u].get(j) : none;
+                v[u][j] = WHOLE || at[u] < vectors ? raw[u].get(j) : none;
                 most_of[u] = fmaxf(most_of[u], v[u][j]);
             }
             most = fmaxf(most, most_of[u]);
         }
         if constexpr (ONE) most = fmaxf(most, rest_v);
-        r.raise(fmaxf(r.m, most));
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u)
-#pragma unroll
-            for (int j = 0; j < V; ++j) r.add(v[u][j]);
+        r.add_batch(v, most);
         if constexpr (TOP && ONE) {
             best = pick<V>([&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
@@ -192,8 +190,16 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
             if (b == first) run.first_batch(most, p.top, lane);
             else run.next_batch();
 #pragma unroll
-            for (int u = 0; u < LOADS; ++u) run.take(v[u], most_of[u], at[u] < vectors, static_cast<uint32_t>(at[u] * V), p.top, lane);
+            for (int u = 0; u < LOADS; ++u) run.take(v[u], most_of[u], WHOLE || at[u] < vectors, static_cast<uint32_t>(at[u] * V), p.top, lane);
         }
+    };
+    if constexpr (ONE) {
+        batch(first, std::false_type{});
+    } else {
+        const int whole = min(end, vectors / (kWaves * 64 * LOADS));
+        int b = first;
+        for (; b < whole; ++b) batch(b, std::true_type{});
+        for (; b < end; ++b) batch(b, std::false_type{});
     }
     if (ONE) {
         r.add(rest_v);
@@ -207,19 +213,40 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
             run.take(one, rest_v, has_rest, static_cast<uint32_t>(rest_at), p.top, lane);
         }
     }
-    if constexpr (TOP && !ONE) {
-        run.finish(p.top, lane);
-        best = run.best;
-    }
     r = wave_stats(r);
-    if (lane == 0) s_part[wave] = {r.m, r.s, r.t, 0.0f};
-    if constexpr (TOP && !ONE) s_best[wave][lane] = best.mine;
+    if (lane == 0) s_part[wave] = {r.m, r.s, r.t, run.bound};
+    bool sorted = false;                                   // (of the same value in all waves)
+    if constexpr (TOP && !ONE) {
+        // what waits reaches the bound of its wave; what counts, the largest of the waves' bounds
+        if (threadIdx.x == 0) s_candidates.count = 0;
+        if (lane == 0) s_candidates.keys[wave][0] = run.best.last != 0;
+        __syncthreads();
+        float bound = s_part[0].bound;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            bound = fmaxf(bound, s_part[w].bound);
+            sorted |= s_candidates.keys[w][0] != 0;
+        }
+        if (!sorted) {
+            static_assert(kCandidates >= 64 * kWaves, "room for all that wait");
+            run.wave_order();
+            const Entry e = lane < run.count ? s_waiting[wave][lane] : 0;
+            if (e != 0 && value_of(e) >= bound) s_candidates.at[atomicAdd(&s_candidates.count, 1)] = e;
+        } else {
+            run.finish(p.top, lane);
+            best = run.best;
+            s_best[wave][lane] = best.mine;
+        }
+    }
     __syncthreads();
     if (wave != 0) return;
+    if constexpr (TOP && !ONE) {
+        if (!sorted) take_candidates(best, s_candidates, s_candidates.count, p.top, lane);
+    }
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) {
         r.join({s_part[w].m, s_part[w].s, s_part[w].t});
-        if constexpr (TOP && !ONE) best.mine = merge_waves(best.mine, s_best[w][lane], lane);
+        if (TOP && !ONE && sorted) best.mine = merge_waves(best.mine, s_best[w][lane], lane);
     }
     if (segments == 1) {
         answer(p, row, r, best.mine, lane);

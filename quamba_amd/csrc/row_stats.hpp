@@ -12,7 +12,7 @@
 namespace qa {
 namespace lm {
 
-constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr float kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
@@ -32,6 +32,33 @@ struct RowStats {
         const float d = value - m, e = exp_fast(d);
         s += e;
         t = __builtin_fmaf(fmaxf(d, -200.0f), e, t);                       // (e is 0 from -104 on)
+    }
+    // a batch of values, the largest of them `most`.  With c = log2(e) and r the rounded m c an exponent is one fused step, v c - r; what the
+    // rounding left out, m c - r, is exact in one number and corrects the sums.  (Where m c might not be a number the differences are
+    // taken as they are; a product of 0 and -inf has no place here, and e is 0 long before the exponent is -200.)
+    template <int A, int B>
+    __device__ __forceinline__ void add_batch(const float (&v)[A][B], float most) {
+        raise(fmaxf(m, most));
+        if (__builtin_amdgcn_ballot_w64(fabsf(m) > 1e38f)) {
+#pragma unroll
+            for (int i = 0; i < A; ++i)
+#pragma unroll
+                for (int j = 0; j < B; ++j) add(v[i][j]);
+            return;
+        }
+        const float r = m * kLog2e, rest = __builtin_fmaf(m, kLog2e, -r);
+        float sum = 0.0f, weighted = 0.0f;
+#pragma unroll
+        for (int i = 0; i < A; ++i)
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                const float d = __builtin_fmaf(v[i][j], kLog2e, -r), e = __builtin_amdgcn_exp2f(d);
+                sum += e;
+                weighted = __builtin_fmaf(fmaxf(d, -200.0f), e, weighted);
+            }
+        const float f = __builtin_amdgcn_exp2f(-rest);
+        s = __builtin_fmaf(sum, f, s);
+        t = __builtin_fmaf((weighted - rest * sum) * f, kLn2, t);
     }
     __device__ __forceinline__ void join(RowStats o) {
         const float most = fmaxf(m, o.m);
@@ -132,7 +159,8 @@ struct BestEntries {
     __device__ __forceinline__ void clear() { mine = last = 0; }
     // one candidate per lane (0: none)
     __device__ __forceinline__ void take(Entry e, int top, int lane) {
-        mine = merge_waves(mine, sort_wave(e, lane), lane);
+        const Entry sorted = sort_wave(e, lane);
+        mine = __builtin_amdgcn_ballot_w64(mine != 0) ? merge_waves(mine, sorted, lane) : sorted;
         last = entry_of_lane(mine, top - 1);
     }
     // the same, skipped where none comes in

@@ -234,3 +234,25 @@ def test_refusals(dev):
             ops.token_logprobs(**{"logits": logits, "tokens": tokens, **bad})
     with pytest.raises(NotImplementedError):
         ops.token_logprobs(logits, tokens, top=65)
+
+
+def test_answers_are_tensors_of_their_own(dev):
+    """Some lie in one allocation, and none of them notices: writing one leaves the others, copies and files hold what they should."""
+    import copy
+    import io
+    logits, tokens = make(6, 300, torch.float16, dev)
+    got = ops.token_logprobs(logits, tokens, top=3)
+    want = [t.clone() for t in got]
+    assert [t.dtype for t in got] == [torch.float32, torch.float32, torch.float32, torch.int64] and all(t.is_contiguous() and not t.requires_grad for t in got)
+    for i, t in enumerate(got):
+        t.zero_()
+        assert (t == 0).all() and all(torch.equal(a, b) for a, b in zip(got[i + 1:], want[i + 1:]))
+    again = ops.token_logprobs(logits, tokens, top=3)
+    file = io.BytesIO()
+    torch.save(list(again), file)
+    file.seek(0)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(again, torch.load(file, weights_only=True), copy.deepcopy(list(again))))
+    # usable as a leaf and in a graph of gradients
+    leaf = again.logprobs.requires_grad_()
+    (2 * leaf).sum().backward()
+    assert (leaf.grad == 2).all()

@@ -4,8 +4,8 @@
 // and costs an exponential and four operations more (RowStats); a lane raises its maximum once a batch of loads, not
 // once a value.
 //
-// A workgroup of four waves takes a segment of a row, whole rows when there are many; the parts of a cut row go to the workspace
-// and a second launch joins them.  With few rows a segment is one batch, and what costs is not the bytes but what happens one after the
+// A wave takes a row where there are many, four of them a segment of a row otherwise; the parts of a cut row go to the workspace and a
+// second launch joins them.  With few rows a segment is one batch, and what costs is not the bytes but what happens one after the
 // other: there the best entries are picked out of the registers by a bound (pick).  In a longer segment a wave keeps its own, and loads in
 // which no value is above the last of them are passed over with one comparison per lane (BestOfBatches).
 #include "row_stats.hpp"
@@ -24,16 +24,22 @@ struct Part {
     float m, s, t, bound;      // (bound: within a workgroup)
 };
 
-// How the rows are cut: segments of a row, batches of a segment, loads of a lane in a batch.
+// How the rows are cut: waves of a segment, segments of a row, batches of a segment, loads of a lane in a batch.
 struct Cut {
-    int segments, batches, loads;
+    int waves, segments, batches, loads;
 };
 Cut cut_of(int rows, int vocab, int type) {
     const int load = kWaves * 64 * (type == QA_LM_F32 ? 4 : 8), short_batches = (vocab + load - 1) / load, batches = (vocab + load * kUnroll - 1) / (load * kUnroll);
-    const int wanted = static_cast<int>(std::min<int64_t>((4LL * compute_units() + rows - 1) / rows, kMaxSegments));
-    if (short_batches <= wanted) return {short_batches, 1, 1};
+    // A wave for each row where there are waves enough for that, or little for each of them: what comes once a row then comes once, and nothing
+    // waits at barriers (us by four waves and by one: 30000 x 1000 fp16 top 5 90, 36; 20000 x 4000 fp16 47, 34, top 5 82, 45; 4096 x 50280 fp16
+    // 79, 79, top 5 98, 85; but 3200 x 50280 58, 64, 2000 x 20000 top 5 27, 32; 1024 x 4000 6.1, 5.6; 1024 x 4000 fp32, four batches of a wave,
+    // top 5 9.4, 11.2).
+    const int cus = compute_units();
+    if (rows >= 16 * cus || (rows >= cus && vocab <= 2 * kUnroll * load / kWaves)) return {1, 1, batches * kWaves, kUnroll};
+    const int wanted = static_cast<int>(std::min<int64_t>((4LL * cus + rows - 1) / rows, kMaxSegments));
+    if (short_batches <= wanted) return {kWaves, short_batches, 1, 1};
     const int each = (batches + std::min(batches, wanted) - 1) / std::min(batches, wanted);
-    return {(batches + each - 1) / each, each, kUnroll};
+    return {kWaves, (batches + each - 1) / each, each, kUnroll};
 }
 
 __device__ __forceinline__ float logit_at(const QaTokenLogprobsParams& p, int64_t row, int64_t i) {
@@ -129,25 +135,28 @@ __device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, 
     return best;
 }
 
-// ONE: the segment is one batch
-template <class T, bool WIDE, bool TOP, bool ONE, int LOADS>
+// W waves take a segment; ONE: it is one batch.  With W = 1 a workgroup has kWaves whole rows.
+template <class T, bool WIDE, bool TOP, int W, bool ONE, int LOADS>
 __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogprobsParams p, int segments, int batches_each) {
     constexpr int V = 16 / sizeof(T);                      // values a load
+    static_assert(W == kWaves || (W == 1 && !ONE), "rows of a workgroup, or workgroups of a row");
     __shared__ Part s_part[kWaves];
-    __shared__ Entry s_best[TOP ? kWaves : 1][64];
-    __shared__ std::conditional_t<TOP, Candidates, int> s_candidates;
+    __shared__ Entry s_best[TOP && W > 1 ? kWaves : 1][64];
+    __shared__ std::conditional_t<TOP && (W > 1), Candidates, int> s_candidates;
     __shared__ Entry s_waiting[TOP ? kWaves : 1][BestOfBatches<V>::kWaiting];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = blockIdx.x / segments;
-    const int segment = blockIdx.x % segments;
+    const int sub = W > 1 ? wave : 0;
+    const int64_t row = W > 1 ? blockIdx.x / segments : static_cast<int64_t>(blockIdx.x) * kWaves + wave;
+    const int segment = W > 1 ? blockIdx.x % segments : 0;
+    if (W == 1 && row >= p.rows) return;                   // (no wave waits for another one then)
     const T* const logits = static_cast<const T*>(p.logits) + row * p.row_stride;
     const int vectors = p.vocab / V, rest = p.vocab - vectors * V;
-    const int first = segment * batches_each, end = ONE ? first + 1 : min(first + batches_each, (vectors + kWaves * 64 * LOADS - 1) / (kWaves * 64 * LOADS));
+    const int first = segment * batches_each, end = ONE ? first + 1 : min(first + batches_each, (vectors + W * 64 * LOADS - 1) / (W * 64 * LOADS));
     const float none = -__builtin_inff();
 
     // fewer than V values behind the last whole load: one each in the first lanes of the last segment
     const int rest_at = vectors * V + lane;
-    const bool has_rest = segment == segments - 1 && wave == 0 && lane < rest;
+    const bool has_rest = segment == segments - 1 && sub == 0 && lane < rest;
     float rest_v = none;
     if (has_rest) rest_v = static_cast<float>(logits[rest_at]);
     RowStats r;
@@ -164,7 +173,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
         float v[LOADS][V], most_of[LOADS], most = none;
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
-            at[u] = ((b * LOADS + u) * kWaves + wave) * 64 + lane;
+            at[u] = ((b * LOADS + u) * W + sub) * 64 + lane;
             if (!ONE || vectors > 0) raw[u].template load<WIDE>(logits + static_cast<int64_t>(WHOLE ? at[u] : min(at[u], vectors - 1)) * V);
         }
 #pragma unroll
@@ -178,7 +187,8 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
             most = fmaxf(most, most_of[u]);
         }
         if constexpr (ONE) most = fmaxf(most, rest_v);
-        r.add_batch(v, most);
+        const int wanted = (vectors - (b * LOADS * W + sub) * 64 + W * 64 - 1) / (W * 64);         // loads with a lane that has one
+        r.add_batch(v, WHOLE ? LOADS : __builtin_amdgcn_readfirstlane(wanted), most);
         if constexpr (TOP && ONE) {
             best = pick<V>([&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
@@ -188,7 +198,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
             }, most, p.top, s_candidates, s_best, s_waiting[wave], wave, lane);
         } else if constexpr (TOP) {
             if (b == first) run.first_batch(most, p.top, lane);
-            else run.next_batch();
+            else run.next_batch(p.top);
 #pragma unroll
             for (int u = 0; u < LOADS; ++u) run.take(v[u], most_of[u], WHOLE || at[u] < vectors, static_cast<uint32_t>(at[u] * V), p.top, lane);
         }
@@ -196,65 +206,70 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
     if constexpr (ONE) {
         batch(first, std::false_type{});
     } else {
-        const int whole = min(end, vectors / (kWaves * 64 * LOADS));
+        const int whole = min(end, vectors / (W * 64 * LOADS));
         int b = first;
         for (; b < whole; ++b) batch(b, std::true_type{});
         for (; b < end; ++b) batch(b, std::false_type{});
     }
     if (ONE) {
         r.add(rest_v);
-    } else if (segment == segments - 1 && wave == 0 && rest) {
+    } else if (segment == segments - 1 && sub == 0 && rest) {
         r.raise(fmaxf(r.m, rest_v));
         r.add(rest_v);
         if constexpr (TOP) {
             // (they are all there is of a last segment that has no whole load)
             const float one[1] = {rest_v};
-            if (first < end) run.next_batch();
+            run.next_batch(p.top);
             run.take(one, rest_v, has_rest, static_cast<uint32_t>(rest_at), p.top, lane);
         }
     }
     r = wave_stats(r);
-    if (lane == 0) s_part[wave] = {r.m, r.s, r.t, run.bound};
-    bool sorted = false;                                   // (of the same value in all waves)
-    if constexpr (TOP && !ONE) {
-        // what waits reaches the bound of its wave; what counts, the largest of the waves' bounds
-        if (threadIdx.x == 0) s_candidates.count = 0;
-        if (lane == 0) s_candidates.keys[wave][0] = run.best.last != 0;
+    if constexpr (W == 1) {
+        if constexpr (TOP) run.finish(p.top, lane);
+        answer(p, row, r, run.best.mine, lane);
+    } else {
+        if (lane == 0) s_part[wave] = {r.m, r.s, r.t, run.bound};
+        bool sorted = false;                                   // (of the same value in all waves)
+        if constexpr (TOP && !ONE) {
+            // what waits reaches the bound of its wave; what counts, the largest of the waves' bounds
+            if (threadIdx.x == 0) s_candidates.count = 0;
+            if (lane == 0) s_candidates.keys[wave][0] = run.best.last != 0;
+            __syncthreads();
+            float bound = s_part[0].bound;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                bound = fmaxf(bound, s_part[w].bound);
+                sorted |= s_candidates.keys[w][0] != 0;
+            }
+            if (!sorted) {
+                static_assert(kCandidates >= 64 * kWaves, "room for all that wait");
+                run.wave_order();
+                const Entry e = lane < run.count ? s_waiting[wave][lane] : 0;
+                if (e != 0 && value_of(e) >= bound) s_candidates.at[atomicAdd(&s_candidates.count, 1)] = e;
+            } else {
+                run.finish(p.top, lane);
+                best = run.best;
+                s_best[wave][lane] = best.mine;
+            }
+        }
         __syncthreads();
-        float bound = s_part[0].bound;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            bound = fmaxf(bound, s_part[w].bound);
-            sorted |= s_candidates.keys[w][0] != 0;
+        if (wave != 0) return;
+        if constexpr (TOP && !ONE) {
+            if (!sorted) take_candidates(best, s_candidates, s_candidates.count, p.top, lane);
         }
-        if (!sorted) {
-            static_assert(kCandidates >= 64 * kWaves, "room for all that wait");
-            run.wave_order();
-            const Entry e = lane < run.count ? s_waiting[wave][lane] : 0;
-            if (e != 0 && value_of(e) >= bound) s_candidates.at[atomicAdd(&s_candidates.count, 1)] = e;
-        } else {
-            run.finish(p.top, lane);
-            best = run.best;
-            s_best[wave][lane] = best.mine;
-        }
-    }
-    __syncthreads();
-    if (wave != 0) return;
-    if constexpr (TOP && !ONE) {
-        if (!sorted) take_candidates(best, s_candidates, s_candidates.count, p.top, lane);
-    }
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-        r.join({s_part[w].m, s_part[w].s, s_part[w].t});
-        if (TOP && !ONE && sorted) best.mine = merge_waves(best.mine, s_best[w][lane], lane);
+        for (int w = 1; w < kWaves; ++w) {
+            r.join({s_part[w].m, s_part[w].s, s_part[w].t});
+            if (TOP && !ONE && sorted) best.mine = merge_waves(best.mine, s_best[w][lane], lane);
+        }
+        if (segments == 1) {
+            answer(p, row, r, best.mine, lane);
+            return;
+        }
+        Part* const parts = static_cast<Part*>(p.workspace);
+        if (lane == 0) parts[blockIdx.x] = {r.m, r.s, r.t, 0.0f};
+        if (TOP && lane < p.top) reinterpret_cast<Entry*>(parts + static_cast<int64_t>(p.rows) * segments)[static_cast<int64_t>(blockIdx.x) * p.top + lane] = best.mine;
     }
-    if (segments == 1) {
-        answer(p, row, r, best.mine, lane);
-        return;
-    }
-    Part* const parts = static_cast<Part*>(p.workspace);
-    if (lane == 0) parts[blockIdx.x] = {r.m, r.s, r.t, 0.0f};
-    if (TOP && lane < p.top) reinterpret_cast<Entry*>(parts + static_cast<int64_t>(p.rows) * segments)[static_cast<int64_t>(blockIdx.x) * p.top + lane] = best.mine;
 }
 
 // A row's segments.  Their best entries, each segment's in order, are shared out among the waves: whole lists, merged as they are, or with
@@ -306,13 +321,15 @@ template <class T>
 int launch(const QaTokenLogprobsParams& p, hipStream_t stream) {
     const Cut cut = cut_of(p.rows, p.vocab, p.logits_type);
     const bool wide = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.row_stride * static_cast<int64_t>(sizeof(T)) % 16 == 0;
-    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.rows) * cut.segments)), block(64 * kWaves);
+    const bool by_waves = cut.waves == 1;
+    const dim3 grid(static_cast<unsigned>(by_waves ? (static_cast<int64_t>(p.rows) + kWaves - 1) / kWaves : static_cast<int64_t>(p.rows) * cut.segments)), block(64 * kWaves);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, cut.segments, cut.batches); };
     auto of_wide = [&](auto wide_c) {
         constexpr bool WIDE = decltype(wide_c)::value;
-        if (cut.loads == 1) p.top ? go(token_logprobs_kernel<T, WIDE, true, true, 1>) : go(token_logprobs_kernel<T, WIDE, false, true, 1>);
-        else if (cut.batches == 1) p.top ? go(token_logprobs_kernel<T, WIDE, true, true, kUnroll>) : go(token_logprobs_kernel<T, WIDE, false, true, kUnroll>);
-        else p.top ? go(token_logprobs_kernel<T, WIDE, true, false, kUnroll>) : go(token_logprobs_kernel<T, WIDE, false, false, kUnroll>);
+        if (by_waves) p.top ? go(token_logprobs_kernel<T, WIDE, true, 1, false, kUnroll>) : go(token_logprobs_kernel<T, WIDE, false, 1, false, kUnroll>);
+        else if (cut.loads == 1) p.top ? go(token_logprobs_kernel<T, WIDE, true, kWaves, true, 1>) : go(token_logprobs_kernel<T, WIDE, false, kWaves, true, 1>);
+        else if (cut.batches == 1) p.top ? go(token_logprobs_kernel<T, WIDE, true, kWaves, true, kUnroll>) : go(token_logprobs_kernel<T, WIDE, false, kWaves, true, kUnroll>);
+        else p.top ? go(token_logprobs_kernel<T, WIDE, true, kWaves, false, kUnroll>) : go(token_logprobs_kernel<T, WIDE, false, kWaves, false, kUnroll>);
     };
     wide ? of_wide(std::true_type{}) : of_wide(std::false_type{});
     if (cut.segments > 1) {

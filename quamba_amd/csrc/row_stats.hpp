@@ -36,26 +36,31 @@ struct RowStats {
     // a batch of values, the largest of them `most`.  With c = log2(e) and r the rounded m c an exponent is one fused step, v c - r; what the
     // rounding left out, m c - r, is exact in one number and corrects the sums.  (Where m c might not be a number the differences are
     // taken as they are; a product of 0 and -inf has no place here, and e is 0 long before the exponent is -200.)
+    // `loads` of the A groups are there (the same number in all lanes).
     template <int A, int B>
-    __device__ __forceinline__ void add_batch(const float (&v)[A][B], float most) {
+    __device__ __forceinline__ void add_batch(const float (&v)[A][B], int loads, float most) {
         raise(fmaxf(m, most));
         if (__builtin_amdgcn_ballot_w64(fabsf(m) > 1e38f)) {
 #pragma unroll
-            for (int i = 0; i < A; ++i)
+            for (int i = 0; i < A; ++i) {
+                if (i >= loads) break;
 #pragma unroll
                 for (int j = 0; j < B; ++j) add(v[i][j]);
+            }
             return;
         }
         const float r = m * kLog2e, rest = __builtin_fmaf(m, kLog2e, -r);
         float sum = 0.0f, weighted = 0.0f;
 #pragma unroll
-        for (int i = 0; i < A; ++i)
+        for (int i = 0; i < A; ++i) {
+            if (i >= loads) break;
 #pragma unroll
             for (int j = 0; j < B; ++j) {
                 const float d = __builtin_fmaf(v[i][j], kLog2e, -r), e = __builtin_amdgcn_exp2f(d);
                 sum += e;
                 weighted = __builtin_fmaf(fmaxf(d, -200.0f), e, weighted);
             }
+        }
         const float f = __builtin_amdgcn_exp2f(-rest);
         s = __builtin_fmaf(sum, f, s);
         t = __builtin_fmaf((weighted - rest * sum) * f, kLn2, t);
@@ -177,22 +182,24 @@ struct BestOfBatches {
     static constexpr int kWaiting = 64 + 64 * V;
     BestEntries best;
     float bound, reach;    // what comes in is no smaller than `reach`
+    int seen;              // values so far
     int count;             // entries waiting, at most 64 between loads
     Entry* waiting;        // kWaiting of them, of this wave alone
     __device__ __forceinline__ void clear(Entry* place) {
         best.clear();
         bound = reach = -__builtin_inff();
-        count = 0;
+        seen = count = 0;
         waiting = place;
     }
     __device__ __forceinline__ void first_batch(float lane_most, int top, int lane) {
         bound = reach = value_of_key(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sort_wave(key_of(lane_most), lane)), top - 1)));
     }
-    // what a wave has seen has lower indices than what comes: an equal value does not come in any more
-    __device__ __forceinline__ void next_batch() { reach = value_of_key(key_of(bound) + 1); }
+    // what a wave has seen has lower indices than what comes: an equal value does not come in any more (once there were `top` values)
+    __device__ __forceinline__ void next_batch(int top) { reach = seen >= top ? value_of_key(key_of(bound) + 1) : bound; }
     // N values of each lane that says so, index and following
     template <int N>
     __device__ __forceinline__ void take(const float (&v)[N], float most, bool valid, uint32_t index, int top, int lane) {
+        seen += N * __popcll(__builtin_amdgcn_ballot_w64(valid));
         if (!__builtin_amdgcn_ballot_w64(valid && most >= reach)) return;
 #pragma unroll
         for (int j = 0; j < N; ++j) {

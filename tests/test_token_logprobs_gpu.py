@@ -69,6 +69,17 @@ def test_vocabularies(dev, vocab, dtype):
         check(ops.token_logprobs(logits, tokens, top=top), logits, tokens, top)
 
 
+@pytest.mark.parametrize("rows,vocab", [(256, 7), (257, 64), (1000, 513), (300, 2048), (301, 2049), (259, 4096), (258, 4097), (4097, 2500), (4096, 9001)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows(dev, dtype, rows, vocab):
+    """Rows of a wave each; the last workgroup has fewer of them than waves."""
+    for top in (0, min(vocab, 6), min(vocab, 64)):
+        logits, tokens = make(rows, vocab, TYPES[dtype], dev)
+        logits[5] = float("-inf")
+        logits[5, vocab // 2] = 1.0
+        check(ops.token_logprobs(logits, tokens, top=top), logits, tokens, top)
+
+
 @pytest.mark.parametrize("top", [0, 1, 2, 5, 20, 63, 64])
 @pytest.mark.parametrize("rows", [1, 40, 1500])
 def test_numbers_of_alternatives(dev, top, rows):
@@ -84,9 +95,9 @@ def test_large_vocabularies(dev, dtype, vocab, rows):
 
 
 @pytest.mark.parametrize("shape", ["rising", "falling", "equal", "one hot", "two values"])
-@pytest.mark.parametrize("rows", [1, 700])
+@pytest.mark.parametrize("rows", [1, 700, 4100])
 def test_orders_of_the_values(dev, shape, rows):
-    V = 20011
+    V = 20011 if rows < 1000 else 5003
     row = {"rising": torch.linspace(-9, 9, V), "falling": torch.linspace(9, -9, V), "equal": torch.full((V,), 1.25),
            "one hot": torch.zeros(V).index_fill_(0, torch.tensor([V - 1]), 80.0), "two values": (torch.arange(V) % 3 == 1).float()}[shape]
     logits = row.repeat(rows, 1).to(dev)
@@ -107,16 +118,16 @@ def test_values_behind_the_last_whole_load(dev, dtype, vocab, rows):
     assert torch.isnan(got.entropy[0]) and ((got.top_tokens >= 0) & (got.top_tokens < vocab)).all()
 
 
-@pytest.mark.parametrize("rows", [2, 600])
+@pytest.mark.parametrize("rows", [2, 600, 4100])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_masked_logits(dev, dtype, rows):
     """-inf and the type's lowest value in masked places, given tokens among them; fewer values left than alternatives asked for."""
-    V = 9001
+    V = 9001 if rows < 1000 else 3001
     for fill in (float("-inf"), torch.finfo(TYPES[dtype]).min):
         logits, tokens = make(rows, V, TYPES[dtype], dev)
         hidden = torch.rand(rows, V, generator=torch.Generator().manual_seed(3)) < 0.5
         hidden[0] = True
-        hidden[0, [4, 8000, 8999]] = False
+        hidden[0, [4, 2000, V - 2]] = False
         logits.masked_fill_(hidden.to(dev), fill)
         tokens[0] = 7
         check(ops.token_logprobs(logits, tokens, top=6), logits, tokens, 6)
@@ -127,7 +138,7 @@ def test_masked_logits(dev, dtype, rows):
 
 
 @pytest.mark.parametrize("vocab", [5, 3000, 50280])
-@pytest.mark.parametrize("rows", [4, 900])
+@pytest.mark.parametrize("rows", [4, 900, 4100])
 def test_rows_without_a_distribution(dev, vocab, rows):
     """All masked, a NaN, an infinity: NaN in that row alone, and indices that lie in the row."""
     logits, tokens = make(rows, vocab, torch.float32, dev)
@@ -195,7 +206,7 @@ def test_rows_beyond_32_bits(dev):
 
 def test_the_same_bits_again(dev):
     """No sum depends on the order in which workgroups end."""
-    for rows in (1, 300):
+    for rows in (1, 300, 4099):
         logits, tokens = make(rows, 50280, torch.float16, dev)
         want = ops.token_logprobs(logits, tokens, top=5)
         for _ in range(3):

@@ -72,9 +72,17 @@ struct RowStats {
         s += o.s;
         t += o.t;
     }
-    __device__ __forceinline__ float entropy() const { return logf(s) - t / s; }
+    // (s of a row with all of its weight on one value is 1 to within a rounding: neither answer may pass 0 for that, as callers take
+    // logarithms of 1 - p; a NaN stays one)
+    __device__ __forceinline__ float entropy() const {
+        const float h = logf(s) - t / s;
+        return h < 0.0f ? 0.0f : h;
+    }
     // log probability of a value; NaN where the row has no distribution
-    __device__ __forceinline__ float logprob(float value) const { return s > 0.0f ? (value - m) - logf(s) : __builtin_nanf(""); }
+    __device__ __forceinline__ float logprob(float value) const {
+        const float lp = s > 0.0f ? (value - m) - logf(s) : __builtin_nanf("");
+        return lp > 0.0f ? 0.0f : lp;
+    }
 };
 
 // over the wave, in every lane

@@ -71,6 +71,16 @@ def test_whole_heads(dev, rows, vocab, k):
     check(ops.scaled_mm_token_logprobs(**c, top=1, vocab=vocab), c, vocab, 1)
 
 
+@pytest.mark.parametrize("rows", [6, 300])
+def test_certain_tokens(dev, rows):
+    """Logits so far apart that most rows have all of their weight on one token: on the right side of 0"""
+    c = make(rows, 500, 256, dev, size=3000.0)
+    c["tokens"] = logits_of(c, 500).argmax(-1).to(dev)
+    got = ops.scaled_mm_token_logprobs(**c, top=1, vocab=500)
+    check(got, c, 500, 1)
+    assert (got.logprobs <= 0).all() and (got.top_logprobs <= 0).all() and (got.entropy >= 0).all()
+
+
 @pytest.mark.parametrize("rows", [3, 70, 300])
 def test_columns_behind_the_vocabulary_count_for_nothing(dev, rows):
     c = make(rows, 500, 256, dev, pad=300)

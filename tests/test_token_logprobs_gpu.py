@@ -137,6 +137,19 @@ def test_masked_logits(dev, dtype, rows):
     assert torch.allclose(got.logprobs, torch.full_like(got.logprobs, -np.log(V)), rtol=1e-6) and (got.top_tokens == torch.tensor([0, 1], device=dev)).all()
 
 
+@pytest.mark.parametrize("vocab", [9, 2500])
+@pytest.mark.parametrize("rows", [1, 300, 4100])
+def test_certain_tokens(dev, rows, vocab):
+    """All of the weight on one token: its log probability and the entropy are 0 to within the bounds, and on the right side of it"""
+    g = torch.Generator().manual_seed(rows + vocab)
+    logits, tokens = torch.full((rows, vocab), -3e4), torch.randint(0, vocab, (rows,), generator=g)
+    logits[torch.arange(rows), tokens] = 20 * torch.randn(rows, generator=g)
+    logits, tokens = logits.to(dev), tokens.to(dev)
+    got = ops.token_logprobs(logits, tokens, 2)
+    check(got, logits, tokens, 2)
+    assert (got.logprobs <= 0).all() and (got.top_logprobs <= 0).all() and (got.entropy >= 0).all()
+
+
 @pytest.mark.parametrize("vocab", [5, 3000, 50280])
 @pytest.mark.parametrize("rows", [4, 900, 4100])
 def test_rows_without_a_distribution(dev, vocab, rows):

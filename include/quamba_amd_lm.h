@@ -4,7 +4,8 @@
  *
  * The conventions are those of quamba_amd.h: device pointers, strides in elements, the HIP stream as void*, QaStatus codes; no
  * allocation, no synchronisation, no state between calls.  A call over no rows returns QA_OK without a launch, and its tensors
- * may then be null.  The parameter blocks below have a version of their own, qa_lm_abi_version().
+ * may then be null.  A launch has at most 2^32 - 1 threads: calls that would need more return QA_ERR_SHAPE (rows of one wave's width: from
+ * 2^26 of them on).  The parameter blocks below have a version of their own, qa_lm_abi_version().
  */
 #ifndef QUAMBA_AMD_LM_H
 #define QUAMBA_AMD_LM_H
@@ -31,7 +32,7 @@ typedef enum QaGateAct { QA_GATE_PLAIN = 0, QA_GATE_SIGMOID = 1, QA_GATE_SILU = 
  * all in fp32; v is not rounded on its way into y.  residual_out (null: not wanted) gets v; it may be `residual` itself and
  * must not overlap an input otherwise.  out gets y, or with QA_LM_I8 the saturated rint(y / s): s is out_scale (a normal number above 0), or with
  * dynamic_scale max(max|y|, 1e-5) / 127 of the row, written to scales.  A row with a NaN or an infinity, or whose
- * squares pass fp32 (values from some 1e18 on), is NaN as a whole: its y, or its scale.
+ * squares pass fp32 (values from some 1e18 on), is NaN as a whole: its y, or its scale (codes by out_scale mean nothing then).
  */
 typedef struct QaAddNormParams {
     int32_t rows, dim;
@@ -91,7 +92,7 @@ int qa_token_logprobs(const QaTokenLogprobsParams* p, void* stream);
  * qa_gemm_w8a8, in fp32 and never written).  top is 0 or 1.
  */
 typedef struct QaMmTokenLogprobsParams {
-    int32_t rows, vocab, k;     /* vocab up to 2^30, k a multiple of 16 */
+    int32_t rows, vocab, k;     /* rows up to 2^28, vocab up to 2^30, k a multiple of 16 */
     int32_t a_scale_numel, w_scale_numel;   /* 1 or rows, 1 or at least vocab */
     int32_t token_bytes;
     int32_t top, reserved0;

@@ -212,6 +212,7 @@ __global__ __launch_bounds__(64 * max_waves(PIECES)) void add_rmsnorm_kernel(QaA
 template <class X, class R, class P>
 int add_rmsnorm_launch(const QaAddNormParams& p, const AddNormShape& s, bool wide, hipStream_t stream) {
     const int64_t blocks = (static_cast<int64_t>(p.rows) + s.rows - 1) / s.rows;
+    if (!launchable(blocks, 64 * s.waves * s.rows)) return QA_ERR_SHAPE;
     const dim3 grid(static_cast<unsigned>(blocks)), block(64 * s.waves * s.rows);
     const bool of_block = p.post_weight || p.gate || p.scale_vector;
     auto go = [&](auto pieces_c) {

@@ -374,10 +374,10 @@ Plan plan_of(const QaMmTokenLogprobsParams& p) {
 // a tile's operands are addressed with 32-bit byte offsets
 constexpr int64_t kWidestRow = 4 << 20;
 static_assert(320 * kWidestRow < 0x70000000LL, "the widest tile");
-constexpr int kMostColumns = 1 << 30;
+constexpr int kMostColumns = 1 << 30, kMostRows = 1 << 28;     // (sums of them and a tile's stay in 32 bits, and so do the join's threads)
 
 int check(const QaMmTokenLogprobsParams& p) {
-    if (p.rows < 0 || p.vocab < 1 || p.vocab > kMostColumns || p.k < 1) return QA_ERR_SHAPE;
+    if (p.rows < 0 || p.rows > kMostRows || p.vocab < 1 || p.vocab > kMostColumns || p.k < 1) return QA_ERR_SHAPE;
     if (p.token_bytes != 4 && p.token_bytes != 8) return QA_ERR_UNSUPPORTED;
     if (p.top != 0 && p.top != 1) return QA_ERR_UNSUPPORTED;
     return QA_OK;
@@ -394,7 +394,7 @@ int launch(const QaMmTokenLogprobsParams& p, int columns, hipStream_t stream) {
     static_assert(C::kBM == kTiles[TILE].bm && C::kBN == kTiles[TILE].bn, "the tile of the table");
     const int tiles_n = (p.vocab + columns - 1) / columns;
     const int64_t tiles = static_cast<int64_t>((p.rows + C::kBM - 1) / C::kBM) * tiles_n;
-    if (tiles > 0x7fffffffLL) return QA_ERR_SHAPE;
+    if (!launchable(tiles, C::kThreads)) return QA_ERR_SHAPE;
     auto kernel = p.top ? mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES, true, TURN> : mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES, false, TURN>;
     constexpr int kLds = C::kLdsBytes + TileScales<C::kBM, C::kBN, C::kWaves>::kBytes + C::kBM * 4;
     static_assert(kLds <= 160 * 1024, "LDS of a CU");

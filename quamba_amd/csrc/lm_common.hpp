@@ -20,6 +20,9 @@ template <> struct TypeOf<QA_LM_F32> { using type = float; };
 inline int bytes_of(int type) { return type == QA_LM_I8 ? 1 : type == QA_LM_F32 ? 4 : 2; }
 inline bool is_float_type(int type) { return type == QA_LM_F16 || type == QA_LM_BF16 || type == QA_LM_F32; }
 
+// A launch counts its threads in 32 bits.
+inline bool launchable(int64_t workgroups, int64_t threads) { return workgroups <= 0xffffffffLL / threads; }
+
 // N values of T as they lie in memory.  WIDE: on 16 bytes; else anywhere a T may lie (the hardware takes such addresses).
 template <class T, int N>
 struct Raw {

@@ -97,8 +97,8 @@ __device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, 
         }
         reached = max(every, one);
     } else {
-        // the top-th largest of all of them: more steps, and fewer values than that bound lets through (20000 x 1000 top 5 66 us, 56 as
-        // above; 1 x 50280 top 64 12 us, 17 as above)
+        // the top-th largest of all of them: more steps, and fewer values than that bound lets through (1 x 50280 top 64 12 us, 17 as above;
+        // 20000 x 1000 top 5, by four waves a row, 66, 56 as above)
         const uint32_t all = merge_waves(merge_waves(c.keys[0][lane], c.keys[1][lane], lane), merge_waves(c.keys[2][lane], c.keys[3][lane], lane), lane);
         reached = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(all), top - 1));
     }
@@ -322,7 +322,9 @@ int launch(const QaTokenLogprobsParams& p, hipStream_t stream) {
     const Cut cut = cut_of(p.rows, p.vocab, p.logits_type);
     const bool wide = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.row_stride * static_cast<int64_t>(sizeof(T)) % 16 == 0;
     const bool by_waves = cut.waves == 1;
-    const dim3 grid(static_cast<unsigned>(by_waves ? (static_cast<int64_t>(p.rows) + kWaves - 1) / kWaves : static_cast<int64_t>(p.rows) * cut.segments)), block(64 * kWaves);
+    const int64_t workgroups = by_waves ? (static_cast<int64_t>(p.rows) + kWaves - 1) / kWaves : static_cast<int64_t>(p.rows) * cut.segments;
+    if (!launchable(workgroups, 64 * kWaves)) return QA_ERR_SHAPE;
+    const dim3 grid(static_cast<unsigned>(workgroups)), block(64 * kWaves);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, cut.segments, cut.batches); };
     auto of_wide = [&](auto wide_c) {
         constexpr bool WIDE = decltype(wide_c)::value;

@@ -130,3 +130,28 @@ def test_mm_token_logprobs_refusals():
         for k, v in bad.items():
             setattr(q, k, v)
         assert l.qa_mm_token_logprobs_workspace_bytes(C.byref(q)) == 0
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """Work that a launch cannot count: refused on the host, before anything is enqueued"""
+    l, most = _lib.lib(), (1 << 31) - 1
+    p = _lib.QaAddNormParams()
+    p.x_type = p.param_type = p.residual_type = p.out_type = _lib.QA_LM_F16
+    p.x = p.weight = p.out = AT
+    for dim, rows in ((8, 1 << 26), (512, most), (2560, 1 << 25), (32768, 1 << 22)):
+        p.rows, p.dim, p.x_row_stride, p.out_row_stride = rows, dim, dim, dim
+        assert l.qa_add_rmsnorm(C.byref(p), None) == -2, (dim, rows)
+    t = _lib.QaTokenLogprobsParams()
+    t.logits_type, t.token_bytes, t.top = _lib.QA_LM_F16, 8, 1
+    t.logits = t.tokens = t.logprobs = t.entropy = t.top_logprobs = t.top_tokens = AT
+    for vocab, rows in ((8, 1 << 26), (8, most), (50280, most)):
+        t.rows, t.vocab, t.row_stride = rows, vocab, vocab
+        assert l.qa_token_logprobs_workspace_bytes(C.byref(t)) == 0 and l.qa_token_logprobs(C.byref(t), None) == -2, (vocab, rows)
+    h = _lib.QaMmTokenLogprobsParams()
+    h.k = h.lda = h.ldw = 16
+    h.a_scale_numel = h.w_scale_numel = 1
+    h.token_bytes = 8
+    h.a = h.w = h.a_scale = h.w_scale = h.tokens = h.logprobs = h.entropy = h.workspace = AT
+    for vocab, rows in ((16, (1 << 28) + 1), (16, most), (1 << 30, 1 << 20)):
+        h.rows, h.vocab, h.workspace_bytes = rows, vocab, (1 << 63) - 1
+        assert l.qa_mm_token_logprobs(C.byref(h), None) == -2, (vocab, rows)

@@ -280,3 +280,13 @@ def test_answers_are_tensors_of_their_own(dev):
     leaf = again.logprobs.requires_grad_()
     (2 * leaf).sum().backward()
     assert (leaf.grad == 2).all()
+
+
+def test_in_inference_mode(dev):
+    logits, tokens = make(6, 300, torch.float16, dev)
+    want = ops.token_logprobs(logits, tokens, top=3)
+    with torch.inference_mode():
+        got = ops.token_logprobs(logits.clone(), tokens, top=3)
+        got.logprobs.add_(1).sub_(1)
+    assert all(t.is_inference() for t in got) and not any(t.is_inference() for t in want)
+    assert torch.equal(got.entropy, want.entropy) and torch.equal(got.top_tokens, want.top_tokens)

@@ -124,7 +124,7 @@ __device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, 
     }
     BestOfBatches<V> run;
     run.clear(waiting);
-    run.first_batch(most, top, lane);
+    run.batch(most, top, lane);
     visit([&](const auto& v, float most_of, bool valid, uint32_t index) __attribute__((always_inline)) { run.take(v, most_of, valid, index, top, lane); });
     run.finish(top, lane);
     lists[wave][lane] = run.best.mine;
@@ -135,9 +135,11 @@ __device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, 
     return best;
 }
 
-// W waves take a segment; ONE: it is one batch.  With W = 1 a workgroup has kWaves whole rows.
+// W waves take a segment; ONE: it is one batch.  With W = 1 a workgroup has kWaves whole rows.  Six waves a SIMD are asked for: fp16 values that are
+// kept beside their loads take three registers more than that many waves have, and 12 bytes of scratch cost less than a wave (us with five and
+// six: 500 x 256000 fp16 top 20 74, 66; 20000 x 4000 fp16 top 5 47.7, 45.4; but 2000 x 50280 top 5 49.2, 52.5).
 template <class T, bool WIDE, bool TOP, int W, bool ONE, int LOADS>
-__global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogprobsParams p, int segments, int batches_each) {
+__global__ __launch_bounds__(64 * kWaves, 6) void token_logprobs_kernel(QaTokenLogprobsParams p, int segments, int batches_each) {
     constexpr int V = 16 / sizeof(T);                      // values a load
     static_assert(W == kWaves || (W == 1 && !ONE), "rows of a workgroup, or workgroups of a row");
     __shared__ Part s_part[kWaves];
@@ -197,8 +199,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
                 f(one, rest_v, has_rest, static_cast<uint32_t>(rest_at));
             }, most, p.top, s_candidates, s_best, s_waiting[wave], wave, lane);
         } else if constexpr (TOP) {
-            if (b == first) run.first_batch(most, p.top, lane);
-            else run.next_batch(p.top);
+            run.batch(most, p.top, lane);
 #pragma unroll
             for (int u = 0; u < LOADS; ++u) run.take(v[u], most_of[u], WHOLE || at[u] < vectors, static_cast<uint32_t>(at[u] * V), p.top, lane);
         }
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(QaTokenLogp
         if constexpr (TOP) run.finish(p.top, lane);
         answer(p, row, r, run.best.mine, lane);
     } else {
-        if (lane == 0) s_part[wave] = {r.m, r.s, r.t, run.bound};
+        if (lane == 0) s_part[wave] = {r.m, r.s, r.t, value_of_key(run.bound)};
         bool sorted = false;                                   // (of the same value in all waves)
         if constexpr (TOP && !ONE) {
             // what waits reaches the bound of its wave; what counts, the largest of the waves' bounds

@@ -14,6 +14,7 @@ namespace lm {
 
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr float kLowest = -3.402823466e38f;
+constexpr float kFarthest = 1 << 20;       // (what the rounding of m log2(e) leaves out is below 2^-4 up to here)
 
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
@@ -34,13 +35,14 @@ struct RowStats {
         t = __builtin_fmaf(fmaxf(d, -200.0f), e, t);                       // (e is 0 from -104 on)
     }
     // a batch of values, the largest of them `most`.  With c = log2(e) and r the rounded m c an exponent is one fused step, v c - r; what the
-    // rounding left out, m c - r, is exact in one number and corrects the sums.  (Where m c might not be a number the differences are
-    // taken as they are; a product of 0 and -inf has no place here, and e is 0 long before the exponent is -200.)
+    // rounding left out, m c - r, is exact in one number and corrects the sums.  (It is up to 2^-24 of m c: some 1e9 from 0 the sums and the
+    // correction would be 0 and inf, so from kFarthest on the differences are taken as they are - for values that are masked with a large finite
+    // number, and in lanes that have seen none yet.  A product of 0 and -inf has no place here, and e is 0 long before the exponent is -200.)
     // `loads` of the A groups are there (the same number in all lanes).
     template <int A, int B>
     __device__ __forceinline__ void add_batch(const float (&v)[A][B], int loads, float most) {
         raise(fmaxf(m, most));
-        if (__builtin_amdgcn_ballot_w64(fabsf(m) > 1e38f)) {
+        if (__builtin_amdgcn_ballot_w64(!(fabsf(m) <= kFarthest))) {
 #pragma unroll
             for (int i = 0; i < A; ++i) {
                 if (i >= loads) break;

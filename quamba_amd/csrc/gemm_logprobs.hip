@@ -45,25 +45,28 @@ __device__ __forceinline__ float sum_over_columns(float v) {
 // A wave's TM x TN blocks: the statistics of each of its rows to parts[row_at + row], the given tokens' logits to `given`.
 // s_lds: column scales, row scales, and the low words of the tokens, of the workgroup's tile.
 //
-// All waves are in here at the same time, with nothing for the matrix cores to do: what counts is instructions a value.  With z = s_col * acc
-// (turned over where the row's scale is negative) and c = |s_row| log2(e) an exponent is one fused step, z c - r for r the rounded
-// z_max c; the rest of that rounding, z_max c - r, is exact in one number per row and corrects the sums.  s and t are sums of 2^d and of
-// d 2^d until they leave.  Ten instructions' time a value, four of it the exponential's (fifteen with a difference, a product, a clamp and
-// the best column each on its own).
-// PLAIN: all of the wave's columns are the vocabulary's and none of its rows has a negative scale.
+// All waves are in here at the same time, with nothing for the matrix cores to do: what counts is instructions a value.
+// PLAIN: with z = s_col * acc and c = s_row log2(e) an exponent is one fused step, z c - r for r the rounded z_max c; the rest of that
+// rounding, z_max c - r, is exact in one number per row and corrects the sums.  s and t are sums of 2^d and of d 2^d until they leave.  Ten
+// instructions' time a value, four of it the exponential's (fifteen with a difference, a product, a clamp and the best column each on its
+// own).  This holds for columns that are all the vocabulary's, scales of rows that are none of them negative, and logits that the scales
+// keep below kFarthest (plain_scales): every d is a number then, and the rest small.
+// Otherwise the logits are formed as they would be written and taken as RowStats takes them: -inf is masked out (a column behind the
+// vocabulary's end is that too), a NaN or +inf leaves a NaN in s.
 template <bool PLAIN, bool TOP, int TM, int TN, int BM, int BN, class V, int NI, int NJ>
 __device__ __forceinline__ void tile_stats(const QaMmTokenLogprobsParams& p, V (&acc)[NI][NJ], const float* s_lds, int row_at, int col_at, int m0, int n0, int n_end, int lane,
                                            TilePart* parts, float* given) {
     using Q = QuadView<V>;
     constexpr int kQuads = TN * 32 / (256 / Q::kRows), kRowBlocks = TM * 32 / Q::kRows;
     static_assert(NI * Q::kQuadsPer == kQuads && NJ == kRowBlocks, "accumulators of another tile");
+    const float none = -__builtin_inff();
     const int columns = n_end - (n0 + col_at);             // of the tile, from this wave's first one on
 #pragma unroll
     for (int b = 0; b < kRowBlocks; ++b) {
         const int row = row_at + b * Q::kRows + Q::row_of(lane);
-        const float s_row = s_lds[BN + row], size = PLAIN ? s_row : fabsf(s_row), sign = s_row < 0.0f ? -1.0f : 1.0f;
+        const float s_row = s_lds[BN + row], size = PLAIN ? s_row : 1.0f;      // (z: without the row's scale, or with it)
         const int token = reinterpret_cast<const int*>(s_lds)[BN + BM + row] - (n0 + col_at);      // its column among the wave's
-        float z[kQuads][4], most = kLowest;
+        float z[kQuads][4], most = PLAIN ? kLowest : none;
 #pragma unroll
         for (int u = 0; u < kQuads; ++u) {
             const float4 s_quad = *reinterpret_cast<const float4*>(s_lds + col_at + Q::column_of(u, lane));
@@ -71,27 +74,38 @@ __device__ __forceinline__ void tile_stats(const QaMmTokenLogprobsParams& p, V (
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 z[u][t] = s_col[t] * Q::value(acc, u, b, t);
-                if constexpr (!PLAIN) z[u][t] = Q::column_of(u, lane) + t < columns ? sign * z[u][t] : -__builtin_inff();
+                if constexpr (!PLAIN) z[u][t] = Q::column_of(u, lane) + t < columns ? s_row * z[u][t] : none;
                 most = fmaxf(most, z[u][t]);
             }
         }
         most = most_over_columns<Q::kRows>(most);
-        if (!PLAIN && columns <= 0) most = 0.0f;
-        const float c = size * kLog2e, r = most * c, rest = __builtin_fmaf(most, c, -r);
-        float s = 0.0f, w = 0.0f;
+        float s = 0.0f, w = 0.0f, m;
+        if constexpr (PLAIN) {
+            const float c = size * kLog2e, r = most * c, rest = __builtin_fmaf(most, c, -r);
 #pragma unroll
-        for (int u = 0; u < kQuads; ++u)
+            for (int u = 0; u < kQuads; ++u)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                float d = __builtin_fmaf(z[u][t], c, -r);
-                if constexpr (!PLAIN) d = fmaxf(d, -200.0f);           // (its power is 0, and so is the product)
-                const float e = __builtin_amdgcn_exp2f(d);
-                s += e;
-                w = __builtin_fmaf(d, e, w);
-            }
-        s = sum_over_columns<Q::kRows>(s);
-        w = sum_over_columns<Q::kRows>(w);
-        const float f = __builtin_amdgcn_exp2f(-rest), m = PLAIN || columns > 0 ? fmaxf(size * most, kLowest) : kLowest;
+                for (int t = 0; t < 4; ++t) {
+                    const float d = __builtin_fmaf(z[u][t], c, -r), e = __builtin_amdgcn_exp2f(d);
+                    s += e;
+                    w = __builtin_fmaf(d, e, w);
+                }
+            s = sum_over_columns<Q::kRows>(s);
+            w = sum_over_columns<Q::kRows>(w);
+            const float f = __builtin_amdgcn_exp2f(-rest);
+            w = (w - rest * s) * f * kLn2;
+            s *= f;
+            m = fmaxf(size * most, kLowest);
+        } else {
+            m = fmaxf(most, kLowest);                      // (nothing but masked values, or NaNs: the differences are -inf, or NaN)
+            RowStats of_row = {m, 0.0f, 0.0f};
+#pragma unroll
+            for (int u = 0; u < kQuads; ++u)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) of_row.add(z[u][t]);
+            s = sum_over_columns<Q::kRows>(of_row.s);
+            w = sum_over_columns<Q::kRows>(of_row.t);
+        }
         uint32_t best = 0;
         if constexpr (TOP) {
             // (of the rounded logits, as they would be written)
@@ -102,9 +116,9 @@ __device__ __forceinline__ void tile_stats(const QaMmTokenLogprobsParams& p, V (
                 for (int t = 3; t >= 0; --t)
                     if (size * z[u][t] == m) best = Q::column_of(u, lane) + t;
             best = over_columns<Q::kRows>(best, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
-            if (best == 0xffffffffu) best = 0;             // (a row of NaNs)
+            if (best == 0xffffffffu) best = 0;             // (a row of NaNs, or of masked values)
         }
-        if (lane < Q::kRows) parts[row] = {m, s * f, (w - rest * s) * f * kLn2, n0 + col_at + static_cast<int>(best)};
+        if (lane < Q::kRows) parts[row] = {m, s, w, n0 + col_at + static_cast<int>(best)};
         if (__builtin_amdgcn_ballot_w64(token >= 0 && token < TN * 32)) {
             float v = 0.0f;
 #pragma unroll
@@ -115,6 +129,29 @@ __device__ __forceinline__ void tile_stats(const QaMmTokenLogprobsParams& p, V (
             if (token >= 0 && token < min(columns, TN * 32) && lane / Q::kRows == by && m0 + row < p.rows) given[m0 + row] = size * v;
         }
     }
+}
+
+// Whether of a wave's COLUMNS column scales and ROWS row scales the former are numbers, the latter not negative, and no logit of theirs passes
+// kFarthest.  (A row whose scale is NaN is that as a whole either way, and the rows beside it keep their bits.)
+template <int ROWS, int COLUMNS>
+__device__ __forceinline__ bool plain_scales(const float* s_row, const float* s_col, int k, int lane) {
+    bool fine = true;
+    float most_row = 0.0f, most_col = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ROWS; i += 64) {
+        const float v = s_row[ROWS % 64 == 0 ? i + lane : min(i + lane, ROWS - 1)];
+        fine &= !(v < 0.0f);
+        most_row = fmaxf(most_row, v);
+    }
+#pragma unroll
+    for (int i = 0; i < COLUMNS; i += 64) {
+        const float v = s_col[COLUMNS % 64 == 0 ? i + lane : min(i + lane, COLUMNS - 1)];
+        fine &= v == v;
+        most_col = fmaxf(most_col, fabsf(v));
+    }
+    // (the products of two codes are at most 2^14; an infinity times 0 is not below anything either)
+    fine &= wave_max(most_row) * (wave_max(most_col) * (16384.0f * k)) < kFarthest;
+    return !__builtin_amdgcn_ballot_w64(!fine);
 }
 
 // A tile takes `columns` of its BN columns.  TURN: workgroups do not all start at K's beginning (in step, all of them ask for the same 128 bytes of
@@ -165,9 +202,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mm_token_logprobs_kernel(QaMmT
         __syncthreads();
         const float* const s_lds = reinterpret_cast<const float*>(lds + C::kLdsBytes);
         float* const given = reinterpret_cast<float*>(out + static_cast<int64_t>(p.rows) * tiles_n);
-        bool negative = false;
-        for (int row = lane; row < TM * 32; row += 64) negative |= s_lds[BN + wm * TM * 32 + row] < 0.0f;
-        const bool plain = n_end - (n0 + wn * TN * 32) >= TN * 32 && !__builtin_amdgcn_ballot_w64(negative);
+        const bool plain = n_end - (n0 + wn * TN * 32) >= TN * 32 && plain_scales<TM * 32, TN * 32>(s_lds + BN + wm * TM * 32, s_lds + wn * TN * 32, p.k, lane);
         auto stats = [&](auto plain_c) __attribute__((always_inline)) {
             tile_stats<decltype(plain_c)::value, TOP, TM, TN, BM, BN>(p, acc, s_lds, wm * TM * 32, wn * TN * 32, m0, n0, n_end, lane, parts + wn * BM, given);
         };

@@ -92,7 +92,7 @@ int qa_token_logprobs(const QaTokenLogprobsParams* p, void* stream);
  * qa_gemm_w8a8, in fp32 and never written).  top is 0 or 1.
  */
 typedef struct QaMmTokenLogprobsParams {
-    int32_t rows, vocab, k;     /* rows up to 2^28, vocab up to 2^30, k a multiple of 16 */
+    int32_t rows, vocab, k;     /* rows up to 2^28, vocab up to 2^30, k a multiple of 16 up to 131056 (sums in 32 bits) */
     int32_t a_scale_numel, w_scale_numel;   /* 1 or rows, 1 or at least vocab */
     int32_t token_bytes;
     int32_t top, reserved0;

@@ -411,8 +411,11 @@ constexpr int64_t kWidestRow = 4 << 20;
 static_assert(320 * kWidestRow < 0x70000000LL, "the widest tile");
 constexpr int kMostColumns = 1 << 30, kMostRows = 1 << 28;     // (sums of them and a tile's stay in 32 bits, and so do the join's threads)
 
+constexpr int kDeepest = 131056;                               // (a sum of so many products of codes, up to 2^14 each, stays in 32 bits)
+static_assert((kDeepest + 16LL) << 14 == 1LL << 31, "the largest multiple of 16");
+
 int check(const QaMmTokenLogprobsParams& p) {
-    if (p.rows < 0 || p.rows > kMostRows || p.vocab < 1 || p.vocab > kMostColumns || p.k < 1) return QA_ERR_SHAPE;
+    if (p.rows < 0 || p.rows > kMostRows || p.vocab < 1 || p.vocab > kMostColumns || p.k < 1 || p.k > kDeepest) return QA_ERR_SHAPE;
     if (p.token_bytes != 4 && p.token_bytes != 8) return QA_ERR_UNSUPPORTED;
     if (p.top != 0 && p.top != 1) return QA_ERR_UNSUPPORTED;
     return QA_OK;

@@ -392,7 +392,7 @@ PyObject* scaled_mm_token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t 
         beside(b, "b", device);
         const int64_t M = a.size(0), K = a.size(1), N = b.size(1), vocab = args[6] == Py_None ? N : whole(args[6]);
         require(vocab >= 1 && vocab <= N, "vocab must be between 1 and the columns of b");
-        require(K >= 1 && K % 16 == 0, "K must be a multiple of 16");
+        require(K >= 1 && K % 16 == 0 && K <= 131056, "K must be a multiple of 16 up to 131056");
         require(a.stride(1) == 1 && b.stride(0) == 1, "a must be row-major and b column-major");
         const int64_t lda = M > 1 ? a.stride(0) : K, ldw = N > 1 ? b.stride(1) : K;
         require(lda % 16 == 0 && ldw % 16 == 0, "row strides of a and b must be multiples of 16");

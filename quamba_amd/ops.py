@@ -933,7 +933,7 @@ def token_logprobs(logits, tokens, top=0):
 
 def scaled_mm_token_logprobs(a, b, a_scales, b_scales, tokens, top=0, vocab=None):
     """token_logprobs(a_scales * (b_scales * (a @ b)), tokens, top) of int8 operands as scaled_mm_dq takes them, the logits in fp32
-    and never written (qa_mm_token_logprobs).  a int8 (M, K) row-major, b int8 (K, N) column-major, scales fp32 with 1 or M / 1 or N
+    and never written (qa_mm_token_logprobs).  a int8 (M, K) row-major, K up to 131056, b int8 (K, N) column-major, scales fp32 with 1 or M / 1 or N
     elements, tokens int32 or int64 (M,), top 0 or 1.  vocab: how many of b's columns are tokens (default all; the others are
     padding).  Returns TokenLogprobs."""
     return TokenLogprobs._make(_lm().scaled_mm_token_logprobs(a, b, a_scales, b_scales, tokens, top, vocab))

@@ -409,7 +409,7 @@ Plan plan_of(const QaMmTokenLogprobsParams& p) {
 // a tile's operands are addressed with 32-bit byte offsets
 constexpr int64_t kWidestRow = 4 << 20;
 static_assert(320 * kWidestRow < 0x70000000LL, "the widest tile");
-constexpr int kMostColumns = 1 << 30, kMostRows = 1 << 28;     // (sums of them and a tile's stay in 32 bits, and so do the join's threads)
+constexpr int kMostColumns = 1 << 30, kMostRows = 1 << 28;     // (sums of them and a tile's stay in 32 bits)
 
 constexpr int kDeepest = 131056;                               // (a sum of so many products of codes, up to 2^14 each, stays in 32 bits)
 static_assert((kDeepest + 16LL) << 14 == 1LL << 31, "the largest multiple of 16");
@@ -432,15 +432,15 @@ int launch(const QaMmTokenLogprobsParams& p, int columns, hipStream_t stream) {
     static_assert(C::kBM == kTiles[TILE].bm && C::kBN == kTiles[TILE].bn, "the tile of the table");
     const int tiles_n = (p.vocab + columns - 1) / columns;
     const int64_t tiles = static_cast<int64_t>((p.rows + C::kBM - 1) / C::kBM) * tiles_n;
-    if (!launchable(tiles, C::kThreads)) return QA_ERR_SHAPE;
+    const int at_once = p.rows >= 4096 ? 16 : p.rows >= 512 ? 4 : 1, joins = (p.rows + at_once - 1) / at_once;
+    if (!launchable(tiles, C::kThreads) || !launchable(joins, kJoinThreads)) return QA_ERR_SHAPE;
     auto kernel = p.top ? mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES, true, TURN> : mm_token_logprobs_kernel<TM, TN, WGM, WGN, STAGES, false, TURN>;
     constexpr int kLds = C::kLdsBytes + TileScales<C::kBM, C::kBN, C::kWaves>::kBytes + C::kBM * 4;
     static_assert(kLds <= 160 * 1024, "LDS of a CU");
     if (kLds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) return check_launch();
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles)), dim3(C::kThreads), kLds, stream, p, columns);
     if (const int status = check_launch()) return status;
-    const int at_once = p.rows >= 4096 ? 16 : p.rows >= 512 ? 4 : 1;
-    const dim3 grid(static_cast<unsigned>((p.rows + at_once - 1) / at_once));
+    const dim3 grid(static_cast<unsigned>(joins));
     auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kJoinThreads), 0, stream, p, tiles_n); };
     at_once == 16 ? join(mm_token_logprobs_join_kernel<16>) : at_once == 4 ? join(mm_token_logprobs_join_kernel<4>) : join(mm_token_logprobs_join_kernel<1>);
     return check_launch();

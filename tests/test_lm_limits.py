@@ -25,3 +25,12 @@ def test_sums_that_32_bits_do_not_hold(k, status):
     l, p = _lib.lib(), _head(4, 1000, k)
     assert (l.qa_mm_token_logprobs_workspace_bytes(C.byref(p)) > 0) == (status == -6)
     assert l.qa_mm_token_logprobs(C.byref(p), None) == status
+
+
+def test_rows_whose_join_a_launch_does_not_count():
+    """16 rows for each workgroup of 256: 2^32 threads for the last 16 of 2^28 rows, refused before the tiles are enqueued"""
+    l, p = _lib.lib(), _head(1 << 28, 16, 16)
+    p.workspace_bytes = (1 << 63) - 1
+    assert l.qa_mm_token_logprobs(C.byref(p), None) == -2
+    p.rows -= 15
+    assert l.qa_mm_token_logprobs(C.byref(p), None) == -2

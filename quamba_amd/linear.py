@@ -197,16 +197,18 @@ class W8A8B16O16Linear(_W8A8Base, _AlphaHooks):
         q.alpha = (w_s * input_scale).item()
         return q
 
+    def _logits(self, x2d):
+        """fp16, the columns of the padding among them"""
+        if x2d.shape[0] != 1:
+            return self._mm(x2d, torch.float16)
+        y = torch.empty((1, self.out_features + self.pad_out), dtype=torch.float16, device=x2d.device)
+        ops.scaled_mv_dq(y, self.weight.t(), x2d, self.alpha, 0.0)
+        return y
+
     @torch.no_grad()
     def forward(self, x):
         x_shape = x.shape
-        x2d = x.view(-1, x_shape[-1]).contiguous()
-        if x2d.shape[0] == 1:
-            y = torch.empty((1, self.out_features + self.pad_out), dtype=torch.float16, device=x.device)
-            ops.scaled_mv_dq(y, self.weight.t(), x2d, self.alpha, 0.0)
-        else:
-            y = self._mm(x2d, torch.float16)
-        return self._finish(y, x_shape)
+        return self._finish(self._logits(x.view(-1, x_shape[-1]).contiguous()), x_shape)
 
     @torch.no_grad()
     def token_logprobs(self, x, tokens, top=0, x_scale=None):
@@ -214,15 +216,19 @@ class W8A8B16O16Linear(_W8A8Base, _AlphaHooks):
         ``top`` best alternatives, an ops.TokenLogprobs.  ``x_scale`` fp32 (...,): one scale per token, as QRMSNorm gives them, in
         place of the layer's input scale.
 
-        With ``top`` up to 1 the logits stay in fp32 and are never written (ops.scaled_mm_token_logprobs); with more they are
-        those of ``forward``, rounded to fp16."""
+        With ``top`` up to 1 the logits stay in fp32 and are never written (ops.scaled_mm_token_logprobs).  With more they are those of
+        ``forward`` (with ``x_scale``, of ops.scaled_mm_dq), rounded to fp16: a log probability is then off by up to 2^-10 of the largest of
+        them, and differs by that from what ``top`` up to 1 gives."""
         x2d, shape = x.reshape(-1, x.shape[-1]).contiguous(), x.shape[:-1]
         a, flat = _token_scales(x_scale, shape, self.a), _tokens_like(tokens, shape)
         if top <= 1:
             r = ops.scaled_mm_token_logprobs(x2d, self.weight, a, self.b, flat, top, self.out_features)
         else:
-            y = torch.empty((x2d.shape[0], self.out_features + self.pad_out), dtype=torch.float16, device=x.device)
-            ops.scaled_mm_dq(y, x2d, self.weight, a, self.b)
+            if x_scale is None:
+                y = self._logits(x2d)
+            else:
+                y = torch.empty((x2d.shape[0], self.out_features + self.pad_out), dtype=torch.float16, device=x.device)
+                ops.scaled_mm_dq(y, x2d, self.weight, a, self.b)
             r = ops.token_logprobs(y[:, :self.out_features], flat, top)
         return _shaped_logprobs(r, shape)
 

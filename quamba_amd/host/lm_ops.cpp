@@ -299,6 +299,8 @@ PyObject* add_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+constexpr int64_t kTogether = 1024;        // fp32 answers of one allocation, at most
+
 // Tokens, answers and workspace of both operators, the call, and the answers as a tuple.
 template <class Params>
 PyObject* answer(Params& p, const at::Tensor& tokens_as_given, at::IntArrayRef shape, int64_t top, at::Device device, int64_t (*bytes)(const Params*),
@@ -312,14 +314,18 @@ PyObject* answer(Params& p, const at::Tensor& tokens_as_given, at::IntArrayRef s
     at::DimVector best(shape.begin(), shape.end());
     best.push_back(top);
     const at::Tensor top_tokens = at::empty(best, opts.dtype(at::kLong));
-    // (the three fp32 answers in one allocation, and without torch's dispatch: a call on one row takes the GPU 8 us and the host as long)
-    const at::Tensor memory = at::empty({c10::multiply_integers(shape) * (2 + top)}, opts.dtype(at::kFloat));
+    // (A call on few rows takes the GPU 8 us and the host as long: there the three fp32 answers are one allocation, each on 16 bytes, and made without
+    // torch's dispatch.  Above kTogether values who keeps one of them would keep the others' memory, and the time does not show.)
+    const int64_t count = c10::multiply_integers(shape), places = (count + 3) / 4 * 4;
+    const bool together = 2 * places + count * top <= kTogether;
+    const at::Tensor memory = together ? at::empty({2 * places + count * top}, opts.dtype(at::kFloat)) : at::Tensor();
     int64_t used = 0;
     auto part = [&](at::IntArrayRef sizes) {
+        if (!together) return at::empty(sizes, opts.dtype(at::kFloat));
         at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(memory.storage()), memory.key_set(), memory.dtype());
         t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
         t.unsafeGetTensorImpl()->set_storage_offset(used);
-        used += t.numel();
+        used += places;
         return t;
     };
     const at::Tensor logprobs = part(shape), entropy = part(shape), top_logprobs = part(best);

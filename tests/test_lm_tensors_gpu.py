@@ -1,0 +1,29 @@
+"""The tensors that the operators around the mixers return and write: their memory, their versions, how they may lie."""
+import pytest
+import torch
+
+from quamba_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows", [500, 5000])
+def test_large_answers_do_not_keep_each_other(dev, rows):
+    """What is kept, or saved, of many rows is what it shows"""
+    logits, tokens = torch.randn(rows, 100, device=dev), torch.zeros(rows, dtype=torch.int64, device=dev)
+    a, b = torch.zeros(rows, 64, dtype=torch.int8, device=dev), torch.zeros(96, 64, dtype=torch.int8, device=dev).t()
+    one = torch.ones(1, device=dev)
+    for got in (ops.token_logprobs(logits, tokens, top=20), ops.scaled_mm_token_logprobs(a, b, one, one, tokens, top=1)):
+        for t in got:
+            assert t.untyped_storage().nbytes() == t.numel() * t.element_size() and t.storage_offset() == 0
+        assert len({t.untyped_storage().data_ptr() for t in got}) == 4
+
+
+@pytest.mark.parametrize("lead,top", [((1,), 5), ((3,), 1), ((), 3), ((2, 3), 20), ((0,), 4), ((7,), 0)])
+def test_small_answers_lie_on_whole_words(dev, lead, top):
+    logits, tokens = torch.randn(*lead, 100, device=dev), torch.zeros(lead, dtype=torch.int64, device=dev)
+    got = ops.token_logprobs(logits, tokens, top=top)
+    assert [t.shape for t in got] == [lead, lead, (*lead, top), (*lead, top)]
+    assert all(t.data_ptr() % 16 == 0 and t.is_contiguous() for t in got)
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in got if t.numel())
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))

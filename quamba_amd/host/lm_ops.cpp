@@ -295,6 +295,7 @@ PyObject* add_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         p.out = y.data_ptr();
         p.scales = dynamic ? scales.data_ptr<float>() : nullptr;
         enqueue(g.add_rmsnorm, p, device, "add_rmsnorm");
+        if (given && !given->is_inference()) given->unsafeGetTensorImpl()->bump_version();      // (as torch's own writes in place do)
         return Py_BuildValue("(NNN)", wrapped(y), given ? Py_NewRef(a[10]) : wrapped_or_none(v), wrapped_or_none(scales));
     });
 }

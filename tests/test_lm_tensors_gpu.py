@@ -27,3 +27,31 @@ def test_small_answers_lie_on_whole_words(dev, lead, top):
     assert all(t.data_ptr() % 16 == 0 and t.is_contiguous() for t in got)
     spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in got if t.numel())
     assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+
+
+def test_a_stream_that_is_written_has_another_version(dev):
+    """so that autograd notices where it saved what was there before"""
+    x, w = torch.randn(4, 64, device=dev), torch.ones(64, device=dev)
+    stream = torch.randn(4, 64, device=dev)
+    before = stream._version
+    ops.add_rmsnorm(x, w, 1e-5, residual=stream)
+    assert stream._version == before
+    ops.add_rmsnorm(x, w, 1e-5, residual=stream, residual_out=stream)
+    assert stream._version > before
+    leaf = torch.ones(4, 64, device=dev, requires_grad=True)
+    kept = torch.randn(4, 64, device=dev)
+    product = leaf * kept
+    ops.add_rmsnorm(x, w, 1e-5, residual=kept, residual_out=kept)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    # a view has its base's version; a stream of inference mode has none, there and outside
+    base = torch.zeros(4, 96, device=dev)
+    before = base._version
+    ops.add_rmsnorm(x, w, 1e-5, residual_out=base[:, 16:80])
+    assert base._version > before
+    with torch.inference_mode():
+        held = torch.zeros(4, 64, device=dev)
+        ops.add_rmsnorm(x, w, 1e-5, residual=held, residual_out=held)
+    want = held.clone()
+    ops.add_rmsnorm(x, w, 1e-5, residual=held, residual_out=held)
+    assert torch.equal(held, want + x)

@@ -260,7 +260,15 @@ PyObject* add_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 if (t == residual && t->const_data_ptr() == given->const_data_ptr() && (rows == 1 || t->stride(0) == given->stride(0))) return;
                 const auto [f, l] = span(*t);
                 const auto [of, ol] = span(*given);
-                require(l <= of || ol <= f, std::string("residual_out overlaps ") + name);
+                if (l <= of || ol <= f) return;
+                // rows (or one) between the rows of `given`: in its pitch, behind the columns of one and in front of the next one's
+                const bool one = t->dim() == 1 || t->size(0) == 1 || t->stride(0) == 0;
+                bool between = rows > 1 && (one || t->stride(0) * t->element_size() == given->stride(0) * given->element_size());
+                if (between) {
+                    const int64_t pitch = given->stride(0) * given->element_size(), behind = ((f - of) % pitch + pitch) % pitch;
+                    between = behind >= dim * given->element_size() && behind + dim * t->element_size() <= pitch;
+                }
+                require(between, std::string("residual_out overlaps ") + name);
             };
             apart(&x, "x"); apart(&weight, "weight"); apart(residual, "residual"); apart(post, "post_weight"); apart(gate, "gate"); apart(vector, "residual_scale");
         }

@@ -55,3 +55,30 @@ def test_a_stream_that_is_written_has_another_version(dev):
     want = held.clone()
     ops.add_rmsnorm(x, w, 1e-5, residual=held, residual_out=held)
     assert torch.equal(held, want + x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_rows_that_lie_between_rows(dev, dtype):
+    """x, stream and what is written side by side in one piece of memory"""
+    g = torch.Generator().manual_seed(1)
+    memory = torch.randn(9, 3 * 72, generator=g).to(dtype).to(dev)
+    x, r, out = memory[:, :64], memory[:, 72:136], memory[:, 152:216]
+    w = torch.ones(64, dtype=dtype, device=dev)
+    want = ops.add_rmsnorm(x.contiguous(), w, 1e-5, residual=r.contiguous())
+    rest = memory[:, 64:72].clone(), memory[:, 136:152].clone()
+    got = ops.add_rmsnorm(x, w, 1e-5, residual=r, residual_out=out)
+    assert torch.equal(got[0], want[0]) and torch.equal(out, want[1])
+    got = ops.add_rmsnorm(x, w, 1e-5, residual=r, residual_out=r)
+    assert torch.equal(got[0], want[0]) and torch.equal(r, want[1])
+    # every other row of one piece, and the rows between them
+    pairs = memory[:8].clone()
+    want = ops.add_rmsnorm(pairs[::2, :64].contiguous(), w, 1e-5)
+    got = ops.add_rmsnorm(pairs[::2, :64], w, 1e-5, residual_out=pairs[1::2, :64])
+    assert torch.equal(got[0], want[0]) and torch.equal(pairs[1::2, :64], want[1])
+    assert torch.equal(memory[:, 64:72], rest[0]) and torch.equal(memory[:, 136:152], rest[1])
+    # columns that are shared, a gate of one row among them, rows of another pitch: refused
+    for bad in (dict(residual_out=memory[:, 60:124]), dict(residual_out=memory[:, 10:74]), dict(residual=r, residual_out=memory[:, 100:164]),
+                dict(gate=memory[2, 152:216], residual_out=out),
+                dict(residual_out=memory.view(-1)[64:64 + 9 * 70].view(9, 70)[:, :64])):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ops.add_rmsnorm(x, w, 1e-5, **bad)

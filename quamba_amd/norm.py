@@ -140,10 +140,11 @@ class QRMSNorm(torch.nn.Module):
         self.output_scale = state_dict.pop(prefix + "output_scale")
 
     @torch.no_grad()
-    def forward(self, x, residual=None, prenorm=False, residual_in_fp32=False, gate=None, gate_act="none", residual_scale=1.0):
+    def forward(self, x, residual=None, prenorm=False, residual_in_fp32=False, gate=None, gate_act="none", residual_scale=1.0, residual_out=None):
         """``x`` (..., dim), what the block before gives; ``residual`` (..., dim) or None, the stream in front of that block.  Returns the
         normed stream - a tensor, or the pair (codes, scales (...,)) with a scale per token - and with ``prenorm`` the
-        stream behind it: (normed, stream) or (codes, scales, stream).  ``gate`` is (..., dim) or (dim,)."""
+        stream behind it: (normed, stream) or (codes, scales, stream).  ``gate`` is (..., dim) or (dim,).  The stream is written to
+        ``residual_out`` (..., dim) where that is given; it may be ``residual`` itself."""
         shape, dim = x.shape, x.shape[-1]
 
         def rows(t):
@@ -152,17 +153,20 @@ class QRMSNorm(torch.nn.Module):
             raise RuntimeError(f"residual must have shape {tuple(shape)}, not {tuple(residual.shape)}")
         if gate is not None and gate.dim() > 1 and gate.shape != shape:
             raise RuntimeError(f"gate must have shape {tuple(shape)} or ({dim},), not {tuple(gate.shape)}")
+        if residual_out is not None and residual_out.shape != shape:
+            raise RuntimeError(f"residual_out must have shape {tuple(shape)}, not {tuple(residual_out.shape)}")
         quantized = not self.use_float_output
         y, stream, scales = ops.add_rmsnorm(
             rows(x), self.weight, self.eps, rows(residual), post_weight=self.post_weight, gate=gate if gate is None or gate.dim() == 1 else rows(gate),
             gate_act=gate_act, residual_scale=residual_scale, prenorm=prenorm,
             residual_dtype=torch.float32 if residual is None and residual_in_fp32 else None,
+            residual_out=None if residual_out is None else residual_out.view(-1, dim),
             out_dtype=torch.int8 if quantized else None, out_scale=self.output_scale if quantized else None)
         out = [y.reshape(shape)]
         if scales is not None:
             out.append(scales.reshape(shape[:-1]))
         if prenorm:
-            out.append(stream.reshape(shape))
+            out.append(stream.reshape(shape) if residual_out is None else residual_out)
         return out[0] if len(out) == 1 else tuple(out)
 
     def __repr__(self):

@@ -120,15 +120,15 @@ class QRMSNorm(torch.nn.Module):
         self._register_load_state_dict_pre_hook(self._load_scale)
 
     @classmethod
-    def from_fp16(cls, originalLayer, output_scale=None, use_float_output=False, post_layer=None):
+    def from_fp16(cls, originalLayer, output_scale=None, use_float_output=False, post_layer=None, dtype=torch.float16):
         """``originalLayer``, and ``post_layer`` for the norm behind the block before: anything with weight and eps.  Without an
-        ``output_scale`` each token gets its own."""
+        ``output_scale`` each token gets its own.  ``dtype`` of the weights: that of the rows, or fp32."""
         assert output_scale is None or type(output_scale) is float, "Only support per-tensor static quant for output"
         assert post_layer is None or post_layer.eps == originalLayer.eps, "Only support one eps"
-        q = cls(originalLayer.weight.shape[0], originalLayer.eps, use_float_output, post_layer is not None, originalLayer.weight.device)
-        q.weight = originalLayer.weight.detach().clone().to(torch.float16)
+        q = cls(originalLayer.weight.shape[0], originalLayer.eps, use_float_output, post_layer is not None, originalLayer.weight.device, dtype)
+        q.weight = originalLayer.weight.detach().clone().to(dtype)
         if post_layer is not None:
-            q.post_weight = post_layer.weight.detach().clone().to(torch.float16)
+            q.post_weight = post_layer.weight.detach().clone().to(dtype)
         q.output_scale = output_scale
         return q
 

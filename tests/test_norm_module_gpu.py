@@ -57,3 +57,17 @@ def test_captured_with_the_stream_in_place(dev):
         now, _ = norm(x, eager, prenorm=True, residual_out=eager)
         torch.cuda.synchronize()
         assert torch.equal(codes, now) and torch.equal(stream, eager), i
+
+
+@pytest.mark.parametrize("rows,weights", [(torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                          (torch.float16, torch.float32), (torch.float32, torch.float32)])
+def test_weights_of_each_type(dev, rows, weights):
+    layer, post = Float(dev), Float(dev)
+    norm = QRMSNorm.from_fp16(layer, 0.04, post_layer=post, dtype=weights)
+    x = torch.randn(4, DIM, device=dev).to(rows)
+    by_hand = QRMSNorm(DIM, layer.eps, post_norm=True, device=dev, dtype=weights)
+    by_hand.load_state_dict(norm.state_dict())
+    assert norm.weight.dtype == weights and torch.equal(norm.weight, layer.weight.detach().to(weights))
+    assert norm.post_weight.dtype == weights and torch.equal(norm.post_weight, post.weight.detach().to(weights))
+    assert torch.equal(norm(x), by_hand(x)) and norm(x).dtype == torch.int8
+    assert QRMSNorm.from_fp16(layer).weight.dtype == torch.float16

@@ -21,8 +21,9 @@ namespace lm {
 constexpr int kAddNormWaves = 16;                        // of a workgroup, at most
 constexpr int kAddNormDim = kAddNormWaves * 4 * 512;     // widest row
 
-// within 4 + |z| units of 2^-24 (an exponential and a reciprocal of two each, and the rounding of the exponent); exact divisions and
-// expf made the gate the larger part of the kernel's time
+// For z above -87 within 5 + 1.25 |z| units of 2^-24 (an exponential and a reciprocal of two each, their sum's rounding, and the exponent's); below, where 1 + e^-z has
+// no normal reciprocal, 0 or within 2^-126.  16-bit rows do not see that; for fp32 ones it is the choice made, as exact divisions and expf made the
+// gate the larger part of the kernel's time.
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f)); }
 
 // Pieces of a lane, waves that share a row, rows of a workgroup.  A run is what a wave loads at once, 512 columns.

@@ -900,7 +900,7 @@ def add_rmsnorm(x, weight, eps, residual=None, post_weight=None, gate=None, gate
     fp32; gate (rows, dim) or (dim,) of x's type; weight, post_weight and a residual_scale that is a tensor (dim,) all of x's type
     or all fp32.  Rows may lie apart.
 
-    y is of x's type, or with out_dtype=torch.int8 the codes rint(y / s), saturated: s = out_scale, or without one
+    y is of x's type, or with out_dtype=torch.int8 the codes rint(y * (1 / s)), saturated, the reciprocal in fp32: s = out_scale, or without one
     max(max|y|, 1e-5) / 127 of each row, which scaled_mm_dq takes as its a_scales.
 
     Returns (y, v, scales): v None with prenorm=False, else in the type of residual or residual_dtype, written to residual_out

@@ -30,8 +30,9 @@ typedef enum QaGateAct { QA_GATE_PLAIN = 0, QA_GATE_SIGMOID = 1, QA_GATE_SILU = 
  *   v = residual + scale * u                                                       (residual null: scale * u)
  *   y = v / sqrt(mean(v^2) + eps) * weight
  * all in fp32; v is not rounded on its way into y.  residual_out (null: not wanted) gets v; it may be `residual` itself and
- * must not overlap an input otherwise.  out gets y, or with QA_LM_I8 the saturated rint(y * (1 / s)), the reciprocal rounded to fp32: s is out_scale (a normal number above 0), or with
- * dynamic_scale max(max|y|, 1e-5) / 127 of the row, written to scales.  A row with a NaN or an infinity, or whose
+ * must not overlap an input otherwise.  out gets y, or with QA_LM_I8 the saturated rint(y * (1 / s)), the reciprocal rounded to
+ * fp32: s is out_scale (a normal number above 0), or with dynamic_scale max(max|y|, 1e-5) / 127 of the row, written to scales.
+ * A row with a NaN or an infinity, or whose
  * squares pass fp32 (values from some 1e18 on), is NaN as a whole: its y, or its scale (codes by out_scale mean nothing then).
  */
 typedef struct QaAddNormParams {

@@ -12,6 +12,8 @@ LIB_PATH = os.path.join(_HERE, "libquamba_amd.so")
 QA_OK = 0
 ABI_VERSION = 3          # what qa_abi_version() of a matching library returns
 LM_ABI_VERSION = 1       # and qa_lm_abi_version()
+MX_ABI_VERSION = 1       # and qa_mx_abi_version()
+BEAM_ABI_VERSION = 1     # and qa_beam_abi_version()
 QA_OUT_I8, QA_OUT_F16, QA_OUT_BF16 = 0, 1, 2
 QA_ROUND_RNE, QA_ROUND_HALF_AWAY = 0, 1
 QA_IN_F16, QA_IN_F32 = 0, 1
@@ -238,7 +240,66 @@ class QaMmTokenLogprobsParams(C.Structure):
     ]
 
 
-# name -> (restype, argtypes); every symbol declared in include/quamba_amd_lm.h
+class QaMxQuantParams(C.Structure):
+    _fields_ = [
+        ("rows", i32), ("k", i32), ("x_type", i32), ("reserved0", i32),
+        ("x_row_stride", i64), ("code_row_stride", i64), ("scale_group_stride", i64),
+        ("x", vp), ("codes", vp), ("scales", vp),
+    ]
+
+
+class QaMxDequantParams(C.Structure):
+    _fields_ = [
+        ("rows", i32), ("k", i32), ("out_type", i32), ("reserved0", i32),
+        ("out_row_stride", i64), ("code_row_stride", i64), ("scale_group_stride", i64),
+        ("codes", vp), ("scales", vp), ("out", vp),
+    ]
+
+
+class QaMxGemmParams(C.Structure):
+    _fields_ = [
+        ("m", i32), ("n", i32), ("k", i32), ("a_type", i32), ("out_type", i32), ("reserved0", i32),
+        ("lda", i64), ("ldw", i64), ("ldd", i64), ("a_scale_group_stride", i64), ("w_scale_group_stride", i64),
+        ("a", vp), ("a_scales", vp), ("w", vp), ("w_scales", vp), ("d", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class QaBeamSearchParams(C.Structure):
+    _fields_ = [
+        ("batch", i32), ("beams", i32), ("vocab", i32), ("logits_type", i32), ("count", i32), ("reserved0", i32),
+        ("logits_batch_stride", i64), ("logits_beam_stride", i64), ("logits", vp), ("scores", vp), ("done", vp),
+        ("out_scores", vp), ("tokens", vp), ("parents", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class QaStateRows(C.Structure):
+    _fields_ = [("data", vp), ("row_bytes", i64), ("row_stride", i64)]
+
+
+class QaReorderParams(C.Structure):
+    _fields_ = [
+        ("batch", i32), ("beams", i32), ("tensors", i32), ("index_bytes", i32), ("states", C.POINTER(QaStateRows)), ("parents", vp),
+    ]
+
+
+# name -> (restype, argtypes); every symbol declared in include/quamba_amd_mx.h
+MX_SYMBOLS = {
+    "qa_mx_abi_version": (C.c_int, []),
+    "qa_mxfp4_quant": (C.c_int, [C.POINTER(QaMxQuantParams), vp]),
+    "qa_mxfp4_dequant": (C.c_int, [C.POINTER(QaMxDequantParams), vp]),
+    "qa_mxfp4_mm_workspace_bytes": (C.c_int64, [C.POINTER(QaMxGemmParams)]),
+    "qa_mxfp4_mm": (C.c_int, [C.POINTER(QaMxGemmParams), vp]),
+}
+
+# and in include/quamba_amd_beam.h
+BEAM_SYMBOLS = {
+    "qa_beam_abi_version": (C.c_int, []),
+    "qa_beam_search_workspace_bytes": (C.c_int64, [C.POINTER(QaBeamSearchParams)]),
+    "qa_beam_search_step": (C.c_int, [C.POINTER(QaBeamSearchParams), vp]),
+    "qa_reorder_states": (C.c_int, [C.POINTER(QaReorderParams), vp]),
+}
+
+# and in include/quamba_amd_lm.h
 LM_SYMBOLS = {
     "qa_lm_abi_version": (C.c_int, []),
     "qa_add_rmsnorm": (C.c_int, [C.POINTER(QaAddNormParams), vp]),
@@ -289,13 +350,14 @@ def lib():
                 f"{LIB_PATH} is missing: build it with `python -m quamba_amd.build` "
                 "(quamba_amd has no CPU or PyTorch fallback)")
         handle = C.CDLL(LIB_PATH)
-        for name, (res, args) in (*SYMBOLS.items(), *LM_SYMBOLS.items()):
+        for name, (res, args) in (*SYMBOLS.items(), *LM_SYMBOLS.items(), *MX_SYMBOLS.items(), *BEAM_SYMBOLS.items()):
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
-        found = handle.qa_abi_version(), handle.qa_lm_abi_version()
-        if found != (ABI_VERSION, LM_ABI_VERSION):
-            raise RuntimeError(f"{LIB_PATH} has ABI versions {found}, this binding expects {(ABI_VERSION, LM_ABI_VERSION)}: "
+        found = handle.qa_abi_version(), handle.qa_lm_abi_version(), handle.qa_mx_abi_version(), handle.qa_beam_abi_version()
+        expected = ABI_VERSION, LM_ABI_VERSION, MX_ABI_VERSION, BEAM_ABI_VERSION
+        if found != expected:
+            raise RuntimeError(f"{LIB_PATH} has ABI versions {found}, this binding expects {expected}: "
                                "rebuild it with `python -m quamba_amd.build --force`")
         _lib = handle
     return _lib

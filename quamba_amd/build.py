@@ -2,8 +2,9 @@
 
 Usage: python -m quamba_amd.build [--force]
 The library is cross-compiled without a GPU; the built file sits beside this module so that it
-travels with the source tree.  Beside it go _host.so, the host side of the mixers' calls, and _lm_host.so, that of the
-operators around them (C++ against torch's headers, no device code).
+travels with the source tree.  Beside it go _host.so, the host side of the mixers' calls, _lm_host.so, that of the
+operators around them, and _mx_beam_host.so, that of the microscaled 4-bit operators and of beam search (C++ against torch's
+headers, no device code).
 """
 import os
 import subprocess
@@ -15,8 +16,8 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "csrc", "build")
 LIB = os.path.join(HERE, "libquamba_amd.so")
 # extension -> its source
-HOSTS = {os.path.join(HERE, name): os.path.join(HERE, "host", src) for name, src in (("_host.so", "layer_call.cpp"), ("_lm_host.so", "lm_ops.cpp"))}
-HEADERS = [os.path.join(HERE, "..", "include", h) for h in ("quamba_amd.h", "quamba_amd_lm.h")]
+HOSTS = {os.path.join(HERE, name): os.path.join(HERE, "host", src) for name, src in (("_host.so", "layer_call.cpp"), ("_lm_host.so", "lm_ops.cpp"), ("_mx_beam_host.so", "mx_beam_ops.cpp"))}
+HEADERS = [os.path.join(HERE, "..", "include", h) for h in ("quamba_amd.h", "quamba_amd_lm.h", "quamba_amd_mx.h", "quamba_amd_beam.h")]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
@@ -56,7 +57,7 @@ def _compile(src, force):
 
 def build_host(host, force=False):
     src = HOSTS[host]
-    if not force and not any(_newer(d, host) for d in (src, *HEADERS)):
+    if not force and not any(_newer(d, host) for d in (src, os.path.join(HERE, "host", "host_common.hpp"), *HEADERS)):
         return
     import sysconfig
 

@@ -1,0 +1,138 @@
+// Products of few rows: operands straight from memory into the matrix instruction's registers.
+//
+// What is wanted is the weights, read once: a wave takes RN x 16 columns by RM x 16 rows and a part of K, whole groups of 512 values, so that it asks for
+// all of its rows' lines (256 bytes of codes and a word of scales for each) before it multiplies.  The waves of a workgroup share the columns and split K; their
+// sums meet in LDS, in the order of the waves.
+#include "mx_gemm.hpp"
+
+#include <algorithm>
+
+namespace qa {
+namespace mx {
+namespace {
+
+constexpr int kMaxWaves = 8;
+
+// ROWS_T: type of the rows (int8_t: codes)
+template <int RM, int RN, class ROWS_T>
+__global__ __launch_bounds__(64 * kMaxWaves) void mxfp4_direct_kernel(QaMxGemmParams p, int tiles_m, bool words) {
+    constexpr bool kCodes = std::is_same_v<ROWS_T, int8_t>;
+    extern __shared__ __attribute__((aligned(16))) v4f sums[];             // [wave][RN * RM][64]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int row = lane & 15, q = lane >> 4;
+    const int m0 = static_cast<int>(blockIdx.x % tiles_m) * (RM * 16), n0 = static_cast<int>(blockIdx.x / tiles_m) * (RN * 16);
+    const int blocks = p.k / kBlock, groups = (blocks + 15) / 16;
+    // (rows behind the last one: that one again, and what comes of it is not written)
+    const uint8_t *w[RN], *w_scales[RN], *a_scales[RM];
+    const ROWS_T* a[RM];
+#pragma unroll
+    for (int i = 0; i < RN; ++i) {
+        const int64_t n = min(n0 + i * 16 + row, p.n - 1);
+        w[i] = p.w + n * p.ldw;
+        w_scales[i] = p.w_scales + n * 16 + 4 * q;
+    }
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+        const int64_t m = min(m0 + i * 16 + row, p.m - 1);
+        a[i] = static_cast<const ROWS_T*>(p.a) + m * p.lda;
+        a_scales[i] = kCodes ? p.a_scales + m * 16 + 4 * q : nullptr;
+    }
+    v4f acc[RN][RM];
+#pragma unroll
+    for (int i = 0; i < RN; ++i)
+#pragma unroll
+        for (int j = 0; j < RM; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+    for (int g = wave; g < groups; g += waves) {
+        v4i wv[RN][4], av[RM][4];
+        int ws[RN], as[RM];
+        // (blocks behind K: the last one again, by scales of 2^-127 on both sides, and nothing is left of their products in fp32)
+        const int mine = (blocks - g * 16 - q + 3) >> 2;
+        const uint32_t mask = mine >= 4 ? 0xffffffffu : mine <= 0 ? 0u : (1u << (8 * mine)) - 1;
+        int at[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) at[j] = min(g * 16 + 4 * j + q, blocks - 1);
+#pragma unroll
+        for (int i = 0; i < RN; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wv[i][j] = *reinterpret_cast<const v4i*>(w[i] + at[j] * 16);
+            ws[i] = *reinterpret_cast<const int*>(w_scales[i] + g * p.w_scale_group_stride) & mask;
+        }
+        if constexpr (kCodes) {
+#pragma unroll
+            for (int i = 0; i < RM; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) av[i][j] = *reinterpret_cast<const v4i*>(a[i] + at[j] * 16);
+                as[i] = *reinterpret_cast<const int*>(a_scales[i] + g * p.a_scale_group_stride) & mask;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < RM; ++i) {
+                uint32_t scales = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    Raw<ROWS_T, 32> raw;
+                    raw.template load<false>(a[i] + at[j] * kBlock);
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) most = max(most, __float_as_uint(raw.get(e)) & 0x7fffffffu);
+                    const uint32_t scale = scale_of(most);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) av[i][j][e] = codes_of(scale, [&](int x) { return raw.get(e * 8 + x); });
+                    scales |= scale << (8 * j);
+                }
+                as[i] = scales & mask;
+            }
+        }
+        static_for<0, 4>([&](auto j_c) {
+            constexpr int j = decltype(j_c)::value;
+#pragma unroll
+            for (int x = 0; x < RN; ++x)
+#pragma unroll
+                for (int y = 0; y < RM; ++y) acc[x][y] = multiply<j>(wv[x][j], ws[x], av[y][j], as[y], acc[x][y]);
+        });
+    }
+    if (waves > 1) {
+#pragma unroll
+        for (int i = 0; i < RN; ++i)
+#pragma unroll
+            for (int j = 0; j < RM; ++j) sums[(wave * RN * RM + i * RM + j) * 64 + lane] = acc[i][j];
+        __syncthreads();
+    }
+    // a wave finishes every `waves`-th of the blocks of 16 x 16
+#pragma unroll
+    for (int i = 0; i < RN; ++i)
+#pragma unroll
+        for (int j = 0; j < RM; ++j) {
+            const int f = i * RM + j;
+            if (f % waves != wave) continue;
+            v4f v = acc[i][j];
+            if (waves > 1) {
+                v = sums[f * 64 + lane];
+                for (int o = 1; o < waves; ++o) v += sums[(o * RN * RM + f) * 64 + lane];
+            }
+            store_columns(p, m0 + j * 16 + row, n0 + i * 16 + 4 * q, v, words);
+        }
+}
+
+template <int RM, int RN, class ROWS_T>
+int launch(const QaMxGemmParams& p, hipStream_t stream) {
+    const int64_t tiles_m = (p.m + RM * 16 - 1) / (RM * 16), tiles_n = (p.n + RN * 16 - 1) / (RN * 16);
+    const int waves = static_cast<int>(std::min<int64_t>(kMaxWaves, std::max<int64_t>(1, groups_of(p.k))));
+    if (!launchable(tiles_m * tiles_n, 64 * waves)) return QA_ERR_SHAPE;
+    hipLaunchKernelGGL((mxfp4_direct_kernel<RM, RN, ROWS_T>), dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(64 * waves),
+                       waves > 1 ? waves * RM * RN * 64 * sizeof(v4f) : 0, stream, p, static_cast<int>(tiles_m), whole_words(p));
+    return check_launch();
+}
+
+}  // namespace
+
+int direct_launch(const QaMxGemmParams& p, hipStream_t stream) {
+    if (p.a_type == QA_LM_F32) return launch<1, 1, float>(p, stream);
+    if (p.a_type == QA_LM_BF16) return launch<1, 1, __bf16>(p, stream);
+    if (p.a_type == QA_LM_F16) return launch<1, 1, _Float16>(p, stream);
+    if (p.m <= 16) return launch<1, 1, int8_t>(p, stream);
+    return launch<4, 2, int8_t>(p, stream);
+}
+
+}  // namespace mx
+}  // namespace qa

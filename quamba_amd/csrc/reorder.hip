@@ -1,0 +1,129 @@
+// Rows of states in another order, in place (qa_reorder_states).
+//
+// A thread has one unit of 16 bytes (4 or 1 where a state does not lie on that) of all the rows of an entry: it reads what its rows are to become and then writes them, so
+// that no row is read after it was written and no copy is needed.  Rows that stay are neither read nor written, and a parent of several
+// rows comes from memory once and from the caches again.  Bound by memory.  One launch has up to kTensors tensors, with their addresses in its arguments.
+#include "../../include/quamba_amd_beam.h"
+#include "lm_common.hpp"
+
+#include <algorithm>
+
+namespace qa {
+namespace lm {
+namespace {
+
+constexpr int kTensors = 96, kThreads = 256, kMaxBeams = 64;
+
+struct Tensors {
+    uint8_t* data[kTensors];
+    int64_t row_stride[kTensors];
+    int32_t units[kTensors];           // of a row
+    int32_t first[kTensors + 1];       // workgroup of the first unit; behind the last one, all of them
+    int32_t count;
+};
+static_assert(sizeof(Tensors) < 3072, "arguments of a launch");
+
+template <int BEAMS, class U>
+__device__ __forceinline__ void move_unit(uint8_t* base, int64_t row_stride, const int (&from)[BEAMS], int beams) {
+    U v[BEAMS];
+#pragma unroll
+    for (int i = 0; i < BEAMS; ++i)
+        if (i < beams && from[i] != i) v[i] = *reinterpret_cast<const U*>(base + from[i] * row_stride);
+#pragma unroll
+    for (int i = 0; i < BEAMS; ++i)
+        if (i < beams && from[i] != i) *reinterpret_cast<U*>(base + i * row_stride) = v[i];
+}
+
+// UNIT: bytes; BEAMS: at least as many as there are
+template <int BEAMS, int UNIT>
+__global__ __launch_bounds__(kThreads) void reorder_kernel(Tensors t, const void* parents, int index_bytes, int beams) {
+    const int64_t entry = blockIdx.y;
+    int from[BEAMS], moved = 0;
+#pragma unroll
+    for (int i = 0; i < BEAMS; ++i) {
+        from[i] = i;
+        if (i >= beams) continue;
+        const int64_t parent = token_of(parents, index_bytes, entry * beams + i);
+        if (parent >= 0 && parent < beams) from[i] = static_cast<int>(parent);
+        moved |= from[i] ^ i;
+    }
+    if (!moved) return;
+    int low = 0, high = t.count - 1;                       // the tensor of this workgroup
+    while (low < high) {
+        const int middle = (low + high + 1) / 2;
+        if (t.first[middle] <= static_cast<int>(blockIdx.x)) low = middle;
+        else high = middle - 1;
+    }
+    const int unit = (static_cast<int>(blockIdx.x) - t.first[low]) * kThreads + threadIdx.x;
+    if (unit >= t.units[low]) return;
+    using U = std::conditional_t<UNIT == 16, v4w, std::conditional_t<UNIT == 4, uint32_t, uint8_t>>;
+    move_unit<BEAMS, U>(t.data[low] + entry * beams * t.row_stride[low] + static_cast<int64_t>(unit) * UNIT, t.row_stride[low], from, beams);
+}
+
+template <int UNIT>
+int launch(const QaReorderParams& p, const Tensors& t, hipStream_t stream) {
+    const dim3 grid(t.first[t.count], p.batch);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, t, p.parents, p.index_bytes, p.beams); };
+    if (p.beams <= 4) go(reorder_kernel<4, UNIT>);
+    else if (p.beams <= 8) go(reorder_kernel<8, UNIT>);
+    else if (p.beams <= 16) go(reorder_kernel<16, UNIT>);
+    else if (p.beams <= 32) go(reorder_kernel<32, UNIT>);
+    else go(reorder_kernel<64, UNIT>);
+    return check_launch();
+}
+
+int unit_of(const QaStateRows& s) {
+    const uint64_t all = reinterpret_cast<uintptr_t>(s.data) | static_cast<uint64_t>(s.row_bytes) | static_cast<uint64_t>(s.row_stride);
+    return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+}
+
+}  // namespace
+}  // namespace lm
+}  // namespace qa
+
+extern "C" int qa_reorder_states(const QaReorderParams* p, void* stream_) {
+    using namespace qa;
+    using namespace qa::lm;
+    if (!p) return QA_ERR_NULL;
+    if (p->batch < 0 || p->beams < 1 || p->tensors < 0) return QA_ERR_SHAPE;
+    if (p->beams > kMaxBeams || (p->index_bytes != 4 && p->index_bytes != 8)) return QA_ERR_UNSUPPORTED;
+    if (p->batch == 0 || p->tensors == 0) return QA_OK;
+    if (!p->states || !p->parents) return QA_ERR_NULL;
+    if (reinterpret_cast<uintptr_t>(p->parents) % p->index_bytes != 0) return QA_ERR_STRIDE;
+    if (p->batch > 65535) return QA_ERR_SHAPE;
+    for (int i = 0; i < p->tensors; ++i) {
+        const QaStateRows& s = p->states[i];
+        if (s.row_bytes < 0) return QA_ERR_SHAPE;
+        if (s.row_bytes == 0) continue;
+        if (!s.data) return QA_ERR_NULL;
+        if (s.row_stride < s.row_bytes && static_cast<int64_t>(p->batch) * p->beams > 1) return QA_ERR_STRIDE;
+        const int64_t units = s.row_bytes / unit_of(s);
+        if (units > 0x7fffffffLL || !launchable((units + kThreads - 1) / kThreads * p->batch, kThreads)) return QA_ERR_SHAPE;
+    }
+    if (p->beams == 1) return QA_OK;
+    auto all_of = [&](auto unit_c) {
+        constexpr int UNIT = decltype(unit_c)::value;
+        Tensors t = {};
+        auto flush = [&] {
+            const int status = t.count ? launch<UNIT>(*p, t, static_cast<hipStream_t>(stream_)) : QA_OK;
+            t.count = 0;
+            return status;
+        };
+        for (int i = 0; i < p->tensors; ++i) {
+            const QaStateRows& s = p->states[i];
+            if (s.row_bytes == 0 || unit_of(s) != UNIT) continue;
+            const int64_t units = s.row_bytes / UNIT, workgroups = (units + kThreads - 1) / kThreads;
+            if (t.count == kTensors || !launchable((t.first[t.count] + workgroups) * p->batch, kThreads))
+                if (const int status = flush()) return status;
+            t.data[t.count] = static_cast<uint8_t*>(s.data);
+            t.row_stride[t.count] = s.row_stride;
+            t.units[t.count] = static_cast<int32_t>(units);
+            t.first[t.count + 1] = t.first[t.count] + static_cast<int32_t>(workgroups);
+            ++t.count;
+        }
+        return flush();
+    };
+    if (const int status = all_of(std::integral_constant<int, 16>{})) return status;
+    if (const int status = all_of(std::integral_constant<int, 4>{})) return status;
+    return all_of(std::integral_constant<int, 1>{});
+}

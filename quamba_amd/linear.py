@@ -68,6 +68,12 @@ def _tokens_like(tokens, shape):
     return tokens.reshape(-1)
 
 
+def _beams_like(x):
+    if x.dim() != 3:
+        raise RuntimeError(f"x must have shape (batch, beams, features), not {tuple(x.shape)}")
+    return x.shape[:2]
+
+
 def _shaped_logprobs(r, shape):
     top = r.top_tokens.shape[-1]
     return ops.TokenLogprobs(r.logprobs.view(shape), r.entropy.view(shape), r.top_logprobs.view(*shape, top), r.top_tokens.view(*shape, top))
@@ -232,6 +238,18 @@ class W8A8B16O16Linear(_W8A8Base, _AlphaHooks):
             r = ops.token_logprobs(y[:, :self.out_features], flat, top)
         return _shaped_logprobs(r, shape)
 
+    @torch.no_grad()
+    def beam_search_step(self, x, scores, count, done=None, x_scale=None):
+        """As a model's head: the ``count`` best continuations (ops.beam_search_step) after the beams' hidden states ``x`` int8 (batch, beams, in), an
+        ops.BeamCandidates.  The logits are those of ``forward`` (with ``x_scale`` fp32 (batch, beams), of ops.scaled_mm_dq), in fp16."""
+        shape, x2d = _beams_like(x), x.reshape(-1, x.shape[-1]).contiguous()
+        if x_scale is None:
+            y = self._logits(x2d)
+        else:
+            y = torch.empty((x2d.shape[0], self.out_features + self.pad_out), dtype=torch.float16, device=x.device)
+            ops.scaled_mm_dq(y, x2d, self.weight, _token_scales(x_scale, shape, self.a), self.b)
+        return ops.beam_search_step(y.view(*shape, -1)[..., :self.out_features], scores, count, done)
+
     def __repr__(self):
         return f"W8A8B16O16Linear(in_features={self.in_features}, out_features={self.out_features})"
 
@@ -345,6 +363,14 @@ class W4A8B16O16Linear(_W4A8Base):
         y = ops.w4a8o16_gemm(x2d, self.weight, a, self.s_channel, self.s_group, self.workspace, x2d.shape[0], self.size_n, self.size_k)
         return _shaped_logprobs(ops.token_logprobs(y[:, :self.out_features], flat, top), shape)
 
+    @torch.no_grad()
+    def beam_search_step(self, x, scores, count, done=None, x_scale=None):
+        """As W8A8B16O16Linear.beam_search_step."""
+        shape, x2d = _beams_like(x), x.reshape(-1, x.shape[-1]).contiguous()
+        a = _token_scales(x_scale, shape, self.input_scale)
+        y = ops.w4a8o16_gemm(x2d, self.weight, a, self.s_channel, self.s_group, self.workspace, x2d.shape[0], self.size_n, self.size_k)
+        return ops.beam_search_step(y.view(*shape, -1)[..., :self.out_features], scores, count, done)
+
     @classmethod
     def from_fp16(cls, originalLayer: nn.Linear, input_scale: torch.Tensor):
         return cls._from_fp16(originalLayer, input_scale, None)
@@ -369,3 +395,57 @@ class W4A8B8O8LinearParallel(_W4A8Base):
         per_channel = torch.cat([torch.as_tensor(s, dtype=torch.float32).reshape(1).repeat(d)
                                  for d, s in zip(out_split_dims, output_scales)]).cpu()
         return cls._from_fp16(originalLayer, input_scale, per_channel)
+
+
+# ------------------------------------------------------------------------------------------------
+# Microscaled 4-bit floating point: weights and activations in blocks of 32 values with a power of two each,
+# 4.25 bits a weight, on the matrix instructions that take that format.  Activations need no calibration: every
+# block of every token has its own scale.
+# ------------------------------------------------------------------------------------------------
+class MXFP4Linear(nn.Module):
+    """fp16, bf16 or fp32 in and out (``out_dtype``, by default the type of the input): x @ w.T with x and w in the format of ops.mxfp4_quant.
+    ``in_features`` is a multiple of 32, ``out_features`` anything."""
+
+    def __init__(self, in_features, out_features, device=None, out_dtype=None):
+        super().__init__()
+        assert in_features % 32 == 0, "in_features must be a multiple of 32"
+        device = _default_device() if device is None else device
+        self.bias = None
+        self.in_features, self.out_features, self.out_dtype = in_features, out_features, out_dtype
+        self.register_buffer("weight", torch.empty((out_features, in_features // 2), dtype=torch.uint8, device=device))
+        self.register_buffer("weight_scales", torch.empty((-(-in_features // 512), out_features, 16), dtype=torch.uint8, device=device))
+
+    @classmethod
+    def from_fp16(cls, originalLayer: nn.Linear, out_dtype=None):
+        assert originalLayer.bias is None, "Not support bias yet"
+        q = cls(originalLayer.in_features, originalLayer.out_features, originalLayer.weight.device, out_dtype)
+        q.weight, q.weight_scales = ops.mxfp4_quant(originalLayer.weight.detach())
+        return q
+
+    @torch.no_grad()
+    def forward(self, x, x_scales=None):
+        """``x`` (..., in) of numbers; or uint8 codes (..., in / 2) with the ``x_scales`` of ops.mxfp4_quant, for several layers that read the same
+        (fp16 out, unless ``out_dtype`` says otherwise)."""
+        if x_scales is None:
+            return ops.mxfp4_linear(x, self.weight, self.weight_scales, self.out_dtype)
+        y = ops.mxfp4_mm(x.reshape(-1, x.shape[-1]), x_scales, self.weight, self.weight_scales, self.out_dtype or torch.float16)
+        return y.view(*x.shape[:-1], self.out_features)
+
+    @torch.no_grad()
+    def token_logprobs(self, x, tokens, top=0):
+        """As a model's head: ops.token_logprobs of ``forward``."""
+        return ops.token_logprobs(self(x), tokens, top)
+
+    @torch.no_grad()
+    def beam_search_step(self, x, scores, count, done=None):
+        """As a model's head: ops.beam_search_step of ``forward``; ``x`` (batch, beams, in)."""
+        _beams_like(x)
+        return ops.beam_search_step(self(x), scores, count, done)
+
+    @torch.no_grad()
+    def dequantized_weight(self, dtype=torch.float32):
+        """The values (out, in) that the weights have."""
+        return ops.mxfp4_dequant(self.weight, self.weight_scales, dtype)
+
+    def __repr__(self):
+        return f"MXFP4Linear(in_features={self.in_features}, out_features={self.out_features}, out_dtype={self.out_dtype})"

@@ -373,3 +373,9 @@ class W8A8QMamba2(W4A8QMamba2):
     """The W8A8 Mamba2 mixer of quamba/qMamba2.py:1071-1400: the same chain with int8 weights in in_proj (one
     output scale per z | x | B | C | dt segment) and out_proj."""
     _in_proj_cls, _out_proj_cls = W8A8B8O8LinearParallel, W8A8B16O16Linear
+
+
+def reorder_cache(inference_params, parents):
+    """The states of all layers in an inference_params cache (``key_value_memory_dict``: layer -> (conv_state, ssm_state)) in the beams' new order, in
+    place: row b * beams + i becomes what row b * beams + parents[b, i] was (ops.reorder_states)."""
+    ops.reorder_states([state for states in inference_params.key_value_memory_dict.values() for state in states], parents)

@@ -937,3 +937,99 @@ def scaled_mm_token_logprobs(a, b, a_scales, b_scales, tokens, top=0, vocab=None
     elements, tokens int32 or int64 (M,), top 0 or 1.  vocab: how many of b's columns are tokens (default all; the others are
     padding).  Returns TokenLogprobs."""
     return TokenLogprobs._make(_lm().scaled_mm_token_logprobs(a, b, a_scales, b_scales, tokens, top, vocab))
+
+
+# ----------------------------------------------------------------------------------------------
+# Microscaled 4-bit floating point, and beam search
+# ----------------------------------------------------------------------------------------------
+_mx_beam_native = None
+
+
+def _mx_beam():
+    """quamba_amd._mx_beam_host, bound to the library; raises if it is not built (there is no fallback)."""
+    global _mx_beam_native
+    if _mx_beam_native is None:
+        try:
+            from . import _mx_beam_host as native
+        except ImportError as e:
+            raise RuntimeError("quamba_amd/_mx_beam_host.so is missing or does not load: build it with `python -m quamba_amd.build`") from e
+        if (getattr(native, "MX_ABI_VERSION", None), getattr(native, "BEAM_ABI_VERSION", None)) != (_lib.MX_ABI_VERSION, _lib.BEAM_ABI_VERSION):
+            raise RuntimeError("quamba_amd/_mx_beam_host.so is built for another layout of the parameter blocks: rebuild it with "
+                               "`python -m quamba_amd.build --force`")
+        l = _lib.lib()
+        native.bind(tuple(ct.cast(getattr(l, n), ct.c_void_p).value for n in (
+            "qa_mxfp4_quant", "qa_mxfp4_dequant", "qa_mxfp4_mm_workspace_bytes", "qa_mxfp4_mm", "qa_beam_search_workspace_bytes", "qa_beam_search_step",
+            "qa_reorder_states")),
+            (torch.cuda.current_device, torch.cuda.set_device, torch._C._cuda_getCurrentRawStream, torch.cuda.OutOfMemoryError, _lib.check))
+        _mx_beam_native = native
+    return _mx_beam_native
+
+
+def mxfp4_quant(x):
+    """Rows in microscaled 4-bit floating point (qa_mxfp4_quant): of each 32 neighbours along the last dimension every value becomes
+    one of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times 2^e, e = floor(log2(max|x|)) - 2 and at least -127; the nearest of them, the even code where
+    two are as near, at most 6.  A block with a NaN or an infinity is NaN as a whole.  x (..., K) fp16, bf16 or fp32, K a multiple of 32.
+
+    Returns (codes uint8 (..., K / 2), scales uint8 (groups, rows, 16)).  Two codes are a byte, the earlier value in the low half.  scales hold
+    e + 127, 255 for NaN: 16 blocks, 512 values, are a group, rows are counted over the dimensions in front, and block 4 j + q of
+    a group (j, q = 0 .. 3) is at place 4 q + j; mxfp4_scales and mxfp4_scales_of turn one order into the other."""
+    return _mx_beam().mxfp4_quant(x)
+
+
+def mxfp4_dequant(codes, scales, dtype=torch.float32):
+    """The values (..., K) that codes and scales of mxfp4_quant stand for, rounded to dtype (qa_mxfp4_dequant)."""
+    return _mx_beam().mxfp4_dequant(codes, scales, dtype)
+
+
+def mxfp4_scales(scales):
+    """(rows, K / 32), the scale of block b of a row at place b, in the order of mxfp4_quant: (groups, rows, 16)."""
+    _require(scales.dim() == 2 and scales.dtype == torch.uint8, "scales must be uint8 (rows, K / 32)")
+    rows, blocks = scales.shape
+    groups = -(-blocks // 16)
+    return torch.nn.functional.pad(scales, (0, groups * 16 - blocks)).view(rows, groups, 4, 4).permute(1, 0, 3, 2).reshape(groups, rows, 16).contiguous()
+
+
+def mxfp4_scales_of(scales, blocks):
+    """The first ``blocks`` scales of each row, (rows, blocks), of what mxfp4_quant gives."""
+    _require(scales.dim() == 3 and scales.shape[2] == 16 and scales.dtype == torch.uint8, "scales must be uint8 (groups, rows, 16)")
+    _require(0 <= blocks <= 16 * scales.shape[0], "more blocks than there are scales")
+    return scales.unflatten(2, (4, 4)).permute(1, 0, 3, 2).reshape(scales.shape[1], 16 * scales.shape[0])[:, :blocks]
+
+
+def mxfp4_mm(a, a_scales, w, w_scales, out_dtype=torch.float16):
+    """a @ w.T of two operands as mxfp4_quant gives them, summed in fp32 and rounded once (qa_mxfp4_mm): a uint8 (M, K / 2), w uint8 (N, K / 2).
+    Returns (M, N) of out_dtype, fp16, bf16 or fp32.  Rows of codes may lie apart, on 16 bytes."""
+    return _mx_beam().mxfp4_mm(a, a_scales, w, w_scales, out_dtype)
+
+
+def mxfp4_linear(x, w, w_scales, out_dtype=None):
+    """mxfp4_mm(*mxfp4_quant(x), w, w_scales), bit for bit: x (..., K) fp16, bf16 or fp32, w uint8 (N, K / 2).  Returns (..., N) of out_dtype, by default
+    that of x.  Few rows are quantised where they are multiplied, in one launch."""
+    return _mx_beam().mxfp4_linear(x, w, w_scales, out_dtype)
+
+
+class BeamCandidates(NamedTuple):
+    """What beam_search_step returns, the best first."""
+    scores: torch.Tensor            # fp32 (batch, count): -inf where there is no candidate
+    tokens: torch.Tensor            # int64 (batch, count): -1 of a beam that is done, and where there is no candidate
+    parents: torch.Tensor           # int64 (batch, count): the beam that offers it, -1 where there is no candidate
+
+
+def beam_search_step(logits, scores, count, done=None):
+    """The ``count`` best continuations of each entry's beams (qa_beam_search_step): beam i offers token v with the score
+    scores[b, i] + log_softmax(logits[b, i])[v].  logits (batch, beams, vocab) fp16, bf16 or fp32, contiguous along the last dimension, up to 64
+    beams; scores fp32 (batch, beams); 1 <= count <= 64.  Scores are compared in 64 bits; of equal ones the lower beam's
+    comes first, then the lower token's.  Returns BeamCandidates.
+
+    ``done`` bool (batch, beams): such a beam offers itself once, with its score and the token -1, whatever its logits.  A score of -inf is
+    no candidate: masked tokens, and beams that are not there (the first step: one beam with 0, the others with -inf).  A beam offers nothing either if
+    its logits are all -inf or hold a NaN or +inf, or its score is NaN or +inf."""
+    return BeamCandidates._make(_mx_beam().beam_search_step(logits, scores, count, done))
+
+
+def reorder_states(states, parents):
+    """The beams' states in their new order, in place and in one launch for up to 96 tensors (qa_reorder_states): row b * beams + i of
+    every tensor becomes what row b * beams + parents[b, i] was.  states: a tensor or a sequence of them, of any types, with batch * beams rows
+    along the first dimension, each row in one piece (its dimensions in any order, as conv states have them); no two may share memory.  parents int32 or
+    int64 (batch, beams), up to 64 beams.  A row whose parent is itself, or not one of the entry's beams (-1), stays as it is."""
+    _mx_beam().reorder_states(states, parents)

@@ -6,7 +6,7 @@ namespace mx {
 namespace {
 
 constexpr int kFusedRows = 16;             // of numbers, quantised where they are multiplied
-constexpr int64_t kMaxPitch = 1 << 24;     // bytes of an operand's row: 64 of them in 32 bits
+constexpr int64_t kMaxPitch = 1 << 22;     // bytes of an operand's row: those of a tile in 32 bits
 
 int check(const QaMxGemmParams& p) {
     if (p.m < 0 || p.n < 0 || p.k < 0) return QA_ERR_SHAPE;
@@ -62,7 +62,9 @@ extern "C" int qa_mxfp4_mm(const QaMxGemmParams* p, void* stream_) {
     const int64_t need = workspace_bytes(*p);
     if (need && !p->workspace) return QA_ERR_NULL;
     if (need && (!aligned16(p->workspace) || p->workspace_bytes < need)) return QA_ERR_SCRATCH;
-    if (rows_of_codes || fused(*p)) return direct_launch(*p, stream);
+    auto of_codes = [&](const QaMxGemmParams& q) { return direct_takes(q) ? direct_launch(q, stream) : tiles_launch(q, stream); };
+    if (fused(*p)) return direct_launch(*p, stream);
+    if (rows_of_codes) return of_codes(*p);
     // many rows of numbers: quantised once, for all columns
     QaMxQuantParams rows = {};
     rows.rows = p->m; rows.k = p->k; rows.x_type = p->a_type;
@@ -75,5 +77,5 @@ extern "C" int qa_mxfp4_mm(const QaMxGemmParams* p, void* stream_) {
     product.a_type = QA_LM_I8;
     product.a = rows.codes; product.lda = rows.code_row_stride;
     product.a_scales = rows.scales; product.a_scale_group_stride = rows.scale_group_stride;
-    return direct_launch(product, stream);
+    return of_codes(product);
 }

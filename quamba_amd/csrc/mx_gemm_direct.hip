@@ -114,23 +114,38 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mxfp4_direct_kernel(QaMxGemmPa
         }
 }
 
+template <int RM, int RN>
+int64_t blocks_of(const QaMxGemmParams& p) { return ((p.m + RM * 16 - 1) / (RM * 16)) * static_cast<int64_t>((p.n + RN * 16 - 1) / (RN * 16)); }
+
 template <int RM, int RN, class ROWS_T>
 int launch(const QaMxGemmParams& p, hipStream_t stream) {
-    const int64_t tiles_m = (p.m + RM * 16 - 1) / (RM * 16), tiles_n = (p.n + RN * 16 - 1) / (RN * 16);
+    const int64_t tiles_m = (p.m + RM * 16 - 1) / (RM * 16), blocks = blocks_of<RM, RN>(p);
     const int waves = static_cast<int>(std::min<int64_t>(kMaxWaves, std::max<int64_t>(1, groups_of(p.k))));
-    if (!launchable(tiles_m * tiles_n, 64 * waves)) return QA_ERR_SHAPE;
-    hipLaunchKernelGGL((mxfp4_direct_kernel<RM, RN, ROWS_T>), dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(64 * waves),
+    if (!launchable(blocks, 64 * waves)) return QA_ERR_SHAPE;
+    hipLaunchKernelGGL((mxfp4_direct_kernel<RM, RN, ROWS_T>), dim3(static_cast<unsigned>(blocks)), dim3(64 * waves),
                        waves > 1 ? waves * RM * RN * 64 * sizeof(v4f) : 0, stream, p, static_cast<int>(tiles_m), whole_words(p));
     return check_launch();
 }
 
 }  // namespace
 
+// Rows of numbers: any number of columns.  Codes: the smallest blocks of which each CU has one at most, and up to 16 rows as long as the weights are not so many that
+// tiles ask for them better.  (us by 16 x 16, 32 x 16, 32 x 32, 64 x 32 and in tiles: 64 x 768 x 2560 4.1, 4.5, 5.5, 8, 8; 128 x 768 x 2560 5.1, 4.6, 5.3, 8, 8;
+// 64 x 2560 x 2560 6.7, 6.7, 5.3, 7.3, 7.8; 128 x 2560 x 2560 9.2, 8.8, 8.4, 7.4, 8.0; 16 x 10240 x 2560 6.4, 7.0, 7.0, 8.1, 7.8; 17 x 10240 x 2560 9.1, 7.1, 7.1, 8.3, 7.9;
+// 1 x 50280 x 2560 13.8, 17, 15, 20, 12.5.)
+bool direct_takes(const QaMxGemmParams& p) {
+    const int64_t cus = compute_units();
+    return blocks_of<4, 2>(p) <= cus || (p.m <= 16 && blocks_of<1, 1>(p) <= 10 * cus);
+}
+
 int direct_launch(const QaMxGemmParams& p, hipStream_t stream) {
     if (p.a_type == QA_LM_F32) return launch<1, 1, float>(p, stream);
     if (p.a_type == QA_LM_BF16) return launch<1, 1, __bf16>(p, stream);
     if (p.a_type == QA_LM_F16) return launch<1, 1, _Float16>(p, stream);
-    if (p.m <= 16) return launch<1, 1, int8_t>(p, stream);
+    const int64_t cus = compute_units();
+    if (p.m <= 16 || blocks_of<1, 1>(p) <= cus) return launch<1, 1, int8_t>(p, stream);
+    if (blocks_of<2, 1>(p) <= cus) return launch<2, 1, int8_t>(p, stream);
+    if (blocks_of<2, 2>(p) <= cus) return launch<2, 2, int8_t>(p, stream);
     return launch<4, 2, int8_t>(p, stream);
 }
 

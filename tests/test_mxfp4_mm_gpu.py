@@ -17,7 +17,7 @@ TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
 SIZES = [(1, 1, 32), (1, 16, 64), (1, 10, 768), (1, 2560, 2560), (2, 100, 96), (3, 257, 512), (5, 48, 544), (15, 33, 1056), (16, 64, 160), (17, 130, 480), (31, 1000, 1536),
          (32, 96, 2048), (33, 31, 992), (48, 1537, 768), (63, 65, 1024), (64, 500, 2560), (64, 4100, 256), (65, 127, 352), (96, 200, 4096), (127, 129, 1248), (128, 128, 1024),
          (129, 384, 608), (200, 777, 2592), (255, 257, 512), (256, 256, 1536), (257, 1000, 736), (384, 513, 2080), (500, 2560, 640), (511, 640, 3104), (1000, 1111, 288),
-         (1021, 50, 1536), (2049, 300, 416), (40, 20000, 96), (3000, 17, 768), (300, 5000, 32), (700, 3001, 1024)]
+         (1021, 50, 1536), (2049, 300, 416), (40, 20000, 96), (3000, 17, 768), (300, 5000, 32), (700, 3001, 1024), (4300, 4201, 1024), (4300, 4201, 160), (4300, 5501, 1536), (600, 50001, 512), (12000, 1501, 1536)]
 
 
 def exact_case(g, m, n, k, dev):

@@ -21,13 +21,13 @@ int qa_beam_abi_version(void);
  * Of each of `batch` entries the `count` best continuations of its beams.  Beam i offers every token v with the score
  *   scores[b, i] + l[b, i, v] - log sum_u exp l[b, i, u]
  * in 64 bits, rounded to fp32 as it is written; larger scores come first, of equal ones the lower beam's, then the lower token's.
- * (Tokens of one beam are ranked by their logits.)
+ * (Tokens of one beam whose logits differ by less than 64 bits of their scores show come in either order.)
  * A beam that is done offers itself once, with its score and the token -1, and its logits are not read.  A score of -inf is no offer: masked
  * tokens, and beams whose own score is that.  A beam offers nothing either where its logits are all -inf or hold a NaN or +inf, or where
  * its score is NaN or +inf.  Places that are left without an offer get the score -inf, the token -1 and the parent -1.
  */
 typedef struct QaBeamSearchParams {
-    int32_t batch, beams, vocab;    /* beams 1 .. 64, vocab up to 2^30 */
+    int32_t batch, beams, vocab;    /* beams 1 .. 64, vocab up to 2^20 */
     int32_t logits_type;            /* QaLmType, not I8 */
     int32_t count;                  /* 1 .. 64, at most beams * vocab */
     int32_t reserved0;

@@ -1,11 +1,11 @@
 // The best continuations over the beams and the vocabulary (qa_beam_search_step).
 //
-// Two launches: every row of logits, cut into segments as token_logprobs cuts them, leaves for each segment the sum of its exponentials and its best
-// `count` entries by logit; then a workgroup for each entry of the batch joins the segments of its beams, turns the entries into scores and merges the beams'.
+// Two launches: every row of logits, cut into segments, leaves for each segment the sum of its exponentials and its best `count` entries by logit; then a
+// workgroup for each entry of the batch joins the sums of its beams, turns the entries into scores and sorts those that reach a bound.
 //
 // Scores of different beams are compared, and which of two comes first is an answer in whole numbers.  So the sums are held in 64 bits and their terms are good to
-// some 1e-10: exp_wide takes 2^(n / 64) from a table and e^r, |r| <= ln 2 / 128, from a polynomial whose first missing term is r^4 / 24 < 4e-11 - nine operations in
-// 64 bits, which run at the rate of those in 32.
+// some 1e-10: e^d is 2^(n / 512) from a table by e^r, |r| <= ln 2 / 1024, from a polynomial whose first missing term is r^3 / 6 < 6e-11.  Operations in 64 bits run at
+// the rate of those in 32, and thirteen instructions a value are what a launch on many rows takes its time for.
 #include "../../include/quamba_amd_beam.h"
 #include "logit_rows.hpp"
 
@@ -13,60 +13,106 @@ namespace qa {
 namespace lm {
 namespace {
 
-constexpr int kMaxBeams = 64;
+constexpr int kMaxBeams = 64, kMaxVocab = 1 << 20;
+constexpr int kMaxLoads = 16;              // chunks of a segment
 
+// A sum of exponentials is s 2^e e^m: e keeps s near 1 where the logits are, m is 0 unless they are further from 0 than kFarthest.
 struct BeamPart {
     float m;
-    float pad;
+    int e;
     double s;
 };
 
-// e^d for d from -700 to 0 (a NaN stays one); powers[i] = 2^(i / 64)
-__device__ __forceinline__ double exp_wide(double d, const double* powers) {
-    constexpr double kPerUnit = 92.332482616893657, kStep = 0.010830424696249145, kRound = 6755399441055744.0;       // 64 log2 e, ln 2 / 64, 1.5 * 2^52
-    const double shifted = __builtin_fma(d, kPerUnit, kRound);
-    const int n = static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, shifted)));
-    const double r = __builtin_fma(shifted - kRound, -kStep, d);
-    double e = __builtin_fma(r, 1.0 / 6.0, 0.5);
-    e = __builtin_fma(e, r, 1.0);
-    e = __builtin_fma(e, r, 1.0);
-    const uint64_t power = __builtin_bit_cast(uint64_t, powers[n & 63]) + (static_cast<uint64_t>(static_cast<uint32_t>(n >> 6)) << 52);
-    return e * __builtin_bit_cast(double, power);
-}
-
-// sum e^(l - m) of a part of a row, as RowStats but in 64 bits
-struct WideStats {
+// The sum of a part of a row, by one wave (m and e are the same in its lanes).  64 bits hold e^600 as well as e^-600, so where the first values are is good enough until one is
+// more than kReach above it.
+constexpr float kReach = 600.0f;
+constexpr int kSteps = 512;
+constexpr double kLn2Wide = 0.69314718055994531;
+struct WideSum {
     float m;
+    int e;
     double s;
-    __device__ __forceinline__ void clear() { m = kLowest; s = 0.0; }
-    __device__ __forceinline__ void raise(float most, const double* powers) {
-        s *= exp_wide(fmax(static_cast<double>(m) - most, -700.0), powers);
-        m = most;
+    bool placed;               // a value was seen
+    __device__ __forceinline__ void clear() { m = 0.0f; e = 0; s = 0.0; placed = false; }
+    // seen from where values up to `most` are
+    __device__ __forceinline__ void place(float most) {
+        const float before_m = m;
+        const int before_e = e;
+        const bool near = fabsf(most) <= kFarthest;
+        m = near ? 0.0f : most;
+        e = near ? static_cast<int>(rintf(most * kLog2e)) : 0;
+        if (placed) s *= exp(fmax((static_cast<double>(before_m) - m) + (before_e - e) * kLn2Wide, -700.0));
+        placed = true;
     }
-    // (a comparison, and not a maximum, which would drop a NaN)
-    __device__ __forceinline__ void add(float value, const double* powers) {
-        const double d = static_cast<double>(value) - m;
-        s += exp_wide(d < -700.0 ? -700.0 : d, powers);
-    }
-    template <int A, int B>
-    __device__ __forceinline__ void add_batch(const float (&v)[A][B], int loads, float most, const double* powers) {
-        raise(fmaxf(m, most), powers);
-        const bool far = __builtin_amdgcn_ballot_w64(!(fabsf(m) <= kFarthest));
-        const float least = m - 700.0f;
+    // e^d, d from -700 to kReach + some (a NaN stays one), added for B values d = v - m; powers[i] = 2^(i / kSteps).  In steps, so that the reads of the table are on their way together: one after
+    // the other they took 130 cycles a value, most of it waiting.
+    template <int B>
+    __device__ __forceinline__ void add_exponentials(const double (&d)[B], const double* powers) {
+        constexpr double kPerUnit = 738.65986093514926, kStep = 0.0013538030870311431;     // 512 log2 e, ln 2 / 512
+        // (1.5 * 2^52: the rounded multiple of a step is in the low word; less the steps of 2^e)
+        const double round = 6755399441055744.0 - static_cast<double>(e) * kSteps;
+        int n[B];
+        double value[B], power[B];
 #pragma unroll
-        for (int i = 0; i < A; ++i) {
-            if (i >= loads) break;
-            if (far) {
+        for (int j = 0; j < B; ++j) {
+            const double shifted = __builtin_fma(d[j], kPerUnit, round);
+            n[j] = static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, shifted)));
+            const double r = __builtin_fma(shifted - round, -kStep, d[j]);
+            value[j] = __builtin_fma(__builtin_fma(r, 0.5, 1.0), r, 1.0);
+        }
 #pragma unroll
-                for (int j = 0; j < B; ++j) add(v[i][j], powers);
-            } else {
-                // (the same, compared in 32 bits)
+        for (int j = 0; j < B; ++j) power[j] = powers[n[j] & (kSteps - 1)];
 #pragma unroll
-                for (int j = 0; j < B; ++j) s += exp_wide(static_cast<double>(v[i][j] < least ? least : v[i][j]) - m, powers);
-            }
+        for (int j = 0; j < B; ++j) {
+            // (into the exponent, which stays a normal one)
+            const uint64_t bits = __builtin_bit_cast(uint64_t, power[j]);
+            const uint32_t high = static_cast<uint32_t>(bits >> 32) + (static_cast<uint32_t>(n[j] & ~(kSteps - 1)) << (20 - 9));
+            s = __builtin_fma(value[j], __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(bits)), s);
         }
     }
+    static_assert(kSteps == 1 << 9, "the shift into the exponent");
+    // values of which `most` is the largest of this lane's
+    template <int B>
+    __device__ __forceinline__ void add(const float (&v)[B], float most, const double* powers) {
+        const float here = !placed ? -__builtin_inff() : m != 0.0f ? m : static_cast<float>(e) * kLn2;
+        if (__builtin_amdgcn_ballot_w64(placed ? most - here > kReach : most > here)) place(wave_max(fmaxf(most, here)));
+        if (!placed) {
+            // (masked values alone, or NaNs)
+#pragma unroll
+            for (int j = 0; j < B; ++j) s = v[j] == v[j] ? s : __builtin_nan("");
+            return;
+        }
+        double d[B];
+        if (m == 0.0f) {
+            const float least = static_cast<float>(e) * kLn2 - 700.0f;
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                float one;                                 // (the larger, a NaN if there is one)
+                asm("v_maximum3_f32 %0, %1, %2, %2" : "=v"(one) : "v"(v[j]), "v"(least));
+                d[j] = one;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < B; ++j) {
+                d[j] = static_cast<double>(v[j]) - m;
+                d[j] = d[j] < -700.0 ? -700.0 : d[j];
+            }
+        }
+        add_exponentials(d, powers);
+    }
 };
+
+// Both sums as one, seen from the higher place.
+__device__ __forceinline__ BeamPart joined(BeamPart a, BeamPart b) {
+    if (a.s == 0.0 || b.s == 0.0) return a.s == 0.0 ? b : a;
+    if (a.m == 0.0f && b.m == 0.0f) {
+        const int e = max(a.e, b.e);
+        return {0.0f, e, ldexp(a.s, max(a.e - e, -2000)) + ldexp(b.s, max(b.e - e, -2000))};
+    }
+    const double apart = (static_cast<double>(b.m) - a.m) + (b.e - a.e) * kLn2Wide;
+    if (apart > 0.0) return {b.m, b.e, a.s * exp(fmax(-apart, -700.0)) + b.s};
+    return {a.m, a.e, a.s + b.s * exp(fmax(apart, -700.0))};
+}
 
 __device__ __forceinline__ double lane_double(double v, int from) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
@@ -75,155 +121,178 @@ __device__ __forceinline__ double lane_double(double v, int from) {
     return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 // over the wave, in every lane: the order of the sum is that of the lanes' numbers' bits, the same in all of them
-__device__ __forceinline__ WideStats wave_stats(WideStats r, const double* powers, int lane) {
-    r.raise(wave_max(r.m), powers);
+__device__ __forceinline__ double wave_sum(double s, int lane) {
 #pragma unroll
-    for (int mask = 1; mask < 64; mask *= 2) r.s += lane_double(r.s, lane ^ mask);
-    return r;
+    for (int mask = 1; mask < 64; mask *= 2) s += lane_double(s, lane ^ mask);
+    return s;
 }
 
-__device__ __forceinline__ void fill_powers(double (&powers)[64]) {
-    if (threadIdx.x < 64) powers[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / 64.0);
+__device__ __forceinline__ void fill_powers(double (&powers)[kSteps]) {
+    for (int i = threadIdx.x; i < kSteps; i += blockDim.x) powers[i] = exp2(static_cast<double>(i) / kSteps);
 }
 
-template <class T, bool WIDE, bool ONE, int LOADS>
-__global__ __launch_bounds__(64 * kWaves) void beam_rows_kernel(QaBeamSearchParams p, int top, int segments, int batches_each) {
-    constexpr int V = 16 / sizeof(T), W = kWaves;
-    __shared__ BeamPart s_part[kWaves];
-    __shared__ float s_bound[kWaves];
-    __shared__ Entry s_best[kWaves][64];
+typedef uint64_t v2k __attribute__((ext_vector_type(2)));
+// How many of the first `n` keys are larger than one, and as large; up to seven behind them are 0 (which no key that is looked at is).
+struct Above {
+    int larger, equal;
+};
+__device__ __forceinline__ Above above(const uint64_t* keys, int n, uint64_t own) {
+    Above a = {0, 0};
+    for (int o = 0; o < n; o += 8) {
+        v2k k[4];                                          // (on their way together)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const v2k*>(keys + o + 2 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a.larger += (k[i][0] > own) + (k[i][1] > own);
+            a.equal += (k[i][0] == own) + (k[i][1] == own);
+        }
+    }
+    return a;
+}
+
+// A workgroup has a segment of up to kMaxLoads chunks, one load a lane each; kAhead of them are under way while one is summed.  What each load's largest value is goes to LDS, and
+// when all were seen a bound says which loads have one of the best entries: those are read once more, all at the same time, and what reaches the bound is ranked (each
+// counts the others that are larger).  A short loop: with four loads a batch and the entries kept on the way, as token_logprobs has them, the code was
+// larger than the instruction cache and 64 x 8 rows of 50280 took 35 us.
+constexpr int kAhead = 3;
+
+template <class T, bool WIDE>
+__global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchParams p, int top, int segments, int each) {
+    constexpr int V = 16 / sizeof(T), W = kWaves, kThreads = 64 * W;
+    typedef BestOfBatches<V> Run;
+    __shared__ BeamPart s_part[W];
     __shared__ Candidates s_candidates;
-    __shared__ Entry s_waiting[kWaves][BestOfBatches<V>::kWaiting];
-    __shared__ double s_powers[64];
+    __shared__ union {
+        float most[kMaxLoads][kThreads];
+        Entry waiting[W][Run::kWaiting];
+    } s;
+    __shared__ uint32_t s_loads[kCandidates];              // (chunk, thread) of those that are read once more
+    __shared__ double s_powers[kSteps];
+    __shared__ int s_count;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x / segments, segment = blockIdx.x % segments, entry = row / p.beams, beam = row % p.beams;
     if (p.done && p.done[row]) return;                     // (its part is not looked at)
     const T* const logits = static_cast<const T*>(p.logits) + entry * p.logits_batch_stride + beam * p.logits_beam_stride;
     const int vectors = p.vocab / V, rest = p.vocab - vectors * V;
-    const int first = segment * batches_each, end = ONE ? first + 1 : min(first + batches_each, (vectors + W * 64 * LOADS - 1) / (W * 64 * LOADS));
+    const int first = segment * each, loads = min(each, (vectors + kThreads - 1) / kThreads - first);
     const float none = -__builtin_inff();
 
+    // load u of thread `thread` (what is not there: the last one)
+    auto place = [&](int u, int thread) { return (first + u) * kThreads + thread; };
+    auto load = [&](Raw<T, V>& raw, int u, int thread) __attribute__((always_inline)) {
+        raw.template load<WIDE>(logits + static_cast<int64_t>(min(place(u, thread), vectors - 1)) * V);
+    };
+    Raw<T, V> raw[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (i < loads) load(raw[i], i, threadIdx.x);
     // fewer than V values behind the last whole load: one each in the first lanes of the last segment
     const int rest_at = vectors * V + lane;
     const bool has_rest = segment == segments - 1 && wave == 0 && lane < rest;
     float rest_v = none;
     if (has_rest) rest_v = static_cast<float>(logits[rest_at]);
     fill_powers(s_powers);
+    if (threadIdx.x == 0) s_count = 0;
     __syncthreads();
-    WideStats r;
+    WideSum r;
     r.clear();
-    BestEntries best;
-    best.clear();
-    BestOfBatches<V> run;
-    if constexpr (!ONE) run.clear(s_waiting[wave]);
-    // WHOLE: every lane has its loads
-    auto batch = [&](int b, auto whole_c) __attribute__((always_inline)) {
-        constexpr bool WHOLE = decltype(whole_c)::value;
-        Raw<T, V> raw[LOADS];
-        int at[LOADS];
-        float v[LOADS][V], most_of[LOADS], most = none;
+    float most = rest_v;
+    for (int u = 0; u < loads; ++u) {
+        const Raw<T, V> now = raw[0];
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            at[u] = ((b * LOADS + u) * W + wave) * 64 + lane;
-            if (!ONE || vectors > 0) raw[u].template load<WIDE>(logits + static_cast<int64_t>(WHOLE ? at[u] : min(at[u], vectors - 1)) * V);
+        for (int i = 0; i + 1 < kAhead; ++i) raw[i] = raw[i + 1];
+        if (u + kAhead < loads) load(raw[kAhead - 1], u + kAhead, threadIdx.x);
+        float v[V], most_of = none;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = now.get(j);
+        if ((first + u + 1) * kThreads > vectors && place(u, threadIdx.x) >= vectors) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = none;
         }
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            most_of[u] = none;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                v[u][j] = WHOLE || at[u] < vectors ? raw[u].get(j) : none;
-                most_of[u] = fmaxf(most_of[u], v[u][j]);
-            }
-            most = fmaxf(most, most_of[u]);
-        }
-        if constexpr (ONE) most = fmaxf(most, rest_v);
-        const int wanted = (vectors - (b * LOADS * W + wave) * 64 + W * 64 - 1) / (W * 64);        // loads with a lane that has one
-        r.add_batch(v, WHOLE ? LOADS : __builtin_amdgcn_readfirstlane(wanted), most, s_powers);
-        if constexpr (ONE) {
-            best = pick<V>([&](auto&& f) __attribute__((always_inline)) {
-#pragma unroll
-                for (int u = 0; u < LOADS; ++u) f(v[u], most_of[u], at[u] < vectors, static_cast<uint32_t>(at[u] * V));
-                const float one[1] = {rest_v};
-                f(one, rest_v, has_rest, static_cast<uint32_t>(rest_at));
-            }, most, top, s_candidates, s_best, s_waiting[wave], wave, lane);
-        } else {
-            run.batch(most, top, lane);
-#pragma unroll
-            for (int u = 0; u < LOADS; ++u) run.take(v[u], most_of[u], WHOLE || at[u] < vectors, static_cast<uint32_t>(at[u] * V), top, lane);
-        }
+        for (int j = 0; j < V; ++j) most_of = fmaxf(most_of, v[j]);
+        s.most[u][threadIdx.x] = most_of;
+        most = fmaxf(most, most_of);
+        r.add(v, most_of, s_powers);
+    }
+    const float one[1] = {rest_v};
+    if (segment == segments - 1 && wave == 0) r.add(one, rest_v, s_powers);
+    r.s = wave_sum(r.s, lane);
+    if (lane == 0) s_part[wave] = {r.m, r.e, r.s};
+
+    const float bound = bound_of_lanes(most, top, s_candidates, wave, lane);
+    for (int u = 0; u < loads; ++u) {
+        // (of lanes that are not there: -inf)
+        if (!(s.most[u][threadIdx.x] >= bound) || place(u, threadIdx.x) >= vectors) continue;
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kCandidates) s_loads[at] = u << 16 | threadIdx.x;
+    }
+    auto candidate = [&](float value, uint32_t index) {
+        if (!(value >= bound)) return;
+        const int at = atomicAdd(&s_candidates.count, 1);
+        if (at < kCandidates) s_candidates.at[at] = entry_of(value, index);
     };
-    if constexpr (ONE) {
-        batch(first, std::false_type{});
-        r.add(rest_v, s_powers);
-    } else {
-        const int whole = min(end, vectors / (W * 64 * LOADS));
-        int b = first;
-        for (; b < whole; ++b) batch(b, std::true_type{});
-        for (; b < end; ++b) batch(b, std::false_type{});
-        if (segment == segments - 1 && wave == 0 && rest) {
-            r.raise(fmaxf(r.m, rest_v), s_powers);
-            r.add(rest_v, s_powers);
-            const float one[1] = {rest_v};
-            run.next_batch(top);
-            run.take(one, rest_v, has_rest, static_cast<uint32_t>(rest_at), top, lane);
-        }
-    }
-    r = wave_stats(r, s_powers, lane);
-    if (lane == 0) {
-        s_part[wave] = {r.m, 0.0f, r.s};
-        if constexpr (!ONE) s_bound[wave] = value_of_key(run.bound);
-    }
-    bool sorted = false;                                   // (of the same value in all waves)
-    if constexpr (!ONE) {
-        // what waits reaches the bound of its wave; what counts, the largest of the waves' bounds
-        if (threadIdx.x == 0) s_candidates.count = 0;
-        if (lane == 0) s_candidates.keys[wave][0] = run.best.last != 0;
-        __syncthreads();
-        float bound = s_bound[0];
+    if (has_rest) candidate(rest_v, rest_at);
+    __syncthreads();
+    const int again = s_count;
+    if (static_cast<int>(threadIdx.x) < again && again <= kCandidates) {
+        const int u = s_loads[threadIdx.x] >> 16, thread = s_loads[threadIdx.x] & 0xffff;
+        Raw<T, V> once_more;
+        load(once_more, u, thread);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            bound = fmaxf(bound, s_bound[w]);
-            sorted |= s_candidates.keys[w][0] != 0;
-        }
-        if (!sorted) {
-            static_assert(kCandidates >= 64 * kWaves, "room for all that wait");
-            run.wave_order();
-            const Entry e = lane < run.count ? s_waiting[wave][lane] : 0;
-            if (e != 0 && value_of(e) >= bound) s_candidates.at[atomicAdd(&s_candidates.count, 1)] = e;
-        } else {
-            run.finish(top, lane);
-            best = run.best;
-            s_best[wave][lane] = best.mine;
-        }
+        for (int j = 0; j < V; ++j) candidate(once_more.get(j), static_cast<uint32_t>(place(u, thread) * V + j));
     }
+    __syncthreads();
+    BeamPart* const parts = static_cast<BeamPart*>(p.workspace);
+    Entry* const out = reinterpret_cast<Entry*>(parts + static_cast<int64_t>(p.batch) * p.beams * segments) + static_cast<int64_t>(blockIdx.x) * top;
+    if (threadIdx.x == 64) parts[blockIdx.x] = joined(joined(s_part[0], s_part[1]), joined(s_part[2], s_part[3]));
+    static_assert(W == 4, "a sum of each wave");
+    const int count = s_candidates.count;
+    if (again <= kCandidates && count <= kCandidates - 8) {
+        if (threadIdx.x < 8) s_candidates.at[count + threadIdx.x] = 0;
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < count) {
+            const Entry mine = s_candidates.at[threadIdx.x];
+            const int before = above(s_candidates.at, count, mine).larger;
+            if (before < top) out[before] = mine;
+        } else if (static_cast<int>(threadIdx.x) < top) {
+            out[threadIdx.x] = 0;
+        }
+        return;
+    }
+    // more reach the bound than there is room for - equal values, or as many as lanes are asked for: every wave keeps its own best as it goes through its loads again
+    Run run;
+    run.clear(s.waiting[wave]);
+    for (int u = 0; u < loads; ++u) {
+        Raw<T, V> once_more;
+        load(once_more, u, threadIdx.x);
+        const bool there = place(u, threadIdx.x) < vectors;
+        float v[V], most_of = none;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            v[j] = there ? once_more.get(j) : none;
+            most_of = fmaxf(most_of, v[j]);
+        }
+        run.batch(most_of, top, lane);
+        run.take(v, most_of, there, static_cast<uint32_t>(place(u, threadIdx.x) * V), top, lane);
+    }
+    run.next_batch(top);
+    run.take(one, rest_v, has_rest, static_cast<uint32_t>(rest_at), top, lane);
+    run.finish(top, lane);
+    __syncthreads();
+    s.waiting[wave][lane] = run.best.mine;
     __syncthreads();
     if (wave != 0) return;
-    if constexpr (!ONE) {
-        if (!sorted) take_candidates(best, s_candidates, s_candidates.count, top, lane);
-    }
-    float most = r.m;
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-        most = fmaxf(most, s_part[w].m);
-        if (!ONE && sorted) best.mine = merge_waves(best.mine, s_best[w][lane], lane);
-    }
-    r.raise(most, s_powers);
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-        WideStats o = {s_part[w].m, s_part[w].s};
-        o.raise(most, s_powers);
-        r.s += o.s;
-    }
-    BeamPart* const parts = static_cast<BeamPart*>(p.workspace);
-    if (lane == 0) parts[blockIdx.x] = {r.m, 0.0f, r.s};
-    if (lane < top) reinterpret_cast<Entry*>(parts + static_cast<int64_t>(p.batch) * p.beams * segments)[static_cast<int64_t>(blockIdx.x) * top + lane] = best.mine;
+    Entry best = run.best.mine;
+    for (int w = 1; w < W; ++w) best = merge_waves(best, s.waiting[w][lane], lane);
+    if (lane < top) out[lane] = best;
 }
 
 // An offer: larger scores first, of equal ones the lower beam, then the place in the beam's own order.  0: none.
 struct Offer {
     uint64_t key;          // of the score in 64 bits
-    uint32_t at;           // ~(beam * 64 + place)
+    uint32_t at;           // ~ of its place among the entries of the beams, a beam's behind those of the one before
     __device__ __forceinline__ bool operator>(const Offer& o) const { return key > o.key || (key == o.key && at > o.at); }
 };
 template <int MASK>
@@ -237,75 +306,188 @@ __device__ __forceinline__ uint64_t key_of_score(double v) {
 }
 __device__ __forceinline__ double score_of_key(uint64_t key) { return __builtin_bit_cast(double, key & 0x8000000000000000u ? key ^ 0x8000000000000000u : ~key); }
 
-// An entry of the batch: its beams are shared out among the waves.
-__global__ __launch_bounds__(64 * kWaves) void beam_join_kernel(QaBeamSearchParams p, int top, int segments) {
+// A bound that `count` of the workgroup's keys or more reach, one a lane (0: none), each of another offer: the count-th largest of groups of four lanes (of lanes, where
+// they are few).  0 where there are fewer groups with a key.
+__device__ __forceinline__ uint64_t bound_of_keys(uint64_t mine, int lanes, int count, uint64_t* keys, uint64_t* found, int lane) {
+    const int by = lanes <= 64 || count > 32 ? 1 : 4, groups = (lanes + by - 1) / by;
+    if (by == 4) {
+        const uint64_t pair = lm::across<1>(mine, lane);
+        mine = pair > mine ? pair : mine;
+        const uint64_t four = lm::across<2>(mine, lane);
+        mine = four > mine ? four : mine;
+    }
+    if (static_cast<int>(threadIdx.x) % by == 0) keys[threadIdx.x / by] = mine;
+    if (threadIdx.x == 0) *found = 0;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < groups) {
+        const uint64_t own = keys[threadIdx.x];
+        const Above a = above(keys, groups, own);
+        if (own != 0 && a.larger < count && count <= a.larger + a.equal) *found = own;             // (equal ones write the same)
+    }
+    __syncthreads();
+    return *found;
+}
+
+// An entry of the batch.  The lanes are shared out among the beams and join their segments' sums.  Of each segment's list the first entry alone says whether any of it
+// counts: a bound that `count` firsts reach leaves about as many lists, and a second bound over their entries about as many offers.  Those are ranked, each
+// counting the others that are larger.  (Sorting all entries, 64 at a time, took 8 us for 4 beams of 25 segments and 26 us for 5 of 64.)  Where more reach the
+// bounds than there is room for - equal scores, or as many places as lanes - each wave sorts what its lanes have.
+constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kOffers = 256;
+__global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchParams p, int top, int segments) {
     static_assert(kMaxSegments <= 64 && kMaxTop <= 64, "a lane for each");
-    __shared__ Offer s_offers[kWaves][64];
-    __shared__ uint32_t s_tokens[kMaxBeams][64];
-    __shared__ double s_powers[64];
+    __shared__ double s_rest[kMaxBeams], s_base[kMaxBeams];        // of a beam: own score - ln s, -inf: it offers nothing; m + e ln 2
+    __shared__ uint8_t s_done[kMaxBeams];
+    __shared__ __attribute__((aligned(16))) uint64_t s_keys[kOffers + 8];
+    __shared__ uint32_t s_at[kOffers], s_token[kOffers];
+    __shared__ uint16_t s_lists[kMaxBeams * kMaxSegments];
+    __shared__ Offer s_sorted[kJoinWaves][64];
+    __shared__ uint64_t s_bound;
+    __shared__ int s_count, s_further;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t entry = blockIdx.x;
-    const BeamPart* const parts = static_cast<const BeamPart*>(p.workspace);
-    const Entry* const entries = reinterpret_cast<const Entry*>(parts + static_cast<int64_t>(p.batch) * p.beams * segments);
-    fill_powers(s_powers);
-    __syncthreads();
-    Offer best = {0, 0};
-    for (int beam = wave; beam < p.beams; beam += kWaves) {
-        const int64_t row = entry * p.beams + beam;
+    const BeamPart* const parts = static_cast<const BeamPart*>(p.workspace) + entry * p.beams * segments;
+    const Entry* const entries = reinterpret_cast<const Entry*>(static_cast<const BeamPart*>(p.workspace) + static_cast<int64_t>(p.batch) * p.beams * segments) +
+                                 entry * p.beams * segments * top;
+    const int lists = p.beams * segments;
+    const Entry mine_first = static_cast<int>(threadIdx.x) < lists ? entries[threadIdx.x * top] : 0;    // (on its way meanwhile)
+    if (threadIdx.x == 0) s_count = s_further = 0;
+    if (threadIdx.x < 8) s_keys[kOffers + threadIdx.x] = 0;
+    {
+        // a power of two of lanes for each beam
+        const int share = kJoinThreads >> (32 - __builtin_clz(max(p.beams, 4) - 1)), beam = threadIdx.x / share, part = threadIdx.x % share;
+        // (all of it on its way at the same time, also what a beam that is done does not need)
+        const bool there = beam < p.beams;
+        const int64_t row = entry * p.beams + (there ? beam : 0);
         const double own = p.scores[row];
-        Offer mine = {0, 0};
-        if (!(own > -__builtin_inf() && own < __builtin_inf())) continue;
-        if (p.done && p.done[row]) {
-            if (lane == 0) mine = {key_of_score(own), ~static_cast<uint32_t>(beam * 64)};
-            s_tokens[beam][lane] = 0xffffffffu;
-        } else {
-            WideStats r;
-            r.clear();
-            if (lane < segments) r = {parts[row * segments + lane].m, parts[row * segments + lane].s};
-            Entry list = 0;
-            const Entry* const from = entries + row * segments * top;
-            if (top >= 16) {
-                for (int i = 0; i < segments; ++i) list = merge_waves(list, lane < top ? from[i * top + lane] : Entry(0), lane);
-            } else {
-                for (int i = 0; i < segments * top; i += 64) list = merge_waves(list, sort_wave(i + lane < segments * top ? from[i + lane] : Entry(0), lane), lane);
-            }
-            r = wave_stats(r, s_powers, lane);
-            const float logit = value_of(list);
-            if (r.s > 0.0 && list != 0 && logit > -__builtin_inff() && lane < top)
-                mine = {key_of_score(own + (static_cast<double>(logit) - r.m - log(r.s))), ~static_cast<uint32_t>(beam * 64 + lane)};
-            s_tokens[beam][lane] = index_of(list);
+        const uint8_t end_reached = p.done ? p.done[row] : 0;
+        BeamPart r = {0.0f, 0, 0.0};
+        if (there && part < segments) r = parts[beam * segments + part];
+        const bool done = end_reached != 0;
+        for (int i = part + share; there && i < segments; i += share) r = joined(r, parts[beam * segments + i]);
+        for (int mask = 1; mask < share; mask *= 2) {
+            const auto word = [&](int w) { return __builtin_amdgcn_ds_bpermute((lane ^ mask) * 4, w); };
+            const BeamPart other = {__int_as_float(word(__float_as_int(r.m))), word(r.e), lane_double(r.s, lane ^ mask)};
+            r = joined(r, other);
         }
-        best = merge_waves(best, mine, lane);
+        if (there && part == 0) {
+            const bool offers = own > -__builtin_inf() && own < __builtin_inf() && (done || r.s > 0.0);
+            s_rest[beam] = !offers ? -__builtin_inf() : done ? own : own - log(r.s);
+            s_base[beam] = done ? 0.0 : r.m + r.e * kLn2Wide;
+            s_done[beam] = done;
+        }
     }
-    s_offers[wave][lane] = best;
+    __syncthreads();
+    // the key of the score of a list's entry; 0: no offer
+    auto key_at = [&](int list, int place, Entry e) -> uint64_t {
+        const int beam = list / segments;
+        const double rest = s_rest[beam];
+        if (!(rest > -__builtin_inf())) return 0;
+        if (s_done[beam]) return place == 0 && list == beam * segments ? key_of_score(rest) : 0;
+        const float logit = value_of(e);
+        // (the difference first: next to a mask of -3e38 nothing else is left of the sum)
+        return e != 0 && logit > -__builtin_inff() ? key_of_score(rest + (static_cast<double>(logit) - s_base[beam])) : 0;
+    };
+    auto each_list = [&](auto&& f) __attribute__((always_inline)) {
+        for (int list = threadIdx.x; list < lists; list += kJoinThreads) {
+            const Entry e = list < kJoinThreads ? mine_first : entries[list * top];
+            if (const uint64_t key = key_at(list, 0, e)) f(list, key);
+        }
+    };
+    uint64_t best_key = 0;
+    each_list([&](int, uint64_t key) { best_key = key > best_key ? key : best_key; });
+    uint64_t bound = bound_of_keys(best_key, min(lists, kJoinThreads), p.count, s_keys, &s_bound, lane);
+    each_list([&](int list, uint64_t key) {
+        if (key >= bound) s_lists[atomicAdd(&s_further, 1)] = static_cast<uint16_t>(list);
+    });
+    __syncthreads();
+    const int items = s_further * top;
+    auto each_item = [&](auto&& f) __attribute__((always_inline)) {
+        for (int i = threadIdx.x; i < items; i += kJoinThreads) {
+            const int list = s_lists[i / top], at = list * top + i % top;
+            const Entry e = entries[at];
+            const uint64_t key = key_at(list, i % top, e);
+            if (key != 0 && key >= bound) f(at, key, e);
+        }
+    };
+    if (items > 48) {
+        best_key = 0;
+        each_item([&](int, uint64_t key, Entry) { best_key = key > best_key ? key : best_key; });
+        const uint64_t closer = bound_of_keys(best_key, min(items, kJoinThreads), p.count, s_keys, &s_bound, lane);
+        bound = closer > bound ? closer : bound;
+        __syncthreads();
+    }
+    each_item([&](int at, uint64_t key, Entry e) {
+        const int place = atomicAdd(&s_count, 1);
+        if (place >= kOffers) return;
+        s_keys[place] = key;
+        s_at[place] = ~static_cast<uint32_t>(at);
+        s_token[place] = index_of(e);
+    });
+    __syncthreads();
+    const int offers = s_count;
+    if (offers < kOffers && threadIdx.x < 8) s_keys[offers + threadIdx.x] = 0;
+    __syncthreads();
+    const int64_t out = entry * p.count;
+    auto write = [&](int place, uint64_t key, uint32_t at, uint32_t token) {
+        const int beam = static_cast<int>(~at) / top / segments;
+        p.out_scores[out + place] = static_cast<float>(score_of_key(key));
+        p.tokens[out + place] = s_done[beam] ? -1 : static_cast<int64_t>(token);
+        p.parents[out + place] = beam;
+    };
+    auto leave = [&](int place) {
+        p.out_scores[out + place] = -__builtin_inff();
+        p.tokens[out + place] = -1;
+        p.parents[out + place] = -1;
+    };
+    if (offers <= kOffers) {
+        if (static_cast<int>(threadIdx.x) < offers) {
+            const uint64_t key = s_keys[threadIdx.x];
+            const uint32_t at = s_at[threadIdx.x];
+            const Above a = above(s_keys, offers, key);
+            int place = a.larger;
+            if (a.equal > 1)
+                for (int n = 0; n < offers; ++n) place += s_keys[n] == key && s_at[n] > at;
+            if (place < p.count) write(place, key, at, s_token[threadIdx.x]);
+        } else if (static_cast<int>(threadIdx.x) < p.count) {
+            leave(threadIdx.x);
+        }
+        return;
+    }
+    Offer best = {0, 0};
+    for (int i = wave * 64; i < items; i += kJoinThreads) {
+        Offer o = {0, 0};
+        if (i + lane < items) {
+            const int list = s_lists[(i + lane) / top], place = (i + lane) % top;
+            const uint64_t key = key_at(list, place, entries[list * top + place]);
+            if (key != 0) o = {key, ~static_cast<uint32_t>(list * top + place)};
+        }
+        if (__builtin_amdgcn_ballot_w64(o.key != 0 && o.key >= bound)) best = merge_waves(best, sort_wave(o, lane), lane);
+    }
+    s_sorted[wave][lane] = best;
     __syncthreads();
     if (wave != 0) return;
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) best = merge_waves(best, s_offers[w][lane], lane);
-    if (lane >= p.count) return;
-    const int64_t out = entry * p.count + lane;
-    const uint32_t at = ~best.at, beam = at / 64;
-    const bool there = best.key != 0;
-    p.out_scores[out] = there ? static_cast<float>(score_of_key(best.key)) : -__builtin_inff();
-    p.tokens[out] = there ? static_cast<int64_t>(static_cast<int32_t>(s_tokens[beam][at % 64])) : -1;
-    p.parents[out] = there ? static_cast<int64_t>(beam) : -1;
+    for (int w = 1; w < kJoinWaves; ++w) best = merge_waves(best, s_sorted[w][lane], lane);
+    if (lane < p.count) best.key != 0 ? write(lane, best.key, best.at, index_of(entries[~best.at])) : leave(lane);
 }
 
 int check(const QaBeamSearchParams& p) {
-    if (p.batch < 0 || p.beams < 1 || p.vocab < 1 || p.vocab > 1 << 30) return QA_ERR_SHAPE;
+    if (p.batch < 0 || p.beams < 1 || p.vocab < 1 || p.vocab > kMaxVocab) return QA_ERR_SHAPE;
     if (!is_float_type(p.logits_type) || p.beams > kMaxBeams || p.count < 1 || p.count > kMaxTop) return QA_ERR_UNSUPPORTED;
     if (p.count > static_cast<int64_t>(p.beams) * p.vocab || static_cast<int64_t>(p.batch) * p.beams > 0x7fffffffLL) return QA_ERR_SHAPE;
     return QA_OK;
 }
 int top_of(const QaBeamSearchParams& p) { return std::min(p.count, p.vocab); }
-// four waves a segment, however many rows there are
-Cut beams_cut(const QaBeamSearchParams& p) {
-    Cut cut = cut_of(p.batch * p.beams, p.vocab, p.logits_type);
-    if (cut.waves == 1) {
-        const int load = kWaves * 64 * (p.logits_type == QA_LM_F32 ? 4 : 8) * kUnroll;
-        cut = {kWaves, 1, (p.vocab + load - 1) / load, kUnroll};
-    }
-    return cut;
+// How a row is cut: segments, chunks of a segment.  Four workgroups for each CU where the rows are few.
+struct BeamsCut {
+    int segments, each;
+};
+BeamsCut beams_cut(const QaBeamSearchParams& p) {
+    const int chunk = kWaves * 64 * (p.logits_type == QA_LM_F32 ? 4 : 8), chunks = (p.vocab + chunk - 1) / chunk;
+    static_assert(kMaxVocab / (kWaves * 64 * 4) <= kMaxSegments * kMaxLoads, "a place for every chunk");
+    const int64_t rows = static_cast<int64_t>(p.batch) * p.beams;
+    const int wanted = static_cast<int>(std::min<int64_t>((4LL * compute_units() + rows - 1) / rows, kMaxSegments));
+    const int each = std::min(kMaxLoads, (chunks + std::min(chunks, wanted) - 1) / std::min(chunks, wanted));
+    return {(chunks + each - 1) / each, each};
 }
 int64_t workspace_bytes(const QaBeamSearchParams& p) {
     return static_cast<int64_t>(p.batch) * p.beams * beams_cut(p).segments * (static_cast<int64_t>(sizeof(BeamPart)) + top_of(p) * static_cast<int64_t>(sizeof(Entry)));
@@ -313,23 +495,17 @@ int64_t workspace_bytes(const QaBeamSearchParams& p) {
 
 template <class T>
 int launch(const QaBeamSearchParams& p, hipStream_t stream) {
-    const Cut cut = beams_cut(p);
+    const BeamsCut cut = beams_cut(p);
     const int top = top_of(p);
     auto whole = [&](int64_t stride, int n) { return n == 1 || stride * static_cast<int64_t>(sizeof(T)) % 16 == 0; };
     const bool wide = aligned16(p.logits) && whole(p.logits_batch_stride, p.batch) && whole(p.logits_beam_stride, p.beams);
     const int64_t workgroups = static_cast<int64_t>(p.batch) * p.beams * cut.segments;
     if (!launchable(workgroups, 64 * kWaves)) return QA_ERR_SHAPE;
     const dim3 grid(static_cast<unsigned>(workgroups)), block(64 * kWaves);
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, top, cut.segments, cut.batches); };
-    auto of_wide = [&](auto wide_c) {
-        constexpr bool WIDE = decltype(wide_c)::value;
-        if (cut.loads == 1) go(beam_rows_kernel<T, WIDE, true, 1>);
-        else if (cut.batches == 1) go(beam_rows_kernel<T, WIDE, true, kUnroll>);
-        else go(beam_rows_kernel<T, WIDE, false, kUnroll>);
-    };
-    wide ? of_wide(std::true_type{}) : of_wide(std::false_type{});
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, top, cut.segments, cut.each); };
+    wide ? go(beam_rows_kernel<T, true>) : go(beam_rows_kernel<T, false>);
     if (const int status = check_launch()) return status;
-    hipLaunchKernelGGL(beam_join_kernel, dim3(p.batch), block, 0, stream, p, top, cut.segments);
+    hipLaunchKernelGGL(beam_join_kernel, dim3(p.batch), dim3(kJoinThreads), 0, stream, p, top, cut.segments);
     return check_launch();
 }
 

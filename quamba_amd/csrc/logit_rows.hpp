@@ -32,7 +32,7 @@ Cut cut_of(int rows, int vocab, int type) {
 }
 
 struct Candidates {
-    Entry at[kCandidates];
+    alignas(16) Entry at[kCandidates];
     uint32_t keys[kWaves][64];
     int count;
 };
@@ -42,12 +42,9 @@ __device__ __forceinline__ void take_candidates(BestEntries& best, const Candida
     for (int i = 0; i < count; i += 64) best.offer(i + lane < count ? c.at[i + lane] : 0, top, lane);
 }
 
-// The best `top` of the workgroup's values: `visit(f)` calls f(values, the largest of them, whether they are there, index) for each load of a
-// lane, `most` is the largest of all.  What the lanes' largest values say is a bound that `top` values or more reach and hardly more than
-// that do: those are put together in LDS (in any order) and one wave sorts them.  Where more come than there is room for - equal values,
-// or as many alternatives as lanes - every wave keeps its own best instead and one wave merges them.  The result is wave 0's.
-template <int V, class Visit>
-__device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, Candidates& c, Entry (&lists)[kWaves][64], Entry* waiting, int wave, int lane) {
+// A bound that `top` of the workgroup's values or more reach and hardly more than that do, from what its lanes' largest values are (at least `top` of them are there,
+// -inf ones among them).  Clears the count of candidates.
+__device__ __forceinline__ float bound_of_lanes(float most, int top, Candidates& c, int wave, int lane) {
     if (threadIdx.x == 0) c.count = 0;
     c.keys[wave][lane] = sort_wave(key_of(most), lane);
     __syncthreads();
@@ -68,7 +65,15 @@ __device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, 
         const uint32_t all = merge_waves(merge_waves(c.keys[0][lane], c.keys[1][lane], lane), merge_waves(c.keys[2][lane], c.keys[3][lane], lane), lane);
         reached = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(all), top - 1));
     }
-    const float bound = value_of_key(reached);
+    return value_of_key(reached);
+}
+
+// The best `top` of the workgroup's values: `visit(f)` calls f(values, the largest of them, whether they are there, index) for each load of a
+// lane, `most` is the largest of all.  Those that reach the bound are put together in LDS (in any order) and one wave sorts them.  Where more come
+// than there is room for - equal values, or as many alternatives as lanes - every wave keeps its own best instead and one wave merges them.  The result is wave 0's.
+template <int V, class Visit>
+__device__ __forceinline__ BestEntries pick(Visit&& visit, float most, int top, Candidates& c, Entry (&lists)[kWaves][64], Entry* waiting, int wave, int lane) {
+    const float bound = bound_of_lanes(most, top, c, wave, lane);
     visit([&](const auto& v, float most_of, bool valid, uint32_t index) __attribute__((always_inline)) {
         if (!__builtin_amdgcn_ballot_w64(valid && most_of >= bound)) return;
         constexpr int N = sizeof(v) / sizeof(v[0]);

@@ -216,7 +216,7 @@ PyObject* beam_search_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         require(beams >= 1 && vocab >= 1, "logits without beams or a vocabulary");
         require(batch <= kMost && vocab <= kMost, "beam_search_step: a size beyond 32 bits");
         require(vocab == 1 || logits.stride(2) == 1, "logits must be contiguous along the last dimension");
-        supported(beams <= 64, "beam_search_step: up to 64 beams");
+        supported(beams <= 64 && vocab <= 1 << 20, "beam_search_step: up to 64 beams and 2^20 tokens");
         require(count >= 1 && count <= beams * vocab, "count must be between 1 and what the beams offer");
         supported(count <= 64, "beam_search_step: count up to 64");
         beside(scores, "scores", device);

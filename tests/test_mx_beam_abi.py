@@ -129,7 +129,7 @@ def test_beam_refusals():
     p.workspace_bytes = need = l.qa_beam_search_workspace_bytes(C.byref(p))
     assert need > 0
     _codes(l.qa_beam_search_step, p, [
-        (dict(batch=-1), -2), (dict(beams=0), -2), (dict(beams=65), -4), (dict(vocab=0), -2), (dict(vocab=(1 << 30) + 1), -2), (dict(count=0), -4), (dict(count=65), -4),
+        (dict(batch=-1), -2), (dict(beams=0), -2), (dict(beams=65), -4), (dict(vocab=0), -2), (dict(vocab=(1 << 20) + 1), -2), (dict(count=0), -4), (dict(count=65), -4),
         (dict(vocab=1, count=5), -2), (dict(logits_type=0), -4), (dict(logits_type=4), -4), (dict(logits=0), -1), (dict(scores=0), -1), (dict(out_scores=0), -1),
         (dict(tokens=0), -1), (dict(parents=0), -1), (dict(logits=AT + 1), -3), (dict(logits_type=3, logits=AT + 2), -3), (dict(scores=AT + 2), -3),
         (dict(logits_beam_stride=-1), -3), (dict(logits_batch_stride=-1), -3), (dict(workspace=0), -1), (dict(workspace=AT + 8), -6), (dict(workspace_bytes=need - 1), -6),

@@ -1,8 +1,12 @@
 // Rows of states in another order, in place (qa_reorder_states).
 //
-// A thread has one unit of 16 bytes (4 or 1 where a state does not lie on that) of all the rows of an entry: it reads what its rows are to become and then writes them, so
+// A thread has two units of 16 bytes (4 or 1 where a state does not lie on that) of all the rows of an entry: it reads what its rows are to become and then writes them, so
 // that no row is read after it was written and no copy is needed.  Rows that stay are neither read nor written, and a parent of several
-// rows comes from memory once and from the caches again.  Bound by memory.  One launch has up to kTensors tensors, with their addresses in its arguments.
+// rows comes from memory once and from the caches again.  One launch has up to kTensors tensors, with their addresses in its arguments.
+//
+// Bound by memory: 16 rows of 64 layers of 5120 x 16 fp32 states and their conv states, 479 MB of them read or written, take 81 us, 5.9 TB/s (one unit a thread 84).  States
+// that the last-level cache does not hold are written past it (89 us otherwise); those that it holds are read again soon (2 x 16 rows of 32 layers, 151 MB, 37 us, and 46
+// past it).
 #include "../../include/quamba_amd_beam.h"
 #include "lm_common.hpp"
 
@@ -23,19 +27,35 @@ struct Tensors {
 };
 static_assert(sizeof(Tensors) < 3072, "arguments of a launch");
 
-template <int BEAMS, class U>
-__device__ __forceinline__ void move_unit(uint8_t* base, int64_t row_stride, const int (&from)[BEAMS], int beams) {
-    U v[BEAMS];
+// units of a thread, as far as the registers go
+template <int BEAMS>
+constexpr int kUnits = BEAMS <= 16 ? 2 : 1;
+
+// left: units of the row from this thread's first one on
+template <int BEAMS, bool PAST, class U>
+__device__ __forceinline__ void move_units(uint8_t* base, int64_t row_stride, const int (&from)[BEAMS], int beams, int left) {
+    constexpr int N = kUnits<BEAMS>;
+    U v[BEAMS][N];
 #pragma unroll
     for (int i = 0; i < BEAMS; ++i)
-        if (i < beams && from[i] != i) v[i] = *reinterpret_cast<const U*>(base + from[i] * row_stride);
+        if (i < beams && from[i] != i)
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (k * kThreads < left) v[i][k] = reinterpret_cast<const U*>(base + from[i] * row_stride)[k * kThreads];
 #pragma unroll
     for (int i = 0; i < BEAMS; ++i)
-        if (i < beams && from[i] != i) *reinterpret_cast<U*>(base + i * row_stride) = v[i];
+        if (i < beams && from[i] != i)
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (k * kThreads < left) {
+                    U* const to = reinterpret_cast<U*>(base + i * row_stride) + k * kThreads;
+                    if constexpr (PAST) __builtin_nontemporal_store(v[i][k], to);
+                    else *to = v[i][k];
+                }
 }
 
-// UNIT: bytes; BEAMS: at least as many as there are
-template <int BEAMS, int UNIT>
+// UNIT: bytes; BEAMS: at least as many as there are; PAST: written past the last-level cache
+template <int BEAMS, int UNIT, bool PAST>
 __global__ __launch_bounds__(kThreads) void reorder_kernel(Tensors t, const void* parents, int index_bytes, int beams) {
     const int64_t entry = blockIdx.y;
     int from[BEAMS], moved = 0;
@@ -54,27 +74,24 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(Tensors t, const void
         if (t.first[middle] <= static_cast<int>(blockIdx.x)) low = middle;
         else high = middle - 1;
     }
-    const int unit = (static_cast<int>(blockIdx.x) - t.first[low]) * kThreads + threadIdx.x;
+    const int unit = (static_cast<int>(blockIdx.x) - t.first[low]) * (kThreads * kUnits<BEAMS>) + threadIdx.x;
     if (unit >= t.units[low]) return;
     using U = std::conditional_t<UNIT == 16, v4w, std::conditional_t<UNIT == 4, uint32_t, uint8_t>>;
-    move_unit<BEAMS, U>(t.data[low] + entry * beams * t.row_stride[low] + static_cast<int64_t>(unit) * UNIT, t.row_stride[low], from, beams);
+    move_units<BEAMS, PAST, U>(t.data[low] + entry * beams * t.row_stride[low] + static_cast<int64_t>(unit) * UNIT, t.row_stride[low], from, beams, t.units[low] - unit);
 }
 
-template <int UNIT>
-int launch(const QaReorderParams& p, const Tensors& t, hipStream_t stream) {
+template <int BEAMS, int UNIT>
+int launch(const QaReorderParams& p, const Tensors& t, bool past, hipStream_t stream) {
     const dim3 grid(t.first[t.count], p.batch);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, t, p.parents, p.index_bytes, p.beams); };
-    if (p.beams <= 4) go(reorder_kernel<4, UNIT>);
-    else if (p.beams <= 8) go(reorder_kernel<8, UNIT>);
-    else if (p.beams <= 16) go(reorder_kernel<16, UNIT>);
-    else if (p.beams <= 32) go(reorder_kernel<32, UNIT>);
-    else go(reorder_kernel<64, UNIT>);
+    past ? go(reorder_kernel<BEAMS, UNIT, true>) : go(reorder_kernel<BEAMS, UNIT, false>);
     return check_launch();
 }
 
-int unit_of(const QaStateRows& s) {
+// (more than 32 beams by 16 bytes are more than the registers of two waves)
+int unit_of(const QaStateRows& s, int beams) {
     const uint64_t all = reinterpret_cast<uintptr_t>(s.data) | static_cast<uint64_t>(s.row_bytes) | static_cast<uint64_t>(s.row_stride);
-    return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+    return all % 16 == 0 && beams <= 32 ? 16 : all % 4 == 0 ? 4 : 1;
 }
 
 }  // namespace
@@ -97,22 +114,26 @@ extern "C" int qa_reorder_states(const QaReorderParams* p, void* stream_) {
         if (s.row_bytes == 0) continue;
         if (!s.data) return QA_ERR_NULL;
         if (s.row_stride < s.row_bytes && static_cast<int64_t>(p->batch) * p->beams > 1) return QA_ERR_STRIDE;
-        const int64_t units = s.row_bytes / unit_of(s);
+        const int64_t units = s.row_bytes / unit_of(s, p->beams);
         if (units > 0x7fffffffLL || !launchable((units + kThreads - 1) / kThreads * p->batch, kThreads)) return QA_ERR_SHAPE;
     }
     if (p->beams == 1) return QA_OK;
-    auto all_of = [&](auto unit_c) {
-        constexpr int UNIT = decltype(unit_c)::value;
+    constexpr int64_t kCached = 224LL << 20;
+    int64_t bytes = 0;
+    for (int i = 0; i < p->tensors; ++i) bytes += p->states[i].row_bytes * p->batch * p->beams;
+    const bool past = bytes >= kCached;
+    auto all_of = [&](auto beams_c, auto unit_c) {
+        constexpr int BEAMS = decltype(beams_c)::value, UNIT = decltype(unit_c)::value, kEach = kThreads * kUnits<BEAMS>;
         Tensors t = {};
         auto flush = [&] {
-            const int status = t.count ? launch<UNIT>(*p, t, static_cast<hipStream_t>(stream_)) : QA_OK;
+            const int status = t.count ? launch<BEAMS, UNIT>(*p, t, past, static_cast<hipStream_t>(stream_)) : QA_OK;
             t.count = 0;
             return status;
         };
         for (int i = 0; i < p->tensors; ++i) {
             const QaStateRows& s = p->states[i];
-            if (s.row_bytes == 0 || unit_of(s) != UNIT) continue;
-            const int64_t units = s.row_bytes / UNIT, workgroups = (units + kThreads - 1) / kThreads;
+            if (s.row_bytes == 0 || unit_of(s, p->beams) != UNIT) continue;
+            const int64_t units = s.row_bytes / UNIT, workgroups = (units + kEach - 1) / kEach;
             if (t.count == kTensors || !launchable((t.first[t.count] + workgroups) * p->batch, kThreads))
                 if (const int status = flush()) return status;
             t.data[t.count] = static_cast<uint8_t*>(s.data);
@@ -123,7 +144,15 @@ extern "C" int qa_reorder_states(const QaReorderParams* p, void* stream_) {
         }
         return flush();
     };
-    if (const int status = all_of(std::integral_constant<int, 16>{})) return status;
-    if (const int status = all_of(std::integral_constant<int, 4>{})) return status;
-    return all_of(std::integral_constant<int, 1>{});
+    auto of_beams = [&](auto beams_c) {
+        if constexpr (decltype(beams_c)::value <= 32)
+            if (const int status = all_of(beams_c, std::integral_constant<int, 16>{})) return status;
+        if (const int status = all_of(beams_c, std::integral_constant<int, 4>{})) return status;
+        return all_of(beams_c, std::integral_constant<int, 1>{});
+    };
+    if (p->beams <= 4) return of_beams(std::integral_constant<int, 4>{});
+    if (p->beams <= 8) return of_beams(std::integral_constant<int, 8>{});
+    if (p->beams <= 16) return of_beams(std::integral_constant<int, 16>{});
+    if (p->beams <= 32) return of_beams(std::integral_constant<int, 32>{});
+    return of_beams(std::integral_constant<int, 64>{});
 }

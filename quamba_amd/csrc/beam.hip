@@ -28,6 +28,7 @@ struct BeamPart {
 constexpr float kReach = 600.0f;
 constexpr int kSteps = 512;
 constexpr double kLn2Wide = 0.69314718055994531;
+constexpr int kNowhere = 1 << 29;          // below it there is no e of a sum
 struct WideSum {
     float m;
     int e;
@@ -114,16 +115,20 @@ __device__ __forceinline__ BeamPart joined(BeamPart a, BeamPart b) {
     return {a.m, a.e, a.s + b.s * exp(fmax(apart, -700.0))};
 }
 
-__device__ __forceinline__ double lane_double(double v, int from) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(from * 4, static_cast<int>(static_cast<uint32_t>(u))));
-    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(from * 4, static_cast<int>(u >> 32)));
-    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+template <int MASK>
+__device__ __forceinline__ double across(double v, int lane) { return __builtin_bit_cast(double, lm::across<MASK>(__builtin_bit_cast(uint64_t, v), lane)); }
+// f(1), f(2), f(4) .. below `end`, each a constant of its own
+template <int MASK = 1, class F>
+__device__ __forceinline__ void each_mask(int end, F&& f) {
+    if constexpr (MASK < 64) {
+        if (MASK >= end) return;
+        f(std::integral_constant<int, MASK>{});
+        each_mask<2 * MASK>(end, f);
+    }
 }
 // over the wave, in every lane: the order of the sum is that of the lanes' numbers' bits, the same in all of them
 __device__ __forceinline__ double wave_sum(double s, int lane) {
-#pragma unroll
-    for (int mask = 1; mask < 64; mask *= 2) s += lane_double(s, lane ^ mask);
+    each_mask(64, [&](auto mask) { s += across<decltype(mask)::value>(s, lane); });
     return s;
 }
 
@@ -153,8 +158,8 @@ __device__ __forceinline__ Above above(const uint64_t* keys, int n, uint64_t own
 
 // A workgroup has a segment of up to kMaxLoads chunks, one load a lane each; kAhead of them are under way while one is summed.  What each load's largest value is goes to LDS, and
 // when all were seen a bound says which loads have one of the best entries: those are read once more, all at the same time, and what reaches the bound is ranked (each
-// counts the others that are larger).  A short loop: with four loads a batch and the entries kept on the way, as token_logprobs has them, the code was
-// larger than the instruction cache and 64 x 8 rows of 50280 took 35 us.
+// counts the others that are larger).  (64 x 8 rows of 50280 bf16, count 16: 26 us, of which the loop without exponentials 12.4, the exponentials 9 and the
+// selection 6; with the entries kept on the way, as token_logprobs has them, 35.  Four or six loads ahead, the loop unrolled over them or more segments: the same.)
 constexpr int kAhead = 3;
 
 template <class T, bool WIDE>
@@ -306,42 +311,36 @@ __device__ __forceinline__ uint64_t key_of_score(double v) {
 }
 __device__ __forceinline__ double score_of_key(uint64_t key) { return __builtin_bit_cast(double, key & 0x8000000000000000u ? key ^ 0x8000000000000000u : ~key); }
 
-// A bound that `count` of the workgroup's keys or more reach, one a lane (0: none), each of another offer: the count-th largest of groups of four lanes (of lanes, where
-// they are few).  0 where there are fewer groups with a key.
-__device__ __forceinline__ uint64_t bound_of_keys(uint64_t mine, int lanes, int count, uint64_t* keys, uint64_t* found, int lane) {
-    const int by = lanes <= 64 || count > 32 ? 1 : 4, groups = (lanes + by - 1) / by;
-    if (by == 4) {
-        const uint64_t pair = lm::across<1>(mine, lane);
-        mine = pair > mine ? pair : mine;
-        const uint64_t four = lm::across<2>(mine, lane);
-        mine = four > mine ? four : mine;
-    }
-    if (static_cast<int>(threadIdx.x) % by == 0) keys[threadIdx.x / by] = mine;
-    if (threadIdx.x == 0) *found = 0;
+// A bound that `count` of the workgroup's keys or more reach, one a lane (0: none): the count-th largest of their upper halves, by sorts of words.  0 where
+// fewer lanes have a key.
+template <int WAVES>
+__device__ __forceinline__ uint64_t bound_of_keys(uint64_t mine, int count, uint32_t (&keys)[WAVES][64], int wave, int lane) {
+    static_assert(WAVES == 4, "two pairs");
+    keys[wave][lane] = sort_wave(static_cast<uint32_t>(mine >> 32), lane);
     __syncthreads();
-    if (static_cast<int>(threadIdx.x) < groups) {
-        const uint64_t own = keys[threadIdx.x];
-        const Above a = above(keys, groups, own);
-        if (own != 0 && a.larger < count && count <= a.larger + a.equal) *found = own;             // (equal ones write the same)
-    }
-    __syncthreads();
-    return *found;
+    const uint32_t all = merge_waves(merge_waves(keys[0][lane], keys[1][lane], lane), merge_waves(keys[2][lane], keys[3][lane], lane), lane);
+    return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(all), count - 1))) << 32;
 }
 
-// An entry of the batch.  The lanes are shared out among the beams and join their segments' sums.  Of each segment's list the first entry alone says whether any of it
-// counts: a bound that `count` firsts reach leaves about as many lists, and a second bound over their entries about as many offers.  Those are ranked, each
-// counting the others that are larger.  (Sorting all entries, 64 at a time, took 8 us for 4 beams of 25 segments and 26 us for 5 of 64.)  Where more reach the
-// bounds than there is room for - equal scores, or as many places as lanes - each wave sorts what its lanes have.
-constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kOffers = 256;
+// An entry of the batch.  The lanes are shared out among the beams and join their segments' sums; meanwhile the lists are on their way.  Up to kKept entries, four a lane,
+// get their scores' keys at once: a bound, the `count`-th largest of what the lanes have best, leaves about as many offers, and those are ranked, each counting the
+// others that are larger.  Of more than that the first entry of each list alone says whether any of it counts: a bound that `count` firsts reach leaves
+// about as many lists, and a second one over their entries about as many offers.  (us of this launch for 4 beams of 25 segments, count 8, and 5 of 63, count 10: 5.6 and
+// 9.0; lists first for both 7.6 and 9.3, all entries first, 13 a lane, 10.5 for the second; all entries sorted, 64 at a time, 8 and 26.)  What is left are some ten
+// waits, for memory and for LDS, one after the other.  Where more reach the bounds than there is room for - equal scores, or as many places as lanes - each
+// wave sorts what its lanes have.
+constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kOffers = 256, kFew = 48, kEach = 4, kKept = kEach * kJoinThreads;
 __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchParams p, int top, int segments) {
     static_assert(kMaxSegments <= 64 && kMaxTop <= 64, "a lane for each");
     __shared__ double s_rest[kMaxBeams], s_base[kMaxBeams];        // of a beam: own score - ln s, -inf: it offers nothing; m + e ln 2
-    __shared__ uint8_t s_done[kMaxBeams];
+    __shared__ uint8_t s_done[kMaxBeams], s_beam[kOffers];
     __shared__ __attribute__((aligned(16))) uint64_t s_keys[kOffers + 8];
     __shared__ uint32_t s_at[kOffers], s_token[kOffers];
+    __shared__ uint64_t s_item_keys[kKept];                // in the order of the lanes
+    __shared__ uint32_t s_item_tokens[kKept];
     __shared__ uint16_t s_lists[kMaxBeams * kMaxSegments];
     __shared__ Offer s_sorted[kJoinWaves][64];
-    __shared__ uint64_t s_bound;
+    __shared__ uint32_t s_bounds[kJoinWaves][64];
     __shared__ int s_count, s_further;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t entry = blockIdx.x;
@@ -349,7 +348,15 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
     const Entry* const entries = reinterpret_cast<const Entry*>(static_cast<const BeamPart*>(p.workspace) + static_cast<int64_t>(p.batch) * p.beams * segments) +
                                  entry * p.beams * segments * top;
     const int lists = p.beams * segments;
-    const Entry mine_first = static_cast<int>(threadIdx.x) < lists ? entries[threadIdx.x * top] : 0;    // (on its way meanwhile)
+    const int all = lists * top;
+    const bool kept = all <= kKept;
+    // this lane's entries: four lanes next to each other have them far apart, so that what a list begins with is in groups of its own
+    auto item_of = [&](int j) { return static_cast<int>(j * kJoinThreads + (threadIdx.x & 3) * (kJoinThreads / 4) + (threadIdx.x >> 2)); };
+    Entry mine[kEach];                                     // (on their way meanwhile)
+    if (kept) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) mine[i] = entries[min(item_of(i), all - 1)];
+    }
     if (threadIdx.x == 0) s_count = s_further = 0;
     if (threadIdx.x < 8) s_keys[kOffers + threadIdx.x] = 0;
     {
@@ -360,14 +367,25 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
         const int64_t row = entry * p.beams + (there ? beam : 0);
         const double own = p.scores[row];
         const uint8_t end_reached = p.done ? p.done[row] : 0;
-        BeamPart r = {0.0f, 0, 0.0};
+        BeamPart r = {0.0f, 0, 0.0}, second = r;
         if (there && part < segments) r = parts[beam * segments + part];
+        if (there && part + share < segments) second = parts[beam * segments + part + share];
         const bool done = end_reached != 0;
-        for (int i = part + share; there && i < segments; i += share) r = joined(r, parts[beam * segments + i]);
-        for (int mask = 1; mask < share; mask *= 2) {
-            const auto word = [&](int w) { return __builtin_amdgcn_ds_bpermute((lane ^ mask) * 4, w); };
-            const BeamPart other = {__int_as_float(word(__float_as_int(r.m))), word(r.e), lane_double(r.s, lane ^ mask)};
-            r = joined(r, other);
+        if (share < segments) r = joined(r, second);
+        for (int i = part + 2 * share; there && i < segments; i += share) r = joined(r, parts[beam * segments + i]);
+        if (__builtin_amdgcn_ballot_w64(r.m != 0.0f) == 0) {
+            // one place for all of them, then their sum
+            int e = r.s == 0.0 ? -kNowhere : r.e;
+            each_mask(share, [&](auto mask) { e = max(e, static_cast<int>(word_across<decltype(mask)::value>(static_cast<uint32_t>(e), lane))); });
+            r.s = ldexp(r.s, max((r.s == 0.0 ? e : r.e) - e, -2000));
+            r.e = e;
+            each_mask(share, [&](auto mask) { r.s += across<decltype(mask)::value>(r.s, lane); });
+        } else {
+            each_mask(share, [&](auto mask_c) {
+                constexpr int mask = decltype(mask_c)::value;
+                const BeamPart other = {__uint_as_float(word_across<mask>(__float_as_uint(r.m), lane)), static_cast<int>(word_across<mask>(static_cast<uint32_t>(r.e), lane)), across<mask>(r.s, lane)};
+                r = joined(r, other);
+            });
         }
         if (there && part == 0) {
             const bool offers = own > -__builtin_inf() && own < __builtin_inf() && (done || r.s > 0.0);
@@ -387,49 +405,85 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
         // (the difference first: next to a mask of -3e38 nothing else is left of the sum)
         return e != 0 && logit > -__builtin_inff() ? key_of_score(rest + (static_cast<double>(logit) - s_base[beam])) : 0;
     };
-    auto each_list = [&](auto&& f) __attribute__((always_inline)) {
-        for (int list = threadIdx.x; list < lists; list += kJoinThreads) {
-            const Entry e = list < kJoinThreads ? mine_first : entries[list * top];
-            if (const uint64_t key = key_at(list, 0, e)) f(list, key);
-        }
-    };
-    uint64_t best_key = 0;
-    each_list([&](int, uint64_t key) { best_key = key > best_key ? key : best_key; });
-    uint64_t bound = bound_of_keys(best_key, min(lists, kJoinThreads), p.count, s_keys, &s_bound, lane);
-    each_list([&](int list, uint64_t key) {
-        if (key >= bound) s_lists[atomicAdd(&s_further, 1)] = static_cast<uint16_t>(list);
-    });
-    __syncthreads();
-    const int items = s_further * top;
-    auto each_item = [&](auto&& f) __attribute__((always_inline)) {
-        for (int i = threadIdx.x; i < items; i += kJoinThreads) {
-            const int list = s_lists[i / top], at = list * top + i % top;
-            const Entry e = entries[at];
-            const uint64_t key = key_at(list, i % top, e);
-            if (key != 0 && key >= bound) f(at, key, e);
-        }
-    };
-    if (items > 48) {
-        best_key = 0;
-        each_item([&](int, uint64_t key, Entry) { best_key = key > best_key ? key : best_key; });
-        const uint64_t closer = bound_of_keys(best_key, min(items, kJoinThreads), p.count, s_keys, &s_bound, lane);
-        bound = closer > bound ? closer : bound;
-        __syncthreads();
-    }
-    each_item([&](int at, uint64_t key, Entry e) {
+    auto offer = [&](int at, int beam, uint64_t key, uint32_t token) {
         const int place = atomicAdd(&s_count, 1);
         if (place >= kOffers) return;
         s_keys[place] = key;
         s_at[place] = ~static_cast<uint32_t>(at);
-        s_token[place] = index_of(e);
-    });
+        s_beam[place] = static_cast<uint8_t>(beam);
+        s_token[place] = token;
+    };
+    uint64_t best_key = 0, bound = 0;
+    int further = lists;                                   // lists that are looked at
+    if (kept) {
+        const int of_beam = segments * top;
+        const float per = 1.0f / static_cast<float>(of_beam);
+        // (half a place from a whole number of beams at least: the product's error is far below that)
+        static_assert(kKept <= 1 << 12, "the quotient by a product in 32 bits");
+        auto beam_of = [&](int at) { return static_cast<int>((static_cast<float>(at) + 0.5f) * per); };
+        double rest[kEach], base[kEach];
+        bool done[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int beam = beam_of(min(item_of(i), all - 1));
+            rest[i] = s_rest[beam];
+            base[i] = s_base[beam];
+            done[i] = s_done[beam];
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            // (key_at without a branch)
+            const int at = item_of(i);
+            const float logit = value_of(mine[i]);
+            const bool of_done = at == beam_of(at) * of_beam, of_logit = (mine[i] != 0) & (logit > -__builtin_inff());
+            const bool offers = (at < all) & (rest[i] > -__builtin_inf()) & (done[i] ? of_done : of_logit);
+            const double score = rest[i] + (done[i] ? 0.0 : static_cast<double>(logit) - base[i]);
+            const uint64_t key = offers ? key_of_score(score) : 0;
+            s_item_keys[i * kJoinThreads + threadIdx.x] = key;
+            s_item_tokens[i * kJoinThreads + threadIdx.x] = index_of(mine[i]);
+            best_key = key > best_key ? key : best_key;
+        }
+        if (all > kFew) bound = bound_of_keys(best_key, p.count, s_bounds, wave, lane);
+        for (int j = 0; j * kJoinThreads < all; ++j) {
+            const uint64_t key = s_item_keys[j * kJoinThreads + threadIdx.x];
+            if (key != 0 && key >= bound) offer(item_of(j), beam_of(item_of(j)), key, s_item_tokens[j * kJoinThreads + threadIdx.x]);
+        }
+    } else {
+        auto each_list = [&](auto&& f) __attribute__((always_inline)) {
+            for (int list = threadIdx.x; list < lists; list += kJoinThreads) {
+                const Entry e = entries[list * top];
+                const uint64_t key = key_at(list, 0, e);
+                if (key != 0 && key >= bound) f(list, key, e);
+            }
+        };
+        const auto better = [&](int, uint64_t key, Entry) { best_key = key > best_key ? key : best_key; };
+        each_list(better);
+        bound = bound_of_keys(best_key, p.count, s_bounds, wave, lane);
+        each_list([&](int list, uint64_t, Entry) { s_lists[atomicAdd(&s_further, 1)] = static_cast<uint16_t>(list); });
+        __syncthreads();
+        further = s_further;
+        auto each_item = [&](auto&& f) __attribute__((always_inline)) {
+            for (int i = threadIdx.x; i < further * top; i += kJoinThreads) {
+                const int list = s_lists[i / top], at = list * top + i % top;
+                const Entry e = entries[at];
+                const uint64_t key = key_at(list, i % top, e);
+                if (key != 0 && key >= bound) f(at, key, e);
+            }
+        };
+        if (further * top > kFew) {
+            best_key = 0;
+            each_item(better);
+            const uint64_t closer = bound_of_keys(best_key, p.count, s_bounds, wave, lane);
+            bound = closer > bound ? closer : bound;
+        }
+        each_item([&](int at, uint64_t key, Entry e) { offer(at, at / top / segments, key, index_of(e)); });
+    }
     __syncthreads();
     const int offers = s_count;
     if (offers < kOffers && threadIdx.x < 8) s_keys[offers + threadIdx.x] = 0;
     __syncthreads();
     const int64_t out = entry * p.count;
-    auto write = [&](int place, uint64_t key, uint32_t at, uint32_t token) {
-        const int beam = static_cast<int>(~at) / top / segments;
+    auto write = [&](int place, uint64_t key, int beam, uint32_t token) {
         p.out_scores[out + place] = static_cast<float>(score_of_key(key));
         p.tokens[out + place] = s_done[beam] ? -1 : static_cast<int64_t>(token);
         p.parents[out + place] = beam;
@@ -447,17 +501,17 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
             int place = a.larger;
             if (a.equal > 1)
                 for (int n = 0; n < offers; ++n) place += s_keys[n] == key && s_at[n] > at;
-            if (place < p.count) write(place, key, at, s_token[threadIdx.x]);
+            if (place < p.count) write(place, key, s_beam[threadIdx.x], s_token[threadIdx.x]);
         } else if (static_cast<int>(threadIdx.x) < p.count) {
             leave(threadIdx.x);
         }
         return;
     }
     Offer best = {0, 0};
-    for (int i = wave * 64; i < items; i += kJoinThreads) {
+    for (int i = wave * 64; i < further * top; i += kJoinThreads) {
         Offer o = {0, 0};
-        if (i + lane < items) {
-            const int list = s_lists[(i + lane) / top], place = (i + lane) % top;
+        if (i + lane < further * top) {
+            const int list = kept ? (i + lane) / top : s_lists[(i + lane) / top], place = (i + lane) % top;
             const uint64_t key = key_at(list, place, entries[list * top + place]);
             if (key != 0) o = {key, ~static_cast<uint32_t>(list * top + place)};
         }
@@ -467,7 +521,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
     __syncthreads();
     if (wave != 0) return;
     for (int w = 1; w < kJoinWaves; ++w) best = merge_waves(best, s_sorted[w][lane], lane);
-    if (lane < p.count) best.key != 0 ? write(lane, best.key, best.at, index_of(entries[~best.at])) : leave(lane);
+    if (lane < p.count) best.key != 0 ? write(lane, best.key, static_cast<int>(~best.at) / top / segments, index_of(entries[~best.at])) : leave(lane);
 }
 
 int check(const QaBeamSearchParams& p) {

@@ -61,7 +61,8 @@ int qa_mxfp4_dequant(const QaMxDequantParams* p, void* stream);
 /*
  * d[m, n] = sum_k a[m, k] * w[n, k], summed in fp32 and rounded once to the output's type.  w is an operand as above, n rows of it; a is one too,
  * or with an a_type other than QA_LM_I8 rows of floating-point numbers, taken as qa_mxfp4_quant leaves them (their codes
- * are written to the workspace, or to nowhere where the rows are few).
+ * are written to the workspace, or to nowhere where the rows are few).  k up to 2^23, rows of codes up to 2^22 bytes apart, m and n up to 2^31 - 256; with
+ * k 0 the sums are 0, and d's rows lie next to each other.
  */
 typedef struct QaMxGemmParams {
     int32_t m, n, k;

@@ -374,7 +374,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
         if (share < segments) r = joined(r, second);
         for (int i = part + 2 * share; there && i < segments; i += share) r = joined(r, parts[beam * segments + i]);
         if (__builtin_amdgcn_ballot_w64(r.m != 0.0f) == 0) {
-            // one place for all of them, then their sum
+            // one place for all of them, then their sum (bit for bit what joined gives: powers of two round nothing)
             int e = r.s == 0.0 ? -kNowhere : r.e;
             each_mask(share, [&](auto mask) { e = max(e, static_cast<int>(word_across<decltype(mask)::value>(static_cast<uint32_t>(e), lane))); });
             r.s = ldexp(r.s, max((r.s == 0.0 ? e : r.e) - e, -2000));

@@ -7,11 +7,12 @@ namespace {
 
 constexpr int kFusedRows = 16;             // of numbers, quantised where they are multiplied
 constexpr int64_t kMaxPitch = 1 << 22;     // bytes of an operand's row: those of a tile in 32 bits
+constexpr int kMaxRows = 0x7fffffff - 255; // rows and columns: whole tiles of them in 32 bits
 
 int check(const QaMxGemmParams& p) {
     if (p.m < 0 || p.n < 0 || p.k < 0) return QA_ERR_SHAPE;
     if (!is_float_type(p.out_type) || (p.a_type != QA_LM_I8 && !is_float_type(p.a_type))) return QA_ERR_UNSUPPORTED;
-    if (p.k % kBlock != 0 || p.k / 2 > kMaxPitch) return QA_ERR_SHAPE;
+    if (p.k % kBlock != 0 || p.k / 2 > kMaxPitch || p.m > kMaxRows || p.n > kMaxRows) return QA_ERR_SHAPE;
     return QA_OK;
 }
 bool fused(const QaMxGemmParams& p) { return p.a_type != QA_LM_I8 && p.m <= kFusedRows; }

@@ -25,7 +25,7 @@ struct Tensors {
     int32_t first[kTensors + 1];       // workgroup of the first unit; behind the last one, all of them
     int32_t count;
 };
-static_assert(sizeof(Tensors) < 3072, "arguments of a launch");
+static_assert(sizeof(Tensors) <= 4000, "arguments of a launch: 4 KB");
 
 // units of a thread, as far as the registers go
 template <int BEAMS>

@@ -248,7 +248,7 @@ class W8A8B16O16Linear(_W8A8Base, _AlphaHooks):
         else:
             y = torch.empty((x2d.shape[0], self.out_features + self.pad_out), dtype=torch.float16, device=x.device)
             ops.scaled_mm_dq(y, x2d, self.weight, _token_scales(x_scale, shape, self.a), self.b)
-        return ops.beam_search_step(y.view(*shape, -1)[..., :self.out_features], scores, count, done)
+        return ops.beam_search_step(y.view(*shape, y.shape[-1])[..., :self.out_features], scores, count, done)
 
     def __repr__(self):
         return f"W8A8B16O16Linear(in_features={self.in_features}, out_features={self.out_features})"
@@ -369,7 +369,7 @@ class W4A8B16O16Linear(_W4A8Base):
         shape, x2d = _beams_like(x), x.reshape(-1, x.shape[-1]).contiguous()
         a = _token_scales(x_scale, shape, self.input_scale)
         y = ops.w4a8o16_gemm(x2d, self.weight, a, self.s_channel, self.s_group, self.workspace, x2d.shape[0], self.size_n, self.size_k)
-        return ops.beam_search_step(y.view(*shape, -1)[..., :self.out_features], scores, count, done)
+        return ops.beam_search_step(y.view(*shape, y.shape[-1])[..., :self.out_features], scores, count, done)
 
     @classmethod
     def from_fp16(cls, originalLayer: nn.Linear, input_scale: torch.Tensor):

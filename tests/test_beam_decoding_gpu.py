@@ -124,3 +124,12 @@ def test_selection_of_the_int8_heads(dev, out):
             assert scaled.tokens.shape == (batch, beams) or scaled.tokens.shape == (batch, 5)
         with pytest.raises(RuntimeError):
             head.beam_search_step(x[0], scores, 5)
+
+
+def test_heads_without_entries(dev):
+    layer = torch.nn.Linear(256, 500, bias=False).half().to(dev)
+    scores = torch.zeros(0, 4, device=dev)
+    for head in (W8A8B16O16Linear.from_fp16(layer, torch.tensor(0.0217)), W4A8B16O16Linear.from_fp16(layer, torch.tensor(0.0217)), MXFP4Linear.from_fp16(layer)):
+        x = torch.zeros(0, 4, 256, dtype=torch.float16 if isinstance(head, MXFP4Linear) else torch.int8, device=dev)
+        got = head.beam_search_step(x, scores, 3)
+        assert all(t.shape == (0, 3) for t in got)

@@ -236,3 +236,88 @@ def test_the_same_every_time(dev):
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert all(torch.equal(x, y) for x, y in zip(a, b)), step
+
+
+def far_and_equal(dev, vocab, seed):
+    """8 beams, all of them with the logits and the score of the first but for one whose logits are far from 0"""
+    logits, scores = make(1, 1, vocab, "fp32", dev, seed)
+    logits, scores = logits.expand(1, 8, vocab).clone(), scores.expand(1, 8).clone()
+    logits[0, 1] += 3e6
+    scores[0, 1] = -1e6
+    return logits, scores
+
+
+@pytest.mark.parametrize("vocab", [30000, 100000])
+def test_a_beam_does_not_see_the_others(dev, vocab):
+    """equal beams stay equal to the last bit, whichever beams share a wave with them"""
+    for seed in range(12):
+        got = ops.beam_search_step(*far_and_equal(dev, vocab, seed), 35)
+        want = [0, 2, 3, 4, 5, 6, 7] * 5
+        assert got.parents[0].tolist() == want, seed
+        assert all(len(set(got.tokens[0, 7 * i:7 * i + 7].tolist())) == 1 for i in range(5)), seed
+
+
+def test_workspace_that_held_other_things(dev):
+    """parts of beams that are done are not written, and nothing comes of what lay there"""
+    logits, scores = make(2, 7, 40000, "fp16", dev)
+    done = torch.tensor([[False, True, False, False, True, False, False], [True, False, True, False, False, False, True]], device=dev)
+    outs = []
+    for byte in (0, 0x7f, 0xff, 0xc1):
+        held = [torch.full((n,), byte, dtype=torch.uint8, device=dev) for n in (1 << 12, 1 << 16, 1 << 18, 1 << 20) for _ in range(2)]
+        torch.cuda.synchronize()
+        del held
+        outs.append(check(logits, scores, 9, done))
+    assert all(torch.equal(a, b) for o in outs for a, b in zip(o, outs[0]))
+
+
+@pytest.mark.parametrize("batch,beams,vocab,count,dtype", [
+    (1, 1, 1 << 20, 64, "fp32"), (1, 1, 1 << 20, 7, "fp16"), (1, 3, (1 << 20) - 5, 20, "bf16"), (1, 64, 50280, 64, "fp32"), (2, 64, 30011, 33, "fp16"), (1, 40, 5000, 1, "fp32"),
+    (130, 2, 9000, 64, "fp32"), (1, 2, 256000, 48, "fp32")])
+def test_long_rows_and_many_lists(dev, batch, beams, vocab, count, dtype):
+    g = torch.Generator().manual_seed(vocab + count)
+    # (values that are all different, of one type: no two candidates of a beam are equal, and the scores of beams differ by what no logits do)
+    logits = torch.stack([torch.randperm(vocab, generator=g) for _ in range(min(batch * beams, 4))]).repeat(-(-batch * beams // 4), 1)[:batch * beams].float()
+    logits = (logits.view(batch, beams, vocab) * (12.0 / vocab)).to(TYPES[dtype]).to(dev)
+    scores = (torch.arange(batch * beams).view(batch, beams) * 0.0137 - 5).to(dev)
+    check(logits, scores, count)
+
+
+@pytest.mark.parametrize("rows", [(3, 4), (20, 8)])
+def test_captured_and_on_another_stream(dev, rows):
+    """two graphs with workspaces of their own, replayed in turn with eager calls between them"""
+    inputs = [make(*rows, 30000, "bf16", dev, seed) for seed in range(2)]
+    ops.beam_search_step(*inputs[0], 8)
+    graphs, outs = [], []
+    for logits, scores in inputs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.beam_search_step(logits, scores, 8))
+        graphs.append(graph)
+    for step in range(3):
+        for i, (logits, scores) in enumerate(inputs):
+            new = make(*rows, 30000, "bf16", dev, 10 * step + i)
+            logits.copy_(new[0])
+            scores.copy_(new[1])
+        want = [ops.beam_search_step(*x, 8) for x in inputs]
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for o, w in zip(outs, want) for a, b in zip(o, w)), step
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = ops.beam_search_step(*inputs[0], 8)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+
+
+def test_offsets_past_32_bits(dev):
+    """rows more than 4 GiB into the logits"""
+    batch, vocab = 2100, 1 << 20
+    logits = torch.full((batch, 1, vocab), -30.0, dtype=torch.float16, device=dev)
+    some = [0, 1023, 1024, 2047, 2048, batch - 1]
+    for i, b in enumerate(some):
+        logits[b, 0, 100 * i + 7], logits[b, 0, vocab - 1 - i] = 5.0, 4.0
+    got = ops.beam_search_step(logits, torch.zeros(batch, 1, device=dev), 2)
+    for i, b in enumerate(some):
+        assert got.tokens[b].tolist() == [100 * i + 7, vocab - 1 - i]

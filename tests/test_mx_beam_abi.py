@@ -106,7 +106,8 @@ def test_mm_refusals():
         (dict(w_scales=AT + 8), -3), (dict(d=AT + 1), -3), (dict(out_type=3, d=AT + 2), -3), (dict(lda=520), -3), (dict(lda=496), -3), (dict(ldw=520), -3), (dict(ldw=496), -3),
         (dict(ldd=99), -3), (dict(a_scale_group_stride=48), -3), (dict(a_scale_group_stride=72), -3), (dict(w_scale_group_stride=1584), -3), (dict(w_scale_group_stride=1608), -3),
         (dict(lda=(1 << 24) + 16), -2), (dict(ldw=(1 << 24) + 16), -2), (dict(k=(1 << 25) + 32, lda=1 << 25, ldw=1 << 25), -2),
-        (dict(m=0, a=0, w=0, d=0), 0), (dict(n=0, a=0, w=0, d=0), 0)])
+        (dict(lda=(1 << 22) + 16), -2), (dict(ldw=(1 << 22) + 16), -2), (dict(m=(1 << 31) - 255), -2), (dict(n=(1 << 31) - 255, ldd=1 << 31), -2),
+        (dict(k=0, ldd=104), -3), (dict(m=0, a=0, w=0, d=0), 0), (dict(n=0, a=0, w=0, d=0), 0)])
     # rows of numbers: codes of their own where the rows are many
     p.m, p.a_type, p.lda, p.a_scales = 100, _lib.QA_LM_BF16, 1024, None
     p.workspace_bytes = need = l.qa_mxfp4_mm_workspace_bytes(C.byref(p))

@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 import torch
 
+from launched import expect, kernels
 from mxfp4_reference import operand
 from quamba_amd import MXFP4Linear, ops
 
@@ -216,3 +217,45 @@ def test_module(dev):
         MXFP4Linear.from_fp16(torch.nn.Linear(64, 8).to(dev))
     with pytest.raises(AssertionError):
         MXFP4Linear(40, 8, device=dev)
+
+
+@pytest.mark.parametrize("m,n,k,linear,names", [
+    (1, 100, 64, False, ["mxfp4_direct_kernel<1, 1, signed char>"]), (1, 60000, 64, False, ["mxfp4_tiles_kernel<1, 2, 2, 4, 3, true>"]),
+    (17, 4000, 512, False, ["mxfp4_direct_kernel<2, 1, signed char>"]), (20, 6000, 512, False, ["mxfp4_direct_kernel<2, 2, signed char>"]),
+    (64, 4000, 512, False, ["mxfp4_direct_kernel<2, 2, signed char>"]), (64, 8000, 512, False, ["mxfp4_direct_kernel<4, 2, signed char>"]),
+    (16, 60000, 96, True, ["mxfp4_direct_kernel<1, 1, "]), (17, 4000, 512, True, ["mxfp4_quant_kernel<", "mxfp4_direct_kernel<2, 1, signed char>"]),
+    (100, 9000, 512, False, ["mxfp4_tiles_kernel<1, 2, 2, 2, 4, false>"]), (300, 9000, 96, False, ["mxfp4_tiles_kernel<2, 1, 2, 4, 4, true>"]),
+    (300, 20000, 512, False, ["mxfp4_tiles_kernel<2, 2, 2, 4, 3, false>"]), (4000, 9000, 512, False, ["mxfp4_stream_kernel", "mxfp4_tiles_kernel<2, 1, 2, 4, 4, false>"]),
+    (4300, 9000, 96, False, ["mxfp4_tiles_kernel<4, 2, 2, 4, 2, true>", "mxfp4_tiles_kernel<2, 2, 2, 4, 3, true>"])])
+def test_the_choice_of_kernels(dev, m, n, k, linear, names):
+    g = np.random.default_rng(m)
+    w, w_scales, _ = operand(g, n, k, 0, 2, dev)
+    if linear:
+        x = torch.randn(m, k, device=dev).bfloat16()
+        expect(kernels(lambda: ops.mxfp4_linear(x, w, w_scales))[1], *names)
+    else:
+        a, a_scales, _ = operand(g, m, k, 0, 2, dev)
+        expect(kernels(lambda: ops.mxfp4_mm(a, a_scales, w, w_scales))[1], *names)
+
+
+@pytest.mark.parametrize("m,n", [(70001, 40003), (2200000, 1001), (15, 150000000), (3, 900000000)])
+def test_offsets_past_32_bits(dev, m, n):
+    """outputs of more than 2^31 numbers or operands of more than 2 GiB"""
+    k = 32 if n < 1 << 24 else 64
+    def big(rows, generator):
+        few = min(rows, 997)                               # (row r is row r % few of these)
+        codes, scales, values = operand(generator, few, k, 0, 2, dev)
+        times = -(-rows // few)
+        return codes.repeat(times, 1)[:rows], scales.repeat(1, times, 1)[:, :rows].contiguous(), torch.from_numpy(values).to(dev), few
+    g = np.random.default_rng(m)
+    a, a_scales, a_values, of_a = big(m, g)
+    w, w_scales, w_values, of_w = big(n, g)
+    got = ops.mxfp4_mm(a, a_scales, w, w_scales, torch.bfloat16)
+    want = (a_values @ w_values.T).float().bfloat16()
+    rows = torch.tensor(sorted({0, 1 % m, m // 2, m - 2 if m > 1 else 0, m - 1}), device=dev)
+    for r in rows.tolist():
+        row = want[r % of_a]
+        for first in range(0, n, 1 << 27):
+            last = min(n, first + (1 << 27))
+            at = torch.arange(first, last, device=dev) % of_w
+            assert torch.equal(got[r, first:last], row[at]), (r, first)

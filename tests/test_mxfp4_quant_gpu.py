@@ -129,3 +129,36 @@ def test_refusals(dev):
             ops.mxfp4_dequant(c, s)
     with pytest.raises(NotImplementedError):
         ops.mxfp4_dequant(codes, scales, torch.float64)
+
+
+def test_captured_and_on_another_stream(dev):
+    x = torch.randn(40, 1056, device=dev)
+    ops.mxfp4_dequant(*ops.mxfp4_quant(x))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        codes, scales = ops.mxfp4_quant(x)
+        values = ops.mxfp4_dequant(codes, scales, torch.bfloat16)
+    for step in range(3):
+        x.copy_(torch.randn(40, 1056, device=dev) * 10.0 ** step)
+        want = (*ops.mxfp4_quant(x), ops.mxfp4_dequant(*ops.mxfp4_quant(x), torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((codes, scales, values), want)), step
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = ops.mxfp4_quant(x)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_offsets_past_32_bits(dev):
+    """rows more than 4 GiB into numbers, and 2 GiB into codes"""
+    rows, k = 2100000, 2048
+    x = torch.zeros(rows, k, dtype=torch.float16, device=dev)
+    some = [0, 1, 524287, 524288, 1048577, rows - 9, rows - 1]
+    x[some] = torch.randn(len(some), k, generator=torch.Generator().manual_seed(1)).half().to(dev)
+    codes, scales = ops.mxfp4_quant(x)
+    want_codes, want_scales = ops.mxfp4_quant(x[some])
+    assert torch.equal(codes[some], want_codes) and torch.equal(scales[:, some], want_scales)
+    values = ops.mxfp4_dequant(codes, scales, torch.float16)
+    assert torch.equal(values[some], ops.mxfp4_dequant(want_codes, want_scales, torch.float16)) and int(values.count_nonzero(1).count_nonzero()) == len(some)

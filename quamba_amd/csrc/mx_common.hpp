@@ -22,6 +22,11 @@ __device__ __forceinline__ uint32_t scale_of(uint32_t most_bits) {
     const int e = static_cast<int>(most_bits >> 23);
     return e == 255 ? 255u : static_cast<uint32_t>(max(e - 2, 0));
 }
+// the largest of the four lanes of a block, in all of them
+__device__ __forceinline__ uint32_t most_of_block(uint32_t v) {
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xb1, 0xf, 0xf, true)));
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4e, 0xf, 0xf, true)));
+}
 // 2^(scale - 127); 255: NaN
 __device__ __forceinline__ float power_of(uint32_t scale) {
     return __uint_as_float(scale == 0 ? 0x00400000u : scale == 255 ? 0x7fc00000u : scale << 23);

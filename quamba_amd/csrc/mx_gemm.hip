@@ -5,7 +5,6 @@ namespace qa {
 namespace mx {
 namespace {
 
-constexpr int kFusedRows = 16;             // of numbers, quantised where they are multiplied
 constexpr int64_t kMaxPitch = 1 << 22;     // bytes of an operand's row: those of a tile in 32 bits
 constexpr int kMaxRows = 0x7fffffff - 255; // rows and columns: whole tiles of them in 32 bits
 
@@ -15,7 +14,7 @@ int check(const QaMxGemmParams& p) {
     if (p.k % kBlock != 0 || p.k / 2 > kMaxPitch || p.m > kMaxRows || p.n > kMaxRows) return QA_ERR_SHAPE;
     return QA_OK;
 }
-bool fused(const QaMxGemmParams& p) { return p.a_type != QA_LM_I8 && p.m <= kFusedRows; }
+bool fused(const QaMxGemmParams& p) { return p.a_type != QA_LM_I8 && direct_takes_numbers(p); }
 int64_t code_bytes(const QaMxGemmParams& p) { return static_cast<int64_t>(p.m) * ((p.k / 2 + 15) / 16 * 16); }
 
 int64_t workspace_bytes(const QaMxGemmParams& p) {

@@ -50,7 +50,8 @@ inline bool whole_words(const QaMxGemmParams& p) {
 
 // Straight from memory (mx_gemm_direct.hip).  a_type: codes, or numbers that are quantised on the way.
 int direct_launch(const QaMxGemmParams& p, hipStream_t stream);
-bool direct_takes(const QaMxGemmParams& p);
+bool direct_takes(const QaMxGemmParams& p);             // codes
+bool direct_takes_numbers(const QaMxGemmParams& p);
 // Of codes, in tiles through LDS (mx_gemm_tiles.hip).
 int tiles_launch(const QaMxGemmParams& p, hipStream_t stream);
 

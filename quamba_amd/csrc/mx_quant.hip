@@ -13,12 +13,6 @@ namespace {
 
 constexpr int kThreads = 256, kRows = 2, kTogether = kThreads / 64 * kRows;
 
-// the largest of the four lanes of a block, in all of them
-__device__ __forceinline__ uint32_t most_of_block(uint32_t v) {
-    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xb1, 0xf, 0xf, true)));
-    return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4e, 0xf, 0xf, true)));
-}
-
 // Row and values of a lane's load r: a workgroup has a group of kTogether rows, whose scales lie next to each other, a wave kRows of them at the same time.
 struct Place {
     int64_t row;

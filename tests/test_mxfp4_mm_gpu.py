@@ -58,7 +58,8 @@ def test_sums_that_round(dev, m, n, k, spread):
 
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
-@pytest.mark.parametrize("m,n,k", [(1, 500, 768), (3, 33, 32), (7, 40, 544), (16, 100, 2560), (17, 64, 1536), (64, 300, 96), (200, 77, 1024)])
+@pytest.mark.parametrize("m,n,k", [(1, 500, 768), (3, 33, 32), (7, 40, 544), (16, 100, 2560), (17, 64, 1536), (64, 300, 96), (200, 77, 1024),
+                                   (1, 50280, 2560), (2, 300, 5120), (3, 40000, 544), (4, 20000, 2560), (4, 100, 8224), (5, 1000, 2560), (9, 5000, 2080), (16, 50280, 1536)])
 def test_linear_is_the_product_of_quantised_rows(dev, dtype, m, n, k):
     torch.manual_seed(m + n + k)
     x = (torch.randn(m, k) * (1 + 9 * (torch.rand(k) < 0.05))).to(TYPES[dtype]).to(dev)
@@ -220,10 +221,11 @@ def test_module(dev):
 
 
 @pytest.mark.parametrize("m,n,k,linear,names", [
-    (1, 100, 64, False, ["mxfp4_direct_kernel<1, 1, signed char>"]), (1, 60000, 64, False, ["mxfp4_tiles_kernel<1, 2, 2, 4, 3, true>"]),
-    (17, 4000, 512, False, ["mxfp4_direct_kernel<2, 1, signed char>"]), (20, 6000, 512, False, ["mxfp4_direct_kernel<2, 2, signed char>"]),
-    (64, 4000, 512, False, ["mxfp4_direct_kernel<2, 2, signed char>"]), (64, 8000, 512, False, ["mxfp4_direct_kernel<4, 2, signed char>"]),
-    (16, 60000, 96, True, ["mxfp4_direct_kernel<1, 1, "]), (17, 4000, 512, True, ["mxfp4_quant_kernel<", "mxfp4_direct_kernel<2, 1, signed char>"]),
+    (1, 100, 64, False, ["mxfp4_direct_kernel<1, 1, signed char, false>"]), (1, 60000, 64, False, ["mxfp4_tiles_kernel<1, 2, 2, 4, 3, true>"]),
+    (17, 4000, 512, False, ["mxfp4_direct_kernel<2, 1, signed char, false>"]), (20, 6000, 512, False, ["mxfp4_direct_kernel<2, 2, signed char, false>"]),
+    (64, 4000, 512, False, ["mxfp4_direct_kernel<2, 2, signed char, false>"]), (64, 8000, 512, False, ["mxfp4_direct_kernel<4, 2, signed char, false>"]),
+    (1, 40000, 96, True, ["mxfp4_direct_kernel<1, 1, float, true>"]), (9, 700, 1056, True, ["mxfp4_direct_kernel<1, 1, float, false>"]),
+    (16, 60000, 96, True, ["mxfp4_quant_kernel<", "mxfp4_tiles_kernel<1, 2, 2, 4, 3, true>"]), (17, 4000, 512, True, ["mxfp4_quant_kernel<", "mxfp4_direct_kernel<2, 1, signed char, false>"]),
     (100, 9000, 512, False, ["mxfp4_tiles_kernel<1, 2, 2, 2, 4, false>"]), (300, 9000, 96, False, ["mxfp4_tiles_kernel<2, 1, 2, 4, 4, true>"]),
     (300, 20000, 512, False, ["mxfp4_tiles_kernel<2, 2, 2, 4, 3, false>"]), (4000, 9000, 512, False, ["mxfp4_stream_kernel", "mxfp4_tiles_kernel<2, 1, 2, 4, 4, false>"]),
     (4300, 9000, 96, False, ["mxfp4_tiles_kernel<4, 2, 2, 4, 2, true>", "mxfp4_tiles_kernel<2, 2, 2, 4, 3, true>"])])
@@ -231,7 +233,7 @@ def test_the_choice_of_kernels(dev, m, n, k, linear, names):
     g = np.random.default_rng(m)
     w, w_scales, _ = operand(g, n, k, 0, 2, dev)
     if linear:
-        x = torch.randn(m, k, device=dev).bfloat16()
+        x = torch.randn(m, k, device=dev)
         expect(kernels(lambda: ops.mxfp4_linear(x, w, w_scales))[1], *names)
     else:
         a, a_scales, _ = operand(g, m, k, 0, 2, dev)

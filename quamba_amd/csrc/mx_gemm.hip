@@ -17,10 +17,7 @@ int check(const QaMxGemmParams& p) {
 bool fused(const QaMxGemmParams& p) { return p.a_type != QA_LM_I8 && direct_takes_numbers(p); }
 int64_t code_bytes(const QaMxGemmParams& p) { return static_cast<int64_t>(p.m) * ((p.k / 2 + 15) / 16 * 16); }
 
-int64_t workspace_bytes(const QaMxGemmParams& p) {
-    if (p.a_type == QA_LM_I8 || fused(p)) return 0;
-    return code_bytes(p) + groups_of(p.k) * 16 * p.m;
-}
+int64_t workspace_bytes(const QaMxGemmParams& p, bool one_launch) { return p.a_type == QA_LM_I8 || one_launch ? 0 : code_bytes(p) + groups_of(p.k) * 16 * p.m; }
 
 }  // namespace
 }  // namespace mx
@@ -28,7 +25,7 @@ int64_t workspace_bytes(const QaMxGemmParams& p) {
 
 extern "C" int64_t qa_mxfp4_mm_workspace_bytes(const QaMxGemmParams* p) {
     using namespace qa::mx;
-    return p && check(*p) == QA_OK && p->m > 0 && p->n > 0 && p->k > 0 ? workspace_bytes(*p) : 0;
+    return p && check(*p) == QA_OK && p->m > 0 && p->n > 0 && p->k > 0 ? workspace_bytes(*p, fused(*p)) : 0;
 }
 
 extern "C" int qa_mxfp4_mm(const QaMxGemmParams* p, void* stream_) {
@@ -59,11 +56,12 @@ extern "C" int qa_mxfp4_mm(const QaMxGemmParams* p, void* stream_) {
         return QA_ERR_STRIDE;
     }
     if (p->n > 1 && p->ldw > kMaxPitch) return QA_ERR_SHAPE;
-    const int64_t need = workspace_bytes(*p);
+    const bool one_launch = fused(*p);
+    const int64_t need = workspace_bytes(*p, one_launch);
     if (need && !p->workspace) return QA_ERR_NULL;
     if (need && (!aligned16(p->workspace) || p->workspace_bytes < need)) return QA_ERR_SCRATCH;
     auto of_codes = [&](const QaMxGemmParams& q) { return direct_takes(q) ? direct_launch(q, stream) : tiles_launch(q, stream); };
-    if (fused(*p)) return direct_launch(*p, stream);
+    if (one_launch) return direct_launch(*p, stream);
     if (rows_of_codes) return of_codes(*p);
     // many rows of numbers: quantised once, for all columns
     QaMxQuantParams rows = {};

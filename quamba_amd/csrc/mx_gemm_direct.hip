@@ -172,10 +172,8 @@ int launch(const QaMxGemmParams& p, hipStream_t stream) {
 // tiles ask for them better.  (us by 16 x 16, 32 x 16, 32 x 32, 64 x 32 and in tiles: 64 x 768 x 2560 4.1, 4.5, 5.5, 8, 8; 128 x 768 x 2560 5.1, 4.6, 5.3, 8, 8;
 // 64 x 2560 x 2560 6.7, 6.7, 5.3, 7.3, 7.8; 128 x 2560 x 2560 9.2, 8.8, 8.4, 7.4, 8.0; 16 x 10240 x 2560 6.4, 7.0, 7.0, 8.1, 7.8; 17 x 10240 x 2560 9.1, 7.1, 7.1, 8.3, 7.9;
 // 1 x 50280 x 2560 13.8, 17, 15, 20, 12.5.)
-bool direct_takes(const QaMxGemmParams& p) {
-    const int64_t cus = compute_units();
-    return blocks_of<4, 2>(p) <= cus || (p.m <= 16 && blocks_of<1, 1>(p) <= 10 * cus);
-}
+static bool takes(const QaMxGemmParams& p, int64_t cus) { return blocks_of<4, 2>(p) <= cus || (p.m <= kRows && blocks_of<1, 1>(p) <= 10 * cus); }
+bool direct_takes(const QaMxGemmParams& p) { return takes(p, compute_units()); }
 
 // Numbers in one launch: each wave quantises its group of the rows again, up to four rows by all its lanes, more of them fragment by fragment, and that has to cost less
 // than a launch in front (us by all lanes, by fragments, with a launch of its own: 1 x 2560 x 5120 4.8, 5.7, 6.4; 1 x 10240 x 2560 5.5, 7.2, 7.2; 1 x 50280 x 2560 17, 28,
@@ -183,9 +181,9 @@ bool direct_takes(const QaMxGemmParams& p) {
 // 16 x 768 x 1536 5.4, 3.8, 5.8; 16 x 2560 x 5120 9.7, 8.5, 7.3; 16 x 50280 x 2560 35, 45, 18).  So for more than four rows each SIMD may have one group, and
 // for fewer 32 rows of a group; and codes of as many rows are summed in the same order, so that both ways give the same bits.
 bool direct_takes_numbers(const QaMxGemmParams& p) {
-    if (!direct_takes(p)) return false;
-    const int64_t simds = 4LL * compute_units(), wanted = blocks_of<1, 1>(p) * groups_of(p.k);
-    return p.m <= kSharedRows ? p.m * wanted <= 32 * simds : p.m <= kRows && groups_of(p.k) <= kMaxWaves && wanted <= simds;
+    if (p.m > kRows) return false;
+    const int64_t cus = compute_units(), simds = 4 * cus, wanted = blocks_of<1, 1>(p) * groups_of(p.k);
+    return takes(p, cus) && (p.m <= kSharedRows ? p.m * wanted <= 32 * simds : groups_of(p.k) <= kMaxWaves && wanted <= simds);
 }
 
 int direct_launch(const QaMxGemmParams& p, hipStream_t stream) {
@@ -196,8 +194,9 @@ int direct_launch(const QaMxGemmParams& p, hipStream_t stream) {
     if (p.a_type == QA_LM_F32) return of_numbers(float{});
     if (p.a_type == QA_LM_BF16) return of_numbers(__bf16{});
     if (p.a_type == QA_LM_F16) return of_numbers(_Float16{});
+    if (p.m <= kRows) return launch<1, 1, int8_t>(p, stream);
     const int64_t cus = compute_units();
-    if (p.m <= 16 || blocks_of<1, 1>(p) <= cus) return launch<1, 1, int8_t>(p, stream);
+    if (blocks_of<1, 1>(p) <= cus) return launch<1, 1, int8_t>(p, stream);
     if (blocks_of<2, 1>(p) <= cus) return launch<2, 1, int8_t>(p, stream);
     if (blocks_of<2, 2>(p) <= cus) return launch<2, 2, int8_t>(p, stream);
     return launch<4, 2, int8_t>(p, stream);

@@ -114,7 +114,8 @@ extern "C" int qa_reorder_states(const QaReorderParams* p, void* stream_) {
         if (s.row_bytes == 0) continue;
         if (!s.data) return QA_ERR_NULL;
         if (s.row_stride < s.row_bytes && static_cast<int64_t>(p->batch) * p->beams > 1) return QA_ERR_STRIDE;
-        const int64_t units = s.row_bytes / unit_of(s, p->beams);
+        const int unit = unit_of(s, p->beams);
+        const int64_t units = unit == 16 ? s.row_bytes / 16 : unit == 4 ? s.row_bytes / 4 : s.row_bytes;
         if (units > 0x7fffffffLL || !launchable((units + kThreads - 1) / kThreads * p->batch, kThreads)) return QA_ERR_SHAPE;
     }
     if (p->beams == 1) return QA_OK;

@@ -38,6 +38,27 @@ at::DimVector with_last(at::IntArrayRef shape, int64_t last) {
     return d;
 }
 
+// Answers of one allocation, each on 16 bytes and made without torch's dispatch (a call on little takes the host as long as the GPU, and an allocation 1.2 us).  For
+// answers of kTogether bytes in all: of larger ones who keeps one would keep the others' memory, and the time does not show.
+constexpr int64_t kTogether = 8192;
+class Together {
+  public:
+    Together(int64_t bytes, at::Device device) : memory_(at::empty({bytes}, at::TensorOptions().device(device).dtype(at::kByte))) {}
+    static int64_t place(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+    at::Tensor next(at::IntArrayRef sizes, at::ScalarType type) {
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(memory_.storage()), memory_.key_set(), c10::scalarTypeToTypeMeta(type));
+        const int64_t each = static_cast<int64_t>(c10::elementSize(type));
+        t.unsafeGetTensorImpl()->set_storage_offset(used_ / each);
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+        used_ += place(t.numel() * each);
+        return t;
+    }
+
+  private:
+    at::Tensor memory_;
+    int64_t used_ = 0;
+};
+
 // an operand's codes (rows, k / 2) and scales (groups, rows, 16)
 struct Operand {
     int64_t rows, k, pitch, group_stride;
@@ -78,8 +99,17 @@ PyObject* mxfp4_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
         in_rows(flat, "x");
         require(flat.size(0) <= kMost && k <= kMost, "mxfp4_quant: a size beyond 32 bits");
         const OnDevice on(x.device());
-        const auto opts = at::TensorOptions().device(x.device()).dtype(at::kByte);
-        const at::Tensor codes = at::empty(with_last(x.sizes(), k / 2), opts), scales = at::empty({groups_of(k), flat.size(0), 16}, opts);
+        at::Tensor codes, scales;
+        const int64_t code_bytes = flat.size(0) * (k / 2), scale_bytes = groups_of(k) * flat.size(0) * 16;
+        if (code_bytes + scale_bytes <= kTogether) {
+            Together all(Together::place(code_bytes) + scale_bytes, x.device());
+            codes = all.next(with_last(x.sizes(), k / 2), at::kByte);
+            scales = all.next({groups_of(k), flat.size(0), 16}, at::kByte);
+        } else {
+            const auto opts = at::TensorOptions().device(x.device()).dtype(at::kByte);
+            codes = at::empty(with_last(x.sizes(), k / 2), opts);
+            scales = at::empty({groups_of(k), flat.size(0), 16}, opts);
+        }
         QaMxQuantParams p = {};
         p.rows = static_cast<int32_t>(flat.size(0));
         p.k = static_cast<int32_t>(k);
@@ -230,8 +260,18 @@ PyObject* beam_search_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const OnDevice on(device);
         const at::Tensor own = scores.is_contiguous() ? scores : scores.contiguous(), at_end = !done || done->is_contiguous() ? (done ? *done : at::Tensor()) : done->contiguous();
         const auto opts = at::TensorOptions().device(device);
-        const at::Tensor best = at::empty({batch, count}, opts.dtype(at::kFloat)), tokens = at::empty({batch, count}, opts.dtype(at::kLong));
-        const at::Tensor parents = at::empty({batch, count}, opts.dtype(at::kLong));
+        at::Tensor best, tokens, parents;
+        const int64_t places = batch * count;
+        if (places * (4 + 2 * 8) <= kTogether) {
+            Together all(2 * Together::place(places * 8) + places * 4, device);
+            tokens = all.next({batch, count}, at::kLong);
+            parents = all.next({batch, count}, at::kLong);
+            best = all.next({batch, count}, at::kFloat);
+        } else {
+            best = at::empty({batch, count}, opts.dtype(at::kFloat));
+            tokens = at::empty({batch, count}, opts.dtype(at::kLong));
+            parents = at::empty({batch, count}, opts.dtype(at::kLong));
+        }
         QaBeamSearchParams p = {};
         p.batch = static_cast<int32_t>(batch);
         p.beams = static_cast<int32_t>(beams);

@@ -960,7 +960,7 @@ def _mx_beam():
         native.bind(tuple(ct.cast(getattr(l, n), ct.c_void_p).value for n in (
             "qa_mxfp4_quant", "qa_mxfp4_dequant", "qa_mxfp4_mm_workspace_bytes", "qa_mxfp4_mm", "qa_beam_search_workspace_bytes", "qa_beam_search_step",
             "qa_reorder_states")),
-            (torch.cuda.current_device, torch.cuda.set_device, torch._C._cuda_getCurrentRawStream, torch.cuda.OutOfMemoryError, _lib.check))
+            (torch._C._cuda_getDevice, torch.cuda.set_device, torch._C._cuda_getCurrentRawStream, torch.cuda.OutOfMemoryError, _lib.check))
         _mx_beam_native = native
     return _mx_beam_native
 

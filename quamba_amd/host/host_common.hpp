@@ -36,11 +36,20 @@ struct Refused {
 };
 struct Raised {};              // a Python error is set
 
-void require(bool fine, const std::string& text) {
-    if (!fine) throw Refused{PyExc_RuntimeError, text};
+// (texts are put together where a check fails only: a dozen of them a call would take it a microsecond)
+template <class... Parts>
+[[noreturn]] void refuse(PyObject* type, const Parts&... parts) {
+    std::string text;
+    ((text += parts), ...);
+    throw Refused{type, text};
 }
-void supported(bool fine, const std::string& text) {
-    if (!fine) throw Refused{PyExc_NotImplementedError, text};
+template <class... Parts>
+void require(bool fine, const Parts&... parts) {
+    if (!fine) refuse(PyExc_RuntimeError, parts...);
+}
+template <class... Parts>
+void supported(bool fine, const Parts&... parts) {
+    if (!fine) refuse(PyExc_NotImplementedError, parts...);
 }
 
 // No C++ exception passes through the interpreter.
@@ -102,16 +111,18 @@ std::string shape_text(at::IntArrayRef s) {
     for (size_t i = 0; i < s.size(); ++i) text += (i ? ", " : "") + std::to_string(s[i]);
     return text + (s.size() == 1 ? ",)" : ")");
 }
-void on_gpu(const at::Tensor& t, const char* name) { require(t.is_cuda(), std::string(name) + " must be a GPU tensor (quamba_amd has no CPU path)"); }
-void beside(const at::Tensor& t, const char* name, at::Device device) { require(t.device() == device, std::string(name) + " must be on " + device.str()); }
+void on_gpu(const at::Tensor& t, const char* name) { require(t.is_cuda(), name, " must be a GPU tensor (quamba_amd has no CPU path)"); }
+void beside(const at::Tensor& t, const char* name, at::Device device) {
+    if (t.device() != device) refuse(PyExc_RuntimeError, name, " must be on ", device.str());
+}
 void shaped(const at::Tensor& t, const char* name, at::IntArrayRef shape) {
-    if (!t.sizes().equals(shape)) require(false, std::string(name) + " must have shape " + shape_text(shape) + ", not " + shape_text(t.sizes()));
+    if (!t.sizes().equals(shape)) refuse(PyExc_RuntimeError, name, " must have shape ", shape_text(shape), ", not ", shape_text(t.sizes()));
 }
 // rows next to or apart from each other, each of them in one piece
 void in_rows(const at::Tensor& t, const char* name) {
     const int64_t n = t.dim();
-    require(n == 0 || t.stride(n - 1) == 1 || t.size(n - 1) <= 1, std::string(name) + " must be contiguous along the last dimension");
-    require(n < 2 || t.size(0) <= 1 || t.stride(0) >= t.size(1), std::string("the rows of ") + name + " must not overlap");
+    require(n == 0 || t.stride(n - 1) == 1 || t.size(n - 1) <= 1, name, " must be contiguous along the last dimension");
+    require(n < 2 || t.size(0) <= 1 || t.stride(0) >= t.size(1), "the rows of ", name, " must not overlap");
 }
 int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 const void* address(const at::Tensor* t) { return t ? t->const_data_ptr() : nullptr; }

@@ -64,21 +64,20 @@ struct Operand {
     int64_t rows, k, pitch, group_stride;
     const uint8_t *codes, *scales;
 };
-Operand operand(const at::Tensor& codes, const at::Tensor& scales, const std::string& name, at::Device device) {
-    const std::string of_scales = name + "_scales";
-    beside(codes, name.c_str(), device);
-    beside(scales, of_scales.c_str(), device);
-    require(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, name + " and " + of_scales + " must be uint8");
-    require(codes.dim() == 2 && codes.size(1) % 16 == 0, name + " must be (rows, K / 2), K a multiple of 32");
-    in_rows(codes, name.c_str());
+Operand operand(const at::Tensor& codes, const at::Tensor& scales, const char* name, const char* of_scales, at::Device device) {
+    beside(codes, name, device);
+    beside(scales, of_scales, device);
+    require(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, name, " and ", of_scales, " must be uint8");
+    require(codes.dim() == 2 && codes.size(1) % 16 == 0, name, " must be (rows, K / 2), K a multiple of 32");
+    in_rows(codes, name);
     Operand o = {codes.size(0), 2 * codes.size(1), row_stride(codes), 0, codes.const_data_ptr<uint8_t>(), scales.const_data_ptr<uint8_t>()};
-    require(std::max(o.rows, o.k) <= kMost, name + ": a size beyond 32 bits");
-    shaped(scales, of_scales.c_str(), {groups_of(o.k), o.rows, 16});
+    require(std::max(o.rows, o.k) <= kMost, name, ": a size beyond 32 bits");
+    shaped(scales, of_scales, {groups_of(o.k), o.rows, 16});
     o.group_stride = scales.size(0) > 1 ? scales.stride(0) : 16 * o.rows;
     require(scales.numel() == 0 || (scales.stride(2) == 1 && (o.rows == 1 || scales.stride(1) == 16) && o.group_stride >= 16 * o.rows && o.group_stride % 16 == 0),
-            of_scales + " must lie as mxfp4_quant gives them: 16 bytes a row, rows next to each other");
+            of_scales, " must lie as mxfp4_quant gives them: 16 bytes a row, rows next to each other");
     auto whole = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-    require(codes.numel() == 0 || (whole(o.codes) && whole(o.scales) && o.pitch % 16 == 0), name + " and " + of_scales + ": rows on 16 bytes");
+    require(codes.numel() == 0 || (whole(o.codes) && whole(o.scales) && o.pitch % 16 == 0), name, " and ", of_scales, ": rows on 16 bytes");
     return o;
 }
 
@@ -138,7 +137,7 @@ PyObject* mxfp4_dequant(PyObject*, PyObject* const* a, Py_ssize_t n) {
         require(codes.dim() >= 1, "codes must be (..., K / 2)");
         on_gpu(codes, "codes");
         const at::Tensor flat = as_rows(codes, codes.size(-1));
-        const Operand o = operand(flat, scales, "codes", codes.device());
+        const Operand o = operand(flat, scales, "codes", "scales", codes.device());
         const OnDevice on(codes.device());
         const at::Tensor out = at::empty(with_last(codes.sizes(), o.k), at::TensorOptions().device(codes.device()).dtype(type));
         QaMxDequantParams p = {};
@@ -188,7 +187,7 @@ PyObject* mxfp4_mm(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const auto type = dtype_or_none(args[4], "out_dtype").value_or(at::kHalf);
         supported(is_float(type), "out_dtype must be fp16, bf16 or fp32");
         on_gpu(a, "a");
-        const Operand of_a = operand(a, tensor(args[1], "a_scales"), "a", a.device()), of_w = operand(w, tensor(args[3], "w_scales"), "w", a.device());
+        const Operand of_a = operand(a, tensor(args[1], "a_scales"), "a", "a_scales", a.device()), of_w = operand(w, tensor(args[3], "w_scales"), "w", "w_scales", a.device());
         require(of_a.k == of_w.k, "a and w must have the same K");
         QaMxGemmParams p = {};
         p.m = static_cast<int32_t>(of_a.rows);
@@ -214,7 +213,7 @@ PyObject* mxfp4_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
         require(is_float(x.scalar_type()), "x must be fp16, bf16 or fp32");
         const auto type = dtype_or_none(args[3], "out_dtype").value_or(x.scalar_type());
         supported(is_float(type), "out_dtype must be fp16, bf16 or fp32");
-        const Operand of_w = operand(w, tensor(args[2], "w_scales"), "w", x.device());
+        const Operand of_w = operand(w, tensor(args[2], "w_scales"), "w", "w_scales", x.device());
         require(x.size(-1) == of_w.k, "x and w must have the same K");
         const at::Tensor flat = as_rows(x, of_w.k);
         in_rows(flat, "x");

@@ -4,8 +4,8 @@
 // workgroup for each entry of the batch joins the sums of its beams, turns the entries into scores and sorts those that reach a bound.
 //
 // Scores of different beams are compared, and which of two comes first is an answer in whole numbers.  So the sums are held in 64 bits and their terms are good to
-// some 1e-10: e^d is 2^(n / 512) from a table by e^r, |r| <= ln 2 / 1024, from a polynomial whose first missing term is r^3 / 6 < 6e-11.  Operations in 64 bits run at
-// the rate of those in 32, and thirteen instructions a value are what a launch on many rows takes its time for.
+// some 1e-10: e^d is 2^(n / 512) from a table by e^r, |r| <= ln 2 / 1024, from a polynomial whose first missing term is r^3 / 6 < 6e-11.  Operations in 64 bits take 5.4
+// cycles of a wave and those in 32 some 4 to 5; thirteen of them a value are what a launch on many rows takes its time for.
 #include "../../include/quamba_amd_beam.h"
 #include "logit_rows.hpp"
 
@@ -23,35 +23,46 @@ struct BeamPart {
     double s;
 };
 
-// The sum of a part of a row, by one wave (m and e are the same in its lanes).  64 bits hold e^600 as well as e^-600, so where the first values are is good enough until one is
+// The sum of a part of a row, by one wave (all but s are the same in its lanes).  64 bits hold e^600 as well as e^-600, so where the first values are is good enough until one is
 // more than kReach above it.
 constexpr float kReach = 600.0f;
 constexpr int kSteps = 512;
 constexpr double kLn2Wide = 0.69314718055994531;
 constexpr int kNowhere = 1 << 29;          // below it there is no e of a sum
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
 struct WideSum {
     float m;
     int e;
     double s;
-    bool placed;               // a value was seen
-    __device__ __forceinline__ void clear() { m = 0.0f; e = 0; s = 0.0; placed = false; }
+    float limit, least;        // values above the one are seen from another place (-inf: none was seen yet), those below the other count as it
+    double round;
+    __device__ __forceinline__ void clear() {
+        m = 0.0f;
+        e = 0;
+        s = 0.0;
+        limit = -__builtin_inff();
+        least = 0.0f;
+        round = 0.0;
+    }
     // seen from where values up to `most` are
     __device__ __forceinline__ void place(float most) {
         const float before_m = m;
         const int before_e = e;
         const bool near = fabsf(most) <= kFarthest;
-        m = near ? 0.0f : most;
-        e = near ? static_cast<int>(rintf(most * kLog2e)) : 0;
-        if (placed) s *= exp(fmax((static_cast<double>(before_m) - m) + (before_e - e) * kLn2Wide, -700.0));
-        placed = true;
+        m = uniform(near ? 0.0f : most);
+        e = __builtin_amdgcn_readfirstlane(near ? static_cast<int>(rintf(most * kLog2e)) : 0);
+        if (limit > -__builtin_inff()) s *= exp(fmax((static_cast<double>(before_m) - m) + (before_e - e) * kLn2Wide, -700.0));
+        const float here = near ? static_cast<float>(e) * kLn2 : m;
+        limit = uniform(here + kReach);
+        least = uniform(here - 700.0f);
+        // (1.5 * 2^52: the rounded multiple of a step is in the low word; less the steps of 2^e)
+        round = 6755399441055744.0 - static_cast<double>(e) * kSteps;
     }
-    // e^d, d from -700 to kReach + some (a NaN stays one), added for B values d = v - m; powers[i] = 2^(i / kSteps).  In steps, so that the reads of the table are on their way together: one after
-    // the other they took 130 cycles a value, most of it waiting.
+    // e^d, d from -700 to kReach + some (a NaN stays one), added for B values d = v - m; powers as fill_powers leaves them.  In steps, so that the reads of the table are on
+    // their way together: one after the other they took 130 cycles a value, most of it waiting.
     template <int B>
     __device__ __forceinline__ void add_exponentials(const double (&d)[B], const double* powers) {
         constexpr double kPerUnit = 738.65986093514926, kStep = 0.0013538030870311431;     // 512 log2 e, ln 2 / 512
-        // (1.5 * 2^52: the rounded multiple of a step is in the low word; less the steps of 2^e)
-        const double round = 6755399441055744.0 - static_cast<double>(e) * kSteps;
         int n[B];
         double value[B], power[B];
 #pragma unroll
@@ -67,7 +78,7 @@ struct WideSum {
         for (int j = 0; j < B; ++j) {
             // (into the exponent, which stays a normal one)
             const uint64_t bits = __builtin_bit_cast(uint64_t, power[j]);
-            const uint32_t high = static_cast<uint32_t>(bits >> 32) + (static_cast<uint32_t>(n[j] & ~(kSteps - 1)) << (20 - 9));
+            const uint32_t high = static_cast<uint32_t>(bits >> 32) + (static_cast<uint32_t>(n[j]) << (20 - 9));
             s = __builtin_fma(value[j], __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(bits)), s);
         }
     }
@@ -75,9 +86,8 @@ struct WideSum {
     // values of which `most` is the largest of this lane's
     template <int B>
     __device__ __forceinline__ void add(const float (&v)[B], float most, const double* powers) {
-        const float here = !placed ? -__builtin_inff() : m != 0.0f ? m : static_cast<float>(e) * kLn2;
-        if (__builtin_amdgcn_ballot_w64(placed ? most - here > kReach : most > here)) place(wave_max(fmaxf(most, here)));
-        if (!placed) {
+        if (__builtin_amdgcn_ballot_w64(most > limit)) place(wave_max(most));
+        if (!(limit > -__builtin_inff())) {
             // (masked values alone, or NaNs)
 #pragma unroll
             for (int j = 0; j < B; ++j) s = v[j] == v[j] ? s : __builtin_nan("");
@@ -85,7 +95,6 @@ struct WideSum {
         }
         double d[B];
         if (m == 0.0f) {
-            const float least = static_cast<float>(e) * kLn2 - 700.0f;
 #pragma unroll
             for (int j = 0; j < B; ++j) {
                 float one;                                 // (the larger, a NaN if there is one)
@@ -132,8 +141,10 @@ __device__ __forceinline__ double wave_sum(double s, int lane) {
     return s;
 }
 
+// powers[i] = 2^(i / kSteps), less i steps in the exponent's place: n steps added there, whatever n, make 2^(n / kSteps) of powers[n mod kSteps]
 __device__ __forceinline__ void fill_powers(double (&powers)[kSteps]) {
-    for (int i = threadIdx.x; i < kSteps; i += blockDim.x) powers[i] = exp2(static_cast<double>(i) / kSteps);
+    for (int i = threadIdx.x; i < kSteps; i += blockDim.x)
+        powers[i] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, exp2(static_cast<double>(i) / kSteps)) - (static_cast<uint64_t>(i) << (52 - 9)));
 }
 
 typedef uint64_t v2k __attribute__((ext_vector_type(2)));
@@ -157,10 +168,11 @@ __device__ __forceinline__ Above above(const uint64_t* keys, int n, uint64_t own
 }
 
 // A workgroup has a segment of up to kMaxLoads chunks, one load a lane each; kAhead of them are under way while one is summed.  What each load's largest value is goes to LDS, and
-// when all were seen a bound says which loads have one of the best entries: those are read once more, all at the same time, and what reaches the bound is ranked (each
-// counts the others that are larger).  (64 x 8 rows of 50280 bf16, count 16: 26 us, of which the loop without exponentials 12.4, the exponentials 9 and the
-// selection 6; with the entries kept on the way, as token_logprobs has them, 35.  Four or six loads ahead, the loop unrolled over them or more segments: the same.)
-constexpr int kAhead = 3;
+// when all were seen a bound says which loads have one of the best entries: their values are read once more, a lane each, and what reaches the bound is ranked (each
+// counts the others that are larger).  64 x 8 rows of 50280 bf16, count 16, take 23 us (2.2 TB/s): the loop 18, bound by the vector units (the loads alone 12), and the
+// selection of the last of a CU's four workgroups, which the others' hide behind their loops.  (Registers handed on from load to load, for which the compiler waits each time,
+// 26; entries kept on the way, as token_logprobs has them, 35; three to five loads ahead the same; six or eight workgroups a CU 26 and 28.)
+constexpr int kAhead = 2;
 
 template <class T, bool WIDE>
 __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchParams p, int top, int segments, int each) {
@@ -185,53 +197,71 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
 
     // load u of thread `thread` (what is not there: the last one)
     auto place = [&](int u, int thread) { return (first + u) * kThreads + thread; };
+    const T* const from = vectors ? logits : static_cast<const T*>(p.workspace);           // (something to load, if for nothing)
     auto load = [&](Raw<T, V>& raw, int u, int thread) __attribute__((always_inline)) {
-        raw.template load<WIDE>(logits + static_cast<int64_t>(min(place(u, thread), vectors - 1)) * V);
+        raw.template load<WIDE>(from + static_cast<int64_t>(min(place(u, thread), max(vectors - 1, 0))) * V);
     };
-    Raw<T, V> raw[kAhead];
+    // chunks that are there for every thread; one that is not may follow
+    const int whole = max(0, min(loads, vectors / kThreads - first));
+    Raw<T, V> raw[kAhead], last;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-        if (i < loads) load(raw[i], i, threadIdx.x);
+    for (int i = 0; i < kAhead; ++i) load(raw[i], i, threadIdx.x);
+    load(last, whole, threadIdx.x);
     // fewer than V values behind the last whole load: one each in the first lanes of the last segment
     const int rest_at = vectors * V + lane;
     const bool has_rest = segment == segments - 1 && wave == 0 && lane < rest;
-    float rest_v = none;
-    if (has_rest) rest_v = static_cast<float>(logits[rest_at]);
+    T rest_raw = static_cast<T>(0.0f);
+    if (has_rest) rest_raw = logits[rest_at];
     fill_powers(s_powers);
     if (threadIdx.x == 0) s_count = 0;
     __syncthreads();
     WideSum r;
     r.clear();
-    float most = rest_v;
-    for (int u = 0; u < loads; ++u) {
-        const Raw<T, V> now = raw[0];
-#pragma unroll
-        for (int i = 0; i + 1 < kAhead; ++i) raw[i] = raw[i + 1];
-        if (u + kAhead < loads) load(raw[kAhead - 1], u + kAhead, threadIdx.x);
+    float most = none;
+    auto sum = [&](int u, const Raw<T, V>& now, auto whole_c) __attribute__((always_inline)) {
         float v[V], most_of = none;
+        const bool there = decltype(whole_c)::value || place(u, threadIdx.x) < vectors;
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = now.get(j);
-        if ((first + u + 1) * kThreads > vectors && place(u, threadIdx.x) >= vectors) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = none;
-        }
+        for (int j = 0; j < V; ++j) v[j] = there ? now.get(j) : none;
 #pragma unroll
         for (int j = 0; j < V; ++j) most_of = fmaxf(most_of, v[j]);
         s.most[u][threadIdx.x] = most_of;
         most = fmaxf(most, most_of);
         r.add(v, most_of, s_powers);
+    };
+    // (loads without a condition, behind the last one that one again: a branch around them, or registers handed on, and the compiler waits for all of them each time)
+    int u = 0;
+    for (; u + kAhead <= whole; u += kAhead) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            sum(u + i, raw[i], std::true_type{});
+            load(raw[i], u + i + kAhead, threadIdx.x);
+        }
     }
-    const float one[1] = {rest_v};
+#pragma unroll
+    for (int i = 0; i + 1 < kAhead; ++i)
+        if (u + i < whole) sum(u + i, raw[i], std::true_type{});
+    if (whole < loads) sum(whole, last, std::false_type{});
+    const float rest_v = has_rest ? static_cast<float>(rest_raw) : none, one[1] = {rest_v};
+    most = fmaxf(most, rest_v);
     if (segment == segments - 1 && wave == 0) r.add(one, rest_v, s_powers);
     r.s = wave_sum(r.s, lane);
     if (lane == 0) s_part[wave] = {r.m, r.e, r.s};
 
     const float bound = bound_of_lanes(most, top, s_candidates, wave, lane);
-    for (int u = 0; u < loads; ++u) {
-        // (of lanes that are not there: -inf)
-        if (!(s.most[u][threadIdx.x] >= bound) || place(u, threadIdx.x) >= vectors) continue;
-        const int at = atomicAdd(&s_count, 1);
-        if (at < kCandidates) s_loads[at] = u << 16 | threadIdx.x;
+    uint32_t hits = 0;
+#pragma unroll
+    for (int u0 = 0; u0 < kMaxLoads; u0 += 4) {
+        if (u0 >= loads) break;
+        float of[4];                                       // (on their way together)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) of[i] = s.most[u0 + i][threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) hits |= static_cast<uint32_t>(of[i] >= bound && u0 + i < loads && place(u0 + i, threadIdx.x) < vectors) << (u0 + i);
+    }
+    if (hits) {
+        for (int at = atomicAdd(&s_count, __popc(hits)); hits; hits &= hits - 1, ++at)
+            if (at < kCandidates) s_loads[at] = static_cast<uint32_t>(__ffs(hits) - 1) << 16 | threadIdx.x;
     }
     auto candidate = [&](float value, uint32_t index) {
         if (!(value >= bound)) return;
@@ -241,12 +271,12 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
     if (has_rest) candidate(rest_v, rest_at);
     __syncthreads();
     const int again = s_count;
-    if (static_cast<int>(threadIdx.x) < again && again <= kCandidates) {
-        const int u = s_loads[threadIdx.x] >> 16, thread = s_loads[threadIdx.x] & 0xffff;
-        Raw<T, V> once_more;
-        load(once_more, u, thread);
-#pragma unroll
-        for (int j = 0; j < V; ++j) candidate(once_more.get(j), static_cast<uint32_t>(place(u, thread) * V + j));
+    // (a lane for each value)
+    if (again <= kCandidates) {
+        for (int i = threadIdx.x; i < again * V; i += kThreads) {
+            const int at = place(static_cast<int>(s_loads[i / V] >> 16), static_cast<int>(s_loads[i / V] & 0xffff)) * V + i % V;
+            candidate(static_cast<float>(logits[at]), static_cast<uint32_t>(at));
+        }
     }
     __syncthreads();
     BeamPart* const parts = static_cast<BeamPart*>(p.workspace);

@@ -30,6 +30,7 @@ constexpr int kSteps = 512;
 constexpr double kLn2Wide = 0.69314718055994531;
 constexpr int kNowhere = 1 << 29;          // below it there is no e of a sum
 __device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 struct WideSum {
     float m;
     int e;
@@ -76,13 +77,15 @@ struct WideSum {
         for (int j = 0; j < B; ++j) power[j] = powers[n[j] & (kSteps - 1)];
 #pragma unroll
         for (int j = 0; j < B; ++j) {
-            // (into the exponent, which stays a normal one)
-            const uint64_t bits = __builtin_bit_cast(uint64_t, power[j]);
-            const uint32_t high = static_cast<uint32_t>(bits >> 32) + (static_cast<uint32_t>(n[j]) << (20 - 9));
-            s = __builtin_fma(value[j], __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(bits)), s);
+            // (into the exponent, which stays a normal one; what the compiler makes of it are five instructions)
+            v2u bits = __builtin_bit_cast(v2u, power[j]);
+            uint32_t high;
+            asm("v_lshl_add_u32 %0, %1, 11, %2" : "=v"(high) : "v"(n[j]), "v"(bits[1]));
+            bits[1] = high;
+            s = __builtin_fma(value[j], __builtin_bit_cast(double, bits), s);
         }
     }
-    static_assert(kSteps == 1 << 9, "the shift into the exponent");
+    static_assert(kSteps == 1 << 9, "the shift into the exponent: 20 - 9");
     // values of which `most` is the largest of this lane's
     template <int B>
     __device__ __forceinline__ void add(const float (&v)[B], float most, const double* powers) {
@@ -148,13 +151,14 @@ __device__ __forceinline__ void fill_powers(double (&powers)[kSteps]) {
 }
 
 typedef uint64_t v2k __attribute__((ext_vector_type(2)));
-// How many of the first `n` keys are larger than one, and as large; up to seven behind them are 0 (which no key that is looked at is).
+// How many of the first `n` keys are larger than one, and as large; up to seven behind them are 0 (which no key that is looked at is).  first, step: some of the
+// eights they are in.
 struct Above {
     int larger, equal;
 };
-__device__ __forceinline__ Above above(const uint64_t* keys, int n, uint64_t own) {
+__device__ __forceinline__ Above above(const uint64_t* keys, int n, uint64_t own, int first = 0, int step = 8) {
     Above a = {0, 0};
-    for (int o = 0; o < n; o += 8) {
+    for (int o = first; o < n; o += step) {
         v2k k[4];                                          // (on their way together)
 #pragma unroll
         for (int i = 0; i < 4; ++i) k[i] = *reinterpret_cast<const v2k*>(keys + o + 2 * i);
@@ -169,7 +173,7 @@ __device__ __forceinline__ Above above(const uint64_t* keys, int n, uint64_t own
 
 // A workgroup has a segment of up to kMaxLoads chunks, one load a lane each; kAhead of them are under way while one is summed.  What each load's largest value is goes to LDS, and
 // when all were seen a bound says which loads have one of the best entries: their values are read once more, a lane each, and what reaches the bound is ranked (each
-// counts the others that are larger).  64 x 8 rows of 50280 bf16, count 16, take 23 us (2.2 TB/s): the loop 18, bound by the vector units (the loads alone 12), and the
+// counts the others that are larger).  64 x 8 rows of 50280 bf16, count 16, take 21 us (2.5 TB/s): the loop 16, bound by the vector units (the loads alone 10), and the
 // selection of the last of a CU's four workgroups, which the others' hide behind their loops.  (Registers handed on from load to load, for which the compiler waits each time,
 // 26; entries kept on the way, as token_logprobs has them, 35; three to five loads ahead the same; six or eight workgroups a CU 26 and 28.)
 constexpr int kAhead = 2;
@@ -214,6 +218,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
     if (has_rest) rest_raw = logits[rest_at];
     fill_powers(s_powers);
     if (threadIdx.x == 0) s_count = 0;
+    static_assert(kCandidates == kThreads, "one each");
+    s_candidates.at[threadIdx.x] = 0;                      // (behind the last candidate none is found)
     __syncthreads();
     WideSum r;
     r.clear();
@@ -281,19 +287,24 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
     __syncthreads();
     BeamPart* const parts = static_cast<BeamPart*>(p.workspace);
     Entry* const out = reinterpret_cast<Entry*>(parts + static_cast<int64_t>(p.batch) * p.beams * segments) + static_cast<int64_t>(blockIdx.x) * top;
-    if (threadIdx.x == 64) parts[blockIdx.x] = joined(joined(s_part[0], s_part[1]), joined(s_part[2], s_part[3]));
+    // (by the last wave, which has the fewest candidates to rank)
+    if (threadIdx.x == kThreads - 64) parts[blockIdx.x] = joined(joined(s_part[0], s_part[1]), joined(s_part[2], s_part[3]));
     static_assert(W == 4, "a sum of each wave");
     const int count = s_candidates.count;
     if (again <= kCandidates && count <= kCandidates - 8) {
-        if (threadIdx.x < 8) s_candidates.at[count + threadIdx.x] = 0;
-        __syncthreads();
-        if (static_cast<int>(threadIdx.x) < count) {
+        if (4 * count <= kThreads) {
+            // four lanes for each, that have every fourth eight of the others
+            const Entry mine = s_candidates.at[threadIdx.x / 4];
+            int before = above(s_candidates.at, count, mine, threadIdx.x % 4 * 8, 32).larger;
+            before += static_cast<int>(lm::across<1>(static_cast<uint32_t>(before), lane));
+            before += static_cast<int>(lm::across<2>(static_cast<uint32_t>(before), lane));
+            if (mine != 0 && threadIdx.x % 4 == 0 && before < top) out[before] = mine;
+        } else if (static_cast<int>(threadIdx.x) < count) {
             const Entry mine = s_candidates.at[threadIdx.x];
             const int before = above(s_candidates.at, count, mine).larger;
             if (before < top) out[before] = mine;
-        } else if (static_cast<int>(threadIdx.x) < top) {
-            out[threadIdx.x] = 0;
         }
+        if (static_cast<int>(threadIdx.x) >= count && static_cast<int>(threadIdx.x) < top) out[threadIdx.x] = 0;
         return;
     }
     // more reach the bound than there is room for - equal values, or as many as lanes are asked for: every wave keeps its own best as it goes through its loads again
@@ -388,6 +399,8 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
         for (int i = 0; i < kEach; ++i) mine[i] = entries[min(item_of(i), all - 1)];
     }
     if (threadIdx.x == 0) s_count = s_further = 0;
+    static_assert(kOffers == kJoinThreads, "one each");
+    s_keys[threadIdx.x] = 0;                               // (behind the last offer none is found)
     if (threadIdx.x < 8) s_keys[kOffers + threadIdx.x] = 0;
     {
         // a power of two of lanes for each beam
@@ -510,8 +523,6 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
     }
     __syncthreads();
     const int offers = s_count;
-    if (offers < kOffers && threadIdx.x < 8) s_keys[offers + threadIdx.x] = 0;
-    __syncthreads();
     const int64_t out = entry * p.count;
     auto write = [&](int place, uint64_t key, int beam, uint32_t token) {
         p.out_scores[out + place] = static_cast<float>(score_of_key(key));

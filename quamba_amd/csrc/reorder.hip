@@ -1,12 +1,12 @@
 // Rows of states in another order, in place (qa_reorder_states).
 //
-// A thread has two units of 16 bytes (4 or 1 where a state does not lie on that) of all the rows of an entry: it reads what its rows are to become and then writes them, so
-// that no row is read after it was written and no copy is needed.  Rows that stay are neither read nor written, and a parent of several
+// A thread has two units of 16 bytes, on any address, of all the rows of an entry, or one of the bytes behind a row's last unit: it reads what its rows are to become and
+// then writes them, so that no row is read after it was written and no copy is needed.  Rows that stay are neither read nor written, and a parent of several
 // rows comes from memory once and from the caches again.  One launch has up to kTensors tensors, with their addresses in its arguments.
 //
 // Bound by memory: 16 rows of 64 layers of 5120 x 16 fp32 states and their conv states, 479 MB of them read or written, take 81 us, 5.9 TB/s (one unit a thread 84).  States
 // that the last-level cache does not hold are written past it (89 us otherwise); those that it holds are read again soon (2 x 16 rows of 32 layers, 151 MB, 37 us, and 46
-// past it).
+// past it).  Rows of 2331 bytes, 256 of them in 64 tensors, take 15.6 us and of 2352 12.2 (a byte a lane 37).
 #include "../../include/quamba_amd_beam.h"
 #include "lm_common.hpp"
 
@@ -22,20 +22,24 @@ struct Tensors {
     uint8_t* data[kTensors];
     int64_t row_stride[kTensors];
     int32_t units[kTensors];           // of a row
+    uint8_t rest[kTensors];            // bytes behind them
     int32_t first[kTensors + 1];       // workgroup of the first unit; behind the last one, all of them
     int32_t count;
 };
 static_assert(sizeof(Tensors) <= 4000, "arguments of a launch: 4 KB");
 
-// units of a thread, as far as the registers go
+// units of a thread, as far as the registers go; their bytes (of more than 32 beams 16 each are more than the registers of two waves)
 template <int BEAMS>
 constexpr int kUnits = BEAMS <= 16 ? 2 : 1;
+template <int BEAMS>
+constexpr int kUnit = BEAMS <= 32 ? 16 : 4;
+typedef uint32_t v4any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t any32 __attribute__((aligned(1)));
 
-// left: units of the row from this thread's first one on
-template <int BEAMS, bool PAST, class U>
+// N units, kThreads apart, of every row; left: how many there are from the first of them on
+template <int N, int BEAMS, bool PAST, class U>
 __device__ __forceinline__ void move_units(uint8_t* base, int64_t row_stride, const int (&from)[BEAMS], int beams, int left) {
-    constexpr int N = kUnits<BEAMS>;
-    U v[BEAMS][N];
+    std::remove_cv_t<U> v[BEAMS][N];
 #pragma unroll
     for (int i = 0; i < BEAMS; ++i)
         if (i < beams && from[i] != i)
@@ -54,8 +58,8 @@ __device__ __forceinline__ void move_units(uint8_t* base, int64_t row_stride, co
                 }
 }
 
-// UNIT: bytes; BEAMS: at least as many as there are; PAST: written past the last-level cache
-template <int BEAMS, int UNIT, bool PAST>
+// BEAMS: at least as many as there are; PAST: written past the last-level cache
+template <int BEAMS, bool PAST>
 __global__ __launch_bounds__(kThreads) void reorder_kernel(Tensors t, const void* parents, int index_bytes, int beams) {
     const int64_t entry = blockIdx.y;
     int from[BEAMS], moved = 0;
@@ -74,24 +78,22 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(Tensors t, const void
         if (t.first[middle] <= static_cast<int>(blockIdx.x)) low = middle;
         else high = middle - 1;
     }
-    const int unit = (static_cast<int>(blockIdx.x) - t.first[low]) * (kThreads * kUnits<BEAMS>) + threadIdx.x;
-    if (unit >= t.units[low]) return;
-    using U = std::conditional_t<UNIT == 16, v4w, std::conditional_t<UNIT == 4, uint32_t, uint8_t>>;
-    move_units<BEAMS, PAST, U>(t.data[low] + entry * beams * t.row_stride[low] + static_cast<int64_t>(unit) * UNIT, t.row_stride[low], from, beams, t.units[low] - unit);
+    constexpr int N = kUnits<BEAMS>, UNIT = kUnit<BEAMS>;
+    static_assert(UNIT <= kThreads, "a thread has one of the bytes at most");
+    const int unit = (static_cast<int>(blockIdx.x) - t.first[low]) * (kThreads * N) + threadIdx.x, units = t.units[low];
+    uint8_t* const rows = t.data[low] + entry * beams * t.row_stride[low];
+    using U = std::conditional_t<UNIT == 16, v4any, any32>;
+    if (unit < units) move_units<N, BEAMS, PAST, U>(rows + static_cast<int64_t>(unit) * UNIT, t.row_stride[low], from, beams, units - unit);
+    const int byte = (unit >= units ? unit : unit + (N - 1) * kThreads) - units;
+    if (byte >= 0 && byte < t.rest[low]) move_units<1, BEAMS, PAST, uint8_t>(rows + static_cast<int64_t>(units) * UNIT + byte, t.row_stride[low], from, beams, 1);
 }
 
-template <int BEAMS, int UNIT>
+template <int BEAMS>
 int launch(const QaReorderParams& p, const Tensors& t, bool past, hipStream_t stream) {
     const dim3 grid(t.first[t.count], p.batch);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, t, p.parents, p.index_bytes, p.beams); };
-    past ? go(reorder_kernel<BEAMS, UNIT, true>) : go(reorder_kernel<BEAMS, UNIT, false>);
+    past ? go(reorder_kernel<BEAMS, true>) : go(reorder_kernel<BEAMS, false>);
     return check_launch();
-}
-
-// (more than 32 beams by 16 bytes are more than the registers of two waves)
-int unit_of(const QaStateRows& s, int beams) {
-    const uint64_t all = reinterpret_cast<uintptr_t>(s.data) | static_cast<uint64_t>(s.row_bytes) | static_cast<uint64_t>(s.row_stride);
-    return all % 16 == 0 && beams <= 32 ? 16 : all % 4 == 0 ? 4 : 1;
 }
 
 }  // namespace
@@ -114,8 +116,7 @@ extern "C" int qa_reorder_states(const QaReorderParams* p, void* stream_) {
         if (s.row_bytes == 0) continue;
         if (!s.data) return QA_ERR_NULL;
         if (s.row_stride < s.row_bytes && static_cast<int64_t>(p->batch) * p->beams > 1) return QA_ERR_STRIDE;
-        const int unit = unit_of(s, p->beams);
-        const int64_t units = unit == 16 ? s.row_bytes / 16 : unit == 4 ? s.row_bytes / 4 : s.row_bytes;
+        const int64_t units = (p->beams <= 32 ? s.row_bytes / 16 : s.row_bytes / 4) + 15;              // (with the bytes behind them)
         if (units > 0x7fffffffLL || !launchable((units + kThreads - 1) / kThreads * p->batch, kThreads)) return QA_ERR_SHAPE;
     }
     if (p->beams == 1) return QA_OK;
@@ -123,33 +124,28 @@ extern "C" int qa_reorder_states(const QaReorderParams* p, void* stream_) {
     int64_t bytes = 0;
     for (int i = 0; i < p->tensors; ++i) bytes += p->states[i].row_bytes * p->batch * p->beams;
     const bool past = bytes >= kCached;
-    auto all_of = [&](auto beams_c, auto unit_c) {
-        constexpr int BEAMS = decltype(beams_c)::value, UNIT = decltype(unit_c)::value, kEach = kThreads * kUnits<BEAMS>;
+    auto of_beams = [&](auto beams_c) {
+        constexpr int BEAMS = decltype(beams_c)::value, UNIT = kUnit<BEAMS>, kEach = kThreads * kUnits<BEAMS>;
         Tensors t = {};
         auto flush = [&] {
-            const int status = t.count ? launch<BEAMS, UNIT>(*p, t, past, static_cast<hipStream_t>(stream_)) : QA_OK;
+            const int status = t.count ? launch<BEAMS>(*p, t, past, static_cast<hipStream_t>(stream_)) : QA_OK;
             t.count = 0;
             return status;
         };
         for (int i = 0; i < p->tensors; ++i) {
             const QaStateRows& s = p->states[i];
-            if (s.row_bytes == 0 || unit_of(s, p->beams) != UNIT) continue;
-            const int64_t units = s.row_bytes / UNIT, workgroups = (units + kEach - 1) / kEach;
+            if (s.row_bytes == 0) continue;
+            const int64_t units = s.row_bytes / UNIT, rest = s.row_bytes % UNIT, workgroups = (units + rest + kEach - 1) / kEach;
             if (t.count == kTensors || !launchable((t.first[t.count] + workgroups) * p->batch, kThreads))
                 if (const int status = flush()) return status;
             t.data[t.count] = static_cast<uint8_t*>(s.data);
             t.row_stride[t.count] = s.row_stride;
             t.units[t.count] = static_cast<int32_t>(units);
+            t.rest[t.count] = static_cast<uint8_t>(rest);
             t.first[t.count + 1] = t.first[t.count] + static_cast<int32_t>(workgroups);
             ++t.count;
         }
         return flush();
-    };
-    auto of_beams = [&](auto beams_c) {
-        if constexpr (decltype(beams_c)::value <= 32)
-            if (const int status = all_of(beams_c, std::integral_constant<int, 16>{})) return status;
-        if (const int status = all_of(beams_c, std::integral_constant<int, 4>{})) return status;
-        return all_of(beams_c, std::integral_constant<int, 1>{});
     };
     if (p->beams <= 4) return of_beams(std::integral_constant<int, 4>{});
     if (p->beams <= 8) return of_beams(std::integral_constant<int, 8>{});

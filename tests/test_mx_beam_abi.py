@@ -157,7 +157,7 @@ def test_reorder_refusals():
     assert l.qa_reorder_states(C.byref(p), None) == -1
     p.states = rows
     for fields, status in ((dict(data=0), -1), (dict(row_bytes=-1), -2), (dict(row_stride=255), -3), (dict(row_stride=-256), -3), (dict(row_bytes=1 << 40, row_stride=1 << 40), -2),
-                           (dict(row_bytes=(1 << 31) + 1, row_stride=1 << 32), -2)):
+                           (dict(row_bytes=(1 << 35) + 1, row_stride=1 << 36), -2)):
         for k, v in fields.items():
             setattr(rows[1], k, v)
         assert l.qa_reorder_states(C.byref(p), None) == status, (fields, status)

@@ -164,3 +164,17 @@ def test_captured_and_on_another_stream(dev):
         ops.reorder_states(states, parents)
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(states, want))
+
+
+@pytest.mark.parametrize("beams", [3, 12, 24, 40])
+def test_bytes_of_a_row(dev, beams):
+    """rows of any number of bytes on any address, next to bytes that are nobody's"""
+    g = torch.Generator().manual_seed(beams)
+    for length in (1, 3, 4, 15, 16, 17, 31, 1023, 1024 + 3, 16 * 255 + 15, 16 * 256, 16 * 256 + 1, 16 * 257 + 7, 16 * 511 + 15, 16 * 512, 16 * 512 + 15, 16 * 513 + 1, 30011):
+        for at in (0, 1, 6):
+            buffer = torch.randint(-100, 100, (2 * beams, length + 9), dtype=torch.int8, generator=g).to(dev)
+            parents = torch.randint(-1, beams, (2, beams), generator=g).to(dev)
+            want = buffer.clone()
+            want[:, at:at + length] = reference([buffer[:, at:at + length]], parents)[0]
+            ops.reorder_states(buffer[:, at:at + length], parents)
+            assert torch.equal(buffer, want), (length, at)

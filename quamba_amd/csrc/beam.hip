@@ -171,6 +171,18 @@ __device__ __forceinline__ Above above(const uint64_t* keys, int n, uint64_t own
     return a;
 }
 
+// f(i, sub, lanes) for each of `count` things by four lanes, two or one, as many as there are; sums over them
+template <class F>
+__device__ __forceinline__ void by_lanes(int count, int threads, F&& f) {
+    const int lanes = 4 * count <= threads ? 4 : 2 * count <= threads ? 2 : 1, i = threadIdx.x / lanes;
+    if (threadIdx.x / 64 * 64 / lanes < static_cast<unsigned>(count)) f(i, static_cast<int>(threadIdx.x % lanes), lanes);
+}
+__device__ __forceinline__ int over_lanes(int v, int lanes, int lane) {
+    if (lanes >= 2) v += static_cast<int>(lm::across<1>(static_cast<uint32_t>(v), lane));
+    if (lanes >= 4) v += static_cast<int>(lm::across<2>(static_cast<uint32_t>(v), lane));
+    return v;
+}
+
 // A workgroup has a segment of up to kMaxLoads chunks, one load a lane each; kAhead of them are under way while one is summed.  What each load's largest value is goes to LDS, and
 // when all were seen a bound says which loads have one of the best entries: their values are read once more, a lane each, and what reaches the bound is ranked (each
 // counts the others that are larger).  64 x 8 rows of 50280 bf16, count 16, take 21 us (2.5 TB/s): the loop 16, bound by the vector units (the loads alone 10), and the
@@ -292,18 +304,11 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
     static_assert(W == 4, "a sum of each wave");
     const int count = s_candidates.count;
     if (again <= kCandidates && count <= kCandidates - 8) {
-        if (4 * count <= kThreads) {
-            // four lanes for each, that have every fourth eight of the others
-            const Entry mine = s_candidates.at[threadIdx.x / 4];
-            int before = above(s_candidates.at, count, mine, threadIdx.x % 4 * 8, 32).larger;
-            before += static_cast<int>(lm::across<1>(static_cast<uint32_t>(before), lane));
-            before += static_cast<int>(lm::across<2>(static_cast<uint32_t>(before), lane));
-            if (mine != 0 && threadIdx.x % 4 == 0 && before < top) out[before] = mine;
-        } else if (static_cast<int>(threadIdx.x) < count) {
-            const Entry mine = s_candidates.at[threadIdx.x];
-            const int before = above(s_candidates.at, count, mine).larger;
-            if (before < top) out[before] = mine;
-        }
+        by_lanes(count, kThreads, [&](int i, int sub, int lanes) {
+            const Entry mine = s_candidates.at[i];
+            const int before = over_lanes(above(s_candidates.at, count, mine, sub * 8, lanes * 8).larger, lanes, lane);
+            if (mine != 0 && sub == 0 && before < top) out[before] = mine;
+        });
         if (static_cast<int>(threadIdx.x) >= count && static_cast<int>(threadIdx.x) < top) out[threadIdx.x] = 0;
         return;
     }
@@ -366,10 +371,10 @@ __device__ __forceinline__ uint64_t bound_of_keys(uint64_t mine, int count, uint
 // An entry of the batch.  The lanes are shared out among the beams and join their segments' sums; meanwhile the lists are on their way.  Up to kKept entries, four a lane,
 // get their scores' keys at once: a bound, the `count`-th largest of what the lanes have best, leaves about as many offers, and those are ranked, each counting the
 // others that are larger.  Of more than that the first entry of each list alone says whether any of it counts: a bound that `count` firsts reach leaves
-// about as many lists, and a second one over their entries about as many offers.  (us of this launch for 4 beams of 25 segments, count 8, and 5 of 63, count 10: 5.6 and
-// 9.0; lists first for both 7.6 and 9.3, all entries first, 13 a lane, 10.5 for the second; all entries sorted, 64 at a time, 8 and 26.)  What is left are some ten
-// waits, for memory and for LDS, one after the other.  Where more reach the bounds than there is room for - equal scores, or as many places as lanes - each
-// wave sorts what its lanes have.
+// about as many lists, and a second one over their entries, a wave four lists at a time, about as many offers.  (us of this launch: 4 beams of 25 segments, count 8, 5.5,
+// lists first 7.6; 5 of 63, count 10, 8.9, all entries first, 13 a lane, 10.5; 30 of 28, count 60, 19, the lists' entries one after the other 27; all entries sorted, 64 at a
+// time, 8 and 26 for the first two.)  What is left are some ten waits, for memory and for LDS, one after the other.  Where more reach the bounds than there is room
+// for - equal scores, or as many places as lanes - each wave sorts what its lanes have.
 constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kOffers = 256, kFew = 48, kEach = 4, kKept = kEach * kJoinThreads;
 __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchParams p, int top, int segments) {
     static_assert(kMaxSegments <= 64 && kMaxTop <= 64, "a lane for each");
@@ -377,8 +382,8 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
     __shared__ uint8_t s_done[kMaxBeams], s_beam[kOffers];
     __shared__ __attribute__((aligned(16))) uint64_t s_keys[kOffers + 8];
     __shared__ uint32_t s_at[kOffers], s_token[kOffers];
-    __shared__ uint64_t s_item_keys[kKept];                // in the order of the lanes
-    __shared__ uint32_t s_item_tokens[kKept];
+    __shared__ uint64_t s_slot_keys[kMaxBeams * kMaxSegments];     // in the order of the lanes: of entries, or of the first ones of lists
+    __shared__ uint32_t s_slot_tokens[kKept];
     __shared__ uint16_t s_lists[kMaxBeams * kMaxSegments];
     __shared__ Offer s_sorted[kJoinWaves][64];
     __shared__ uint32_t s_bounds[kJoinWaves][64];
@@ -391,13 +396,15 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
     const int lists = p.beams * segments;
     const int all = lists * top;
     const bool kept = all <= kKept;
-    // this lane's entries: four lanes next to each other have them far apart, so that what a list begins with is in groups of its own
-    auto item_of = [&](int j) { return static_cast<int>(j * kJoinThreads + (threadIdx.x & 3) * (kJoinThreads / 4) + (threadIdx.x >> 2)); };
+    const int slots = kept ? all : lists;
+    // the entry of this lane's slot j
+    auto entry_at = [&](int j) { return static_cast<int>(j * kJoinThreads + threadIdx.x) * (kept ? 1 : top); };
     Entry mine[kEach];                                     // (on their way meanwhile)
-    if (kept) {
+    auto fetch = [&](int first) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) mine[i] = entries[min(item_of(i), all - 1)];
-    }
+        for (int i = 0; i < kEach; ++i) mine[i] = entries[min(entry_at(first + i), all - 1)];
+    };
+    fetch(0);
     if (threadIdx.x == 0) s_count = s_further = 0;
     static_assert(kOffers == kJoinThreads, "one each");
     s_keys[threadIdx.x] = 0;                               // (behind the last offer none is found)
@@ -438,88 +445,84 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
         }
     }
     __syncthreads();
-    // the key of the score of a list's entry; 0: no offer
-    auto key_at = [&](int list, int place, Entry e) -> uint64_t {
-        const int beam = list / segments;
-        const double rest = s_rest[beam];
-        if (!(rest > -__builtin_inf())) return 0;
-        if (s_done[beam]) return place == 0 && list == beam * segments ? key_of_score(rest) : 0;
+    const int of_beam = segments * top;
+    const float per = 1.0f / static_cast<float>(of_beam);
+    // (half an entry from a whole number of beams at least, 1 / 8192 of one: the product's error is far below that)
+    auto beam_of = [&](int at) { return static_cast<int>((static_cast<float>(at) + 0.5f) * per); };
+    // the key of an entry's score; 0: no offer
+    auto key_of = [&](int at, Entry e, bool there) __attribute__((always_inline)) -> uint64_t {
+        const int beam = beam_of(min(at, all - 1));
+        const double rest = s_rest[beam], base = s_base[beam];
+        const bool done = s_done[beam];
         const float logit = value_of(e);
+        const bool offers = there & (rest > -__builtin_inf()) & (done ? at == beam * of_beam : (e != 0) & (logit > -__builtin_inff()));
         // (the difference first: next to a mask of -3e38 nothing else is left of the sum)
-        return e != 0 && logit > -__builtin_inff() ? key_of_score(rest + (static_cast<double>(logit) - s_base[beam])) : 0;
+        const double score = rest + (done ? 0.0 : static_cast<double>(logit) - base);
+        return offers ? key_of_score(score) : 0;
     };
-    auto offer = [&](int at, int beam, uint64_t key, uint32_t token) {
+    auto offer = [&](int at, uint64_t key, uint32_t token) {
         const int place = atomicAdd(&s_count, 1);
         if (place >= kOffers) return;
         s_keys[place] = key;
         s_at[place] = ~static_cast<uint32_t>(at);
-        s_beam[place] = static_cast<uint8_t>(beam);
+        s_beam[place] = static_cast<uint8_t>(beam_of(at));
         s_token[place] = token;
     };
     uint64_t best_key = 0, bound = 0;
     int further = lists;                                   // lists that are looked at
+    for (int first = 0; first * kJoinThreads < slots; first += kEach) {
+        if (first > 0) fetch(first);
+        uint64_t key[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) key[i] = key_of(entry_at(first + i), mine[i], entry_at(first + i) < all);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            s_slot_keys[(first + i) * kJoinThreads + threadIdx.x] = key[i];
+            best_key = key[i] > best_key ? key[i] : best_key;
+            if (kept) s_slot_tokens[(first + i) * kJoinThreads + threadIdx.x] = index_of(mine[i]);
+        }
+    }
+    if (slots > kFew) bound = bound_of_keys(best_key, p.count, s_bounds, wave, lane);
+    auto each_slot = [&](auto&& f) __attribute__((always_inline)) {
+        for (int j = 0; j * kJoinThreads < slots; ++j) {
+            const uint64_t key = s_slot_keys[j * kJoinThreads + threadIdx.x];
+            if (key != 0 && key >= bound) f(j, key);
+        }
+    };
     if (kept) {
-        const int of_beam = segments * top;
-        const float per = 1.0f / static_cast<float>(of_beam);
-        // (half a place from a whole number of beams at least: the product's error is far below that)
-        static_assert(kKept <= 1 << 12, "the quotient by a product in 32 bits");
-        auto beam_of = [&](int at) { return static_cast<int>((static_cast<float>(at) + 0.5f) * per); };
-        double rest[kEach], base[kEach];
-        bool done[kEach];
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int beam = beam_of(min(item_of(i), all - 1));
-            rest[i] = s_rest[beam];
-            base[i] = s_base[beam];
-            done[i] = s_done[beam];
-        }
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            // (key_at without a branch)
-            const int at = item_of(i);
-            const float logit = value_of(mine[i]);
-            const bool of_done = at == beam_of(at) * of_beam, of_logit = (mine[i] != 0) & (logit > -__builtin_inff());
-            const bool offers = (at < all) & (rest[i] > -__builtin_inf()) & (done[i] ? of_done : of_logit);
-            const double score = rest[i] + (done[i] ? 0.0 : static_cast<double>(logit) - base[i]);
-            const uint64_t key = offers ? key_of_score(score) : 0;
-            s_item_keys[i * kJoinThreads + threadIdx.x] = key;
-            s_item_tokens[i * kJoinThreads + threadIdx.x] = index_of(mine[i]);
-            best_key = key > best_key ? key : best_key;
-        }
-        if (all > kFew) bound = bound_of_keys(best_key, p.count, s_bounds, wave, lane);
-        for (int j = 0; j * kJoinThreads < all; ++j) {
-            const uint64_t key = s_item_keys[j * kJoinThreads + threadIdx.x];
-            if (key != 0 && key >= bound) offer(item_of(j), beam_of(item_of(j)), key, s_item_tokens[j * kJoinThreads + threadIdx.x]);
-        }
+        each_slot([&](int j, uint64_t key) { offer(entry_at(j), key, s_slot_tokens[j * kJoinThreads + threadIdx.x]); });
     } else {
-        auto each_list = [&](auto&& f) __attribute__((always_inline)) {
-            for (int list = threadIdx.x; list < lists; list += kJoinThreads) {
-                const Entry e = entries[list * top];
-                const uint64_t key = key_at(list, 0, e);
-                if (key != 0 && key >= bound) f(list, key, e);
-            }
-        };
-        const auto better = [&](int, uint64_t key, Entry) { best_key = key > best_key ? key : best_key; };
-        each_list(better);
-        bound = bound_of_keys(best_key, p.count, s_bounds, wave, lane);
-        each_list([&](int list, uint64_t, Entry) { s_lists[atomicAdd(&s_further, 1)] = static_cast<uint16_t>(list); });
+        each_slot([&](int j, uint64_t) { s_lists[atomicAdd(&s_further, 1)] = static_cast<uint16_t>(j * kJoinThreads + threadIdx.x); });
         __syncthreads();
         further = s_further;
-        auto each_item = [&](auto&& f) __attribute__((always_inline)) {
-            for (int i = threadIdx.x; i < further * top; i += kJoinThreads) {
-                const int list = s_lists[i / top], at = list * top + i % top;
-                const Entry e = entries[at];
-                const uint64_t key = key_at(list, i % top, e);
-                if (key != 0 && key >= bound) f(at, key, e);
+        // a wave has four lists at a time, their entries from another lane on in each: what they begin with is no lane's alone
+        auto each_entry = [&](auto&& f) __attribute__((always_inline)) {
+            for (int first = wave * kEach; first < further; first += kJoinWaves * kEach) {
+                Entry e[kEach];
+                int at[kEach];
+                bool there[kEach];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int l = min(first + i, further - 1), place = (lane + 17 * l) & 63;
+                    there[i] = (first + i < further) & (place < top);
+                    at[i] = s_lists[l] * top + min(place, top - 1);
+                    e[i] = entries[at[i]];
+                }
+                uint64_t key[kEach];                       // (all of them, then what comes of them: their reads are on their way together)
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) key[i] = key_of(at[i], e[i], there[i]);
+#pragma unroll
+                for (int i = 0; i < kEach; ++i)
+                    if (key[i] != 0 && key[i] >= bound) f(at[i], key[i], e[i]);
             }
         };
         if (further * top > kFew) {
             best_key = 0;
-            each_item(better);
+            each_entry([&](int, uint64_t key, Entry) { best_key = key > best_key ? key : best_key; });
             const uint64_t closer = bound_of_keys(best_key, p.count, s_bounds, wave, lane);
             bound = closer > bound ? closer : bound;
         }
-        each_item([&](int at, uint64_t key, Entry e) { offer(at, at / top / segments, key, index_of(e)); });
+        each_entry([&](int at, uint64_t key, Entry e) { offer(at, key, index_of(e)); });
     }
     __syncthreads();
     const int offers = s_count;
@@ -535,17 +538,19 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
         p.parents[out + place] = -1;
     };
     if (offers <= kOffers) {
-        if (static_cast<int>(threadIdx.x) < offers) {
-            const uint64_t key = s_keys[threadIdx.x];
-            const uint32_t at = s_at[threadIdx.x];
-            const Above a = above(s_keys, offers, key);
-            int place = a.larger;
-            if (a.equal > 1)
-                for (int n = 0; n < offers; ++n) place += s_keys[n] == key && s_at[n] > at;
-            if (place < p.count) write(place, key, s_beam[threadIdx.x], s_token[threadIdx.x]);
-        } else if (static_cast<int>(threadIdx.x) < p.count) {
-            leave(threadIdx.x);
-        }
+        by_lanes(offers, kJoinThreads, [&](int i, int sub, int lanes) {
+            const uint64_t key = s_keys[i];
+            const Above a = above(s_keys, offers, key, sub * 8, lanes * 8);
+            int place = over_lanes(a.larger, lanes, lane);
+            if (over_lanes(a.equal, lanes, lane) > 1 && i < offers) {
+                const uint32_t at = s_at[i];
+                int first = 0;
+                for (int n = sub; n < offers; n += lanes) first += s_keys[n] == key && s_at[n] > at;
+                place += over_lanes(first, lanes, lane);
+            }
+            if (i < offers && sub == 0 && place < p.count) write(place, key, s_beam[i], s_token[i]);
+        });
+        if (static_cast<int>(threadIdx.x) >= offers && static_cast<int>(threadIdx.x) < p.count) leave(threadIdx.x);
         return;
     }
     Offer best = {0, 0};
@@ -553,7 +558,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
         Offer o = {0, 0};
         if (i + lane < further * top) {
             const int list = kept ? (i + lane) / top : s_lists[(i + lane) / top], place = (i + lane) % top;
-            const uint64_t key = key_at(list, place, entries[list * top + place]);
+            const uint64_t key = key_of(list * top + place, entries[list * top + place], true);
             if (key != 0) o = {key, ~static_cast<uint32_t>(list * top + place)};
         }
         if (__builtin_amdgcn_ballot_w64(o.key != 0 && o.key >= bound)) best = merge_waves(best, sort_wave(o, lane), lane);

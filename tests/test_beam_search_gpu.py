@@ -321,3 +321,21 @@ def test_offsets_past_32_bits(dev):
     got = ops.beam_search_step(logits, torch.zeros(batch, 1, device=dev), 2)
     for i, b in enumerate(some):
         assert got.tokens[b].tolist() == [100 * i + 7, vocab - 1 - i]
+
+
+@pytest.mark.parametrize("batch,beams,vocab,count", [(1, 24, 40000, 64), (2, 30, 70001, 60), (1, 64, 20000, 33)])
+def test_many_beams(dev, batch, beams, vocab, count):
+    """equal logits, one beam above all others, half of the beams done or not there"""
+    g = torch.Generator().manual_seed(vocab)
+    mixed = torch.randint(0, 5, (vocab,), generator=g).half().to(dev).expand(batch, beams, vocab).contiguous()
+    check(mixed, torch.zeros(batch, beams, device=dev), count)
+    logits, scores = make(batch, beams, vocab, "fp32", dev)
+    scores = torch.linspace(-40, -30, beams, device=dev).expand(batch, beams).clone()
+    scores[:, beams // 2] = 25.0
+    check(logits, scores, count)
+    scores[:, beams // 2] = -31.7
+    scores[:, ::3] = float("-inf")
+    done = torch.zeros(batch, beams, dtype=torch.bool, device=dev)
+    done[:, 1::4] = True
+    check(logits, scores, count, done)
+    check(logits, scores, 1, done)

@@ -1,7 +1,7 @@
 // The best continuations over the beams and the vocabulary (qa_beam_search_step).
 //
 // Two launches: every row of logits, cut into segments, leaves for each segment the sum of its exponentials and its best `count` entries by logit; then a
-// workgroup for each entry of the batch joins the sums of its beams, turns the entries into scores and sorts those that reach a bound.
+// workgroup for each entry of the batch joins the sums of its beams, turns the entries into scores and ranks those that reach a bound.
 //
 // Scores of different beams are compared, and which of two comes first is an answer in whole numbers.  So the sums are held in 64 bits and their terms are good to
 // some 1e-10: e^d is 2^(n / 512) from a table by e^r, |r| <= ln 2 / 1024, from a polynomial whose first missing term is r^3 / 6 < 6e-11.  Operations in 64 bits take 5.4

@@ -7,7 +7,8 @@
 // each fragment while the two tiles last.
 //
 // Register-only loops of this instruction reach 7.0 PFLOP/s with random operands (9.0 with zeros: the clock follows the power) and those of 32x32x64 6.5
-// (9.5).
+// (9.5).  8192 x 10240 x 2560 takes 98 us, 4.4 PFLOP/s, and 125 where the power leaves a lower clock: the main loop 1.82 us a k tile of 256 x 256 outputs against 1.15 on
+// registers alone (LDS busy for more than half of it), the outputs 18 in all.  64 x 50280 x 2560 takes 13.5 us, its bytes at 5.5 TB/s.
 #include "gemm_core.hpp"
 #include "mx_gemm.hpp"
 

@@ -267,7 +267,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
     if (lane == 0) s_part[wave] = {r.m, r.e, r.s};
 
     const float bound = bound_of_lanes(most, top, s_candidates, wave, lane);
-    uint32_t hits = 0;
+    // (of chunks that are there, in bits)
+    uint32_t hits = 0, there = (1u << max(loads, 0)) - 1;
+    if (whole < loads && place(whole, threadIdx.x) >= vectors) there &= ~(1u << whole);
+    static_assert(kMaxLoads <= 16, "bits, and five planes of their number");
 #pragma unroll
     for (int u0 = 0; u0 < kMaxLoads; u0 += 4) {
         if (u0 >= loads) break;
@@ -275,10 +278,22 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
 #pragma unroll
         for (int i = 0; i < 4; ++i) of[i] = s.most[u0 + i][threadIdx.x];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) hits |= static_cast<uint32_t>(of[i] >= bound && u0 + i < loads && place(u0 + i, threadIdx.x) < vectors) << (u0 + i);
+        for (int i = 0; i < 4; ++i) hits |= of[i] >= bound ? 1u << (u0 + i) : 0u;
     }
-    if (hits) {
-        for (int at = atomicAdd(&s_count, __popc(hits)); hits; hits &= hits - 1, ++at)
+    hits &= there;
+    // (places for the wave's by one atomic; the compiler would go through the lanes one by one)
+    int in_wave = 0, before = 0;
+#pragma unroll
+    for (int plane = 0; plane < 5; ++plane) {
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(__popc(hits) >> plane & 1);
+        in_wave += __popcll(lanes) << plane;
+        before += static_cast<int>(__builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0))) << plane;
+    }
+    if (in_wave > 0) {
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&s_count, in_wave);
+        at = __builtin_amdgcn_readfirstlane(at) + before;
+        for (; hits; hits &= hits - 1, ++at)
             if (at < kCandidates) s_loads[at] = static_cast<uint32_t>(__ffs(hits) - 1) << 16 | threadIdx.x;
     }
     auto candidate = [&](float value, uint32_t index) {
@@ -372,17 +387,18 @@ __device__ __forceinline__ uint64_t bound_of_keys(uint64_t mine, int count, uint
 // get their scores' keys at once: a bound, the `count`-th largest of what the lanes have best, leaves about as many offers, and those are ranked, each counting the
 // others that are larger.  Of more than that the first entry of each list alone says whether any of it counts: a bound that `count` firsts reach leaves
 // about as many lists, and a second one over their entries, a wave four lists at a time, about as many offers.  (us of this launch: 4 beams of 25 segments, count 8, 5.5,
-// lists first 7.6; 5 of 63, count 10, 8.9, all entries first, 13 a lane, 10.5; 30 of 28, count 60, 19, the lists' entries one after the other 27; all entries sorted, 64 at a
-// time, 8 and 26 for the first two.)  What is left are some ten waits, for memory and for LDS, one after the other.  Where more reach the bounds than there is room
+// lists first 7.6; 5 of 63, count 10, 8.3, all entries first, 13 a lane, 10.5; 30 of 28, count 60, 18, the lists' entries one after the other 27; all entries sorted, 64 at a
+// time, 8 and 26 for the first two; a wave eight or sixteen lists at a time 9 and 10.5 for the second.)  What is left are some ten waits, for memory and for LDS, one after the other.  Where more reach the bounds than there is room
 // for - equal scores, or as many places as lanes - each wave sorts what its lanes have.
 constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kOffers = 256, kFew = 48, kEach = 4, kKept = kEach * kJoinThreads;
+constexpr int kSlots = kMaxBeams * kMaxSegments + 1024;
 __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchParams p, int top, int segments) {
     static_assert(kMaxSegments <= 64 && kMaxTop <= 64, "a lane for each");
     __shared__ double s_rest[kMaxBeams], s_base[kMaxBeams];        // of a beam: own score - ln s, -inf: it offers nothing; m + e ln 2
     __shared__ uint8_t s_done[kMaxBeams], s_beam[kOffers];
     __shared__ __attribute__((aligned(16))) uint64_t s_keys[kOffers + 8];
     __shared__ uint32_t s_at[kOffers], s_token[kOffers];
-    __shared__ uint64_t s_slot_keys[kMaxBeams * kMaxSegments];     // in the order of the lanes: of entries, or of the first ones of lists
+    __shared__ uint64_t s_slot_keys[kSlots];               // of this lane's entries or of the first ones of lists; of all entries of lists
     __shared__ uint32_t s_slot_tokens[kKept];
     __shared__ uint16_t s_lists[kMaxBeams * kMaxSegments];
     __shared__ Offer s_sorted[kJoinWaves][64];
@@ -499,12 +515,13 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
         auto each_entry = [&](auto&& f) __attribute__((always_inline)) {
             for (int first = wave * kEach; first < further; first += kJoinWaves * kEach) {
                 Entry e[kEach];
-                int at[kEach];
+                int at[kEach], slot[kEach];
                 bool there[kEach];
 #pragma unroll
                 for (int i = 0; i < kEach; ++i) {
                     const int l = min(first + i, further - 1), place = (lane + 17 * l) & 63;
                     there[i] = (first + i < further) & (place < top);
+                    slot[i] = l * top + min(place, top - 1);
                     at[i] = s_lists[l] * top + min(place, top - 1);
                     e[i] = entries[at[i]];
                 }
@@ -513,16 +530,31 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
                 for (int i = 0; i < kEach; ++i) key[i] = key_of(at[i], e[i], there[i]);
 #pragma unroll
                 for (int i = 0; i < kEach; ++i)
-                    if (key[i] != 0 && key[i] >= bound) f(at[i], key[i], e[i]);
+                    if (there[i]) f(slot[i], at[i], key[i], e[i]);
             }
         };
-        if (further * top > kFew) {
-            best_key = 0;
-            each_entry([&](int, uint64_t key, Entry) { best_key = key > best_key ? key : best_key; });
-            const uint64_t closer = bound_of_keys(best_key, p.count, s_bounds, wave, lane);
-            bound = closer > bound ? closer : bound;
+        // their keys take the place of the lists', if there is room for all
+        const int items = further * top;
+        const bool room = items <= kSlots;
+        best_key = 0;
+        each_entry([&](int slot, int, uint64_t key, Entry) {
+            best_key = key > best_key ? key : best_key;
+            if (room) s_slot_keys[slot] = key;
+        });
+        const uint64_t closer = bound_of_keys(best_key, p.count, s_bounds, wave, lane);
+        bound = closer > bound ? closer : bound;
+        if (room) {
+            for (int i = threadIdx.x; i < items; i += kJoinThreads) {
+                const uint64_t key = s_slot_keys[i];
+                if (key == 0 || key < bound) continue;
+                const int at = s_lists[i / top] * top + i % top;
+                offer(at, key, index_of(entries[at]));
+            }
+        } else {
+            each_entry([&](int, int at, uint64_t key, Entry e) {
+                if (key != 0 && key >= bound) offer(at, key, index_of(e));
+            });
         }
-        each_entry([&](int at, uint64_t key, Entry e) { offer(at, key, index_of(e)); });
     }
     __syncthreads();
     const int offers = s_count;

@@ -59,7 +59,7 @@ struct WideSum {
         // (1.5 * 2^52: the rounded multiple of a step is in the low word; less the steps of 2^e)
         round = 6755399441055744.0 - static_cast<double>(e) * kSteps;
     }
-    // e^d, d from -700 to kReach + some (a NaN stays one), added for B values d = v - m; powers as fill_powers leaves them.  In steps, so that the reads of the table are on
+    // e^d, d from -700 to kReach + some (a NaN stays one), added for B values d = v - m; powers those of kPowers.  In steps, so that the reads of the table are on
     // their way together: one after the other they took 130 cycles a value, most of it waiting.
     template <int B>
     __device__ __forceinline__ void add_exponentials(const double (&d)[B], const double* powers) {
@@ -144,11 +144,24 @@ __device__ __forceinline__ double wave_sum(double s, int lane) {
     return s;
 }
 
-// powers[i] = 2^(i / kSteps), less i steps in the exponent's place: n steps added there, whatever n, make 2^(n / kSteps) of powers[n mod kSteps]
-__device__ __forceinline__ void fill_powers(double (&powers)[kSteps]) {
-    for (int i = threadIdx.x; i < kSteps; i += blockDim.x)
-        powers[i] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, exp2(static_cast<double>(i) / kSteps)) - (static_cast<uint64_t>(i) << (52 - 9)));
+// powers[i] = 2^(i / kSteps), less i steps in the exponent's place: n steps added there, whatever n, make 2^(n / kSteps) of powers[n mod kSteps].  (Worked out by each
+// workgroup they were half of the instructions of a row of 1000 values.)
+struct Powers {
+    uint64_t bits[kSteps];
+};
+constexpr Powers make_powers() {
+    // 2^(1/2), 2^(1/4) .. 2^(1/512): products of nine of them are off by 1e-15
+    constexpr double roots[9] = {1.4142135623730951, 1.189207115002721, 1.0905077326652577, 1.0442737824274138, 1.0218971486541166, 1.0108892860517005, 1.0054299011128027, 1.0027112750502025, 1.0013547198921082};
+    Powers p = {};
+    for (int i = 0; i < kSteps; ++i) {
+        double v = 1.0;
+        for (int b = 0; b < 9; ++b)
+            if (i >> (8 - b) & 1) v *= roots[b];
+        p.bits[i] = __builtin_bit_cast(uint64_t, v) - (static_cast<uint64_t>(i) << (52 - 9));
+    }
+    return p;
 }
+__device__ constexpr Powers kPowers = make_powers();
 
 typedef uint64_t v2k __attribute__((ext_vector_type(2)));
 // How many of the first `n` keys are larger than one, and as large; up to seven behind them are 0 (which no key that is looked at is).  first, step: some of the
@@ -205,6 +218,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
     __shared__ int s_count;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x / segments, segment = blockIdx.x % segments, entry = row / p.beams, beam = row % p.beams;
+    static_assert(kSteps == 2 * kThreads, "two each");
+    const uint64_t powers[2] = {kPowers.bits[2 * threadIdx.x], kPowers.bits[2 * threadIdx.x + 1]};
     if (p.done && p.done[row]) return;                     // (its part is not looked at)
     const T* const logits = static_cast<const T*>(p.logits) + entry * p.logits_batch_stride + beam * p.logits_beam_stride;
     const int vectors = p.vocab / V, rest = p.vocab - vectors * V;
@@ -228,7 +243,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
     const bool has_rest = segment == segments - 1 && wave == 0 && lane < rest;
     T rest_raw = static_cast<T>(0.0f);
     if (has_rest) rest_raw = logits[rest_at];
-    fill_powers(s_powers);
+    s_powers[2 * threadIdx.x] = __builtin_bit_cast(double, powers[0]);
+    s_powers[2 * threadIdx.x + 1] = __builtin_bit_cast(double, powers[1]);
     if (threadIdx.x == 0) s_count = 0;
     static_assert(kCandidates == kThreads, "one each");
     s_candidates.at[threadIdx.x] = 0;                      // (behind the last candidate none is found)
@@ -392,15 +408,17 @@ __device__ __forceinline__ uint64_t bound_of_keys(uint64_t mine, int count, uint
 // for - equal scores, or as many places as lanes - each wave sorts what its lanes have.
 constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kOffers = 256, kFew = 48, kEach = 4, kKept = kEach * kJoinThreads;
 constexpr int kSlots = kMaxBeams * kMaxSegments + 1024;
+constexpr int join_lds(int entries) { return entries <= kKept ? kKept * 12 : kSlots * 8 + kMaxBeams * kMaxSegments * 2; }
 __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchParams p, int top, int segments) {
     static_assert(kMaxSegments <= 64 && kMaxTop <= 64, "a lane for each");
     __shared__ double s_rest[kMaxBeams], s_base[kMaxBeams];        // of a beam: own score - ln s, -inf: it offers nothing; m + e ln 2
     __shared__ uint8_t s_done[kMaxBeams], s_beam[kOffers];
     __shared__ __attribute__((aligned(16))) uint64_t s_keys[kOffers + 8];
     __shared__ uint32_t s_at[kOffers], s_token[kOffers];
-    __shared__ uint64_t s_slot_keys[kSlots];               // of this lane's entries or of the first ones of lists; of all entries of lists
-    __shared__ uint32_t s_slot_tokens[kKept];
-    __shared__ uint16_t s_lists[kMaxBeams * kMaxSegments];
+    // keys of this lane's entries and their tokens; or keys of the first ones of lists, then of all entries of lists, and the lists
+    extern __shared__ uint64_t s_slot_keys[];
+    uint32_t* const s_slot_tokens = reinterpret_cast<uint32_t*>(s_slot_keys + kKept);
+    uint16_t* const s_lists = reinterpret_cast<uint16_t*>(s_slot_keys + kSlots);
     __shared__ Offer s_sorted[kJoinWaves][64];
     __shared__ uint32_t s_bounds[kJoinWaves][64];
     __shared__ int s_count, s_further;
@@ -411,7 +429,7 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
                                  entry * p.beams * segments * top;
     const int lists = p.beams * segments;
     const int all = lists * top;
-    const bool kept = all <= kKept;
+    const bool kept = all <= kKept;                        // (join_lds)
     const int slots = kept ? all : lists;
     // the entry of this lane's slot j
     auto entry_at = [&](int j) { return static_cast<int>(j * kJoinThreads + threadIdx.x) * (kept ? 1 : top); };
@@ -637,7 +655,7 @@ int launch(const QaBeamSearchParams& p, hipStream_t stream) {
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, top, cut.segments, cut.each); };
     wide ? go(beam_rows_kernel<T, true>) : go(beam_rows_kernel<T, false>);
     if (const int status = check_launch()) return status;
-    hipLaunchKernelGGL(beam_join_kernel, dim3(p.batch), dim3(kJoinThreads), 0, stream, p, top, cut.segments);
+    hipLaunchKernelGGL(beam_join_kernel, dim3(p.batch), dim3(kJoinThreads), join_lds(p.beams * cut.segments * top), stream, p, top, cut.segments);
     return check_launch();
 }
 

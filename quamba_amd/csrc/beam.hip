@@ -230,14 +230,14 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
     auto place = [&](int u, int thread) { return (first + u) * kThreads + thread; };
     const T* const from = vectors ? logits : static_cast<const T*>(p.workspace);           // (something to load, if for nothing)
     auto load = [&](Raw<T, V>& raw, int u, int thread) __attribute__((always_inline)) {
-        raw.template load<WIDE>(from + static_cast<int64_t>(min(place(u, thread), max(vectors - 1, 0))) * V);
+        raw.template load<WIDE>(from + static_cast<int64_t>(max(min(place(u, thread), vectors - 1), 0)) * V);
     };
     // chunks that are there for every thread; one that is not may follow
     const int whole = max(0, min(loads, vectors / kThreads - first));
     Raw<T, V> raw[kAhead], last;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) load(raw[i], i, threadIdx.x);
-    load(last, whole, threadIdx.x);
+    for (int i = 0; i < kAhead; ++i) load(raw[i], min(i, loads - 1), threadIdx.x);
+    load(last, min(whole, loads - 1), threadIdx.x);
     // fewer than V values behind the last whole load: one each in the first lanes of the last segment
     const int rest_at = vectors * V + lane;
     const bool has_rest = segment == segments - 1 && wave == 0 && lane < rest;
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             sum(u + i, raw[i], std::true_type{});
-            load(raw[i], u + i + kAhead, threadIdx.x);
+            load(raw[i], min(u + i + kAhead, whole - 1), threadIdx.x);
         }
     }
 #pragma unroll

@@ -198,7 +198,7 @@ __device__ __forceinline__ int over_lanes(int v, int lanes, int lane) {
 
 // A workgroup has a segment of up to kMaxLoads chunks, one load a lane each; kAhead of them are under way while one is summed.  What each load's largest value is goes to LDS, and
 // when all were seen a bound says which loads have one of the best entries: their values are read once more, a lane each, and what reaches the bound is ranked (each
-// counts the others that are larger).  64 x 8 rows of 50280 bf16, count 16, take 21 us (2.5 TB/s): the loop 16, bound by the vector units (the loads alone 10), and the
+// counts the others that are larger).  64 x 8 rows of 50280 bf16, count 16, take 20 us (2.6 TB/s): the loop 16, bound by the vector units (the loads alone 10), and the
 // selection of the last of a CU's four workgroups, which the others' hide behind their loops.  (Registers handed on from load to load, for which the compiler waits each time,
 // 26; entries kept on the way, as token_logprobs has them, 35; three to five loads ahead the same; six or eight workgroups a CU 26 and 28.)
 constexpr int kAhead = 2;

@@ -419,7 +419,9 @@ class MXFP4Linear(nn.Module):
     def from_fp16(cls, originalLayer: nn.Linear, out_dtype=None):
         assert originalLayer.bias is None, "Not support bias yet"
         q = cls(originalLayer.in_features, originalLayer.out_features, originalLayer.weight.device, out_dtype)
-        q.weight, q.weight_scales = ops.mxfp4_quant(originalLayer.weight.detach())
+        codes, scales = ops.mxfp4_quant(originalLayer.weight.detach())
+        q.weight.copy_(codes)                  # (of small layers they lie in one allocation, which some formats of checkpoints refuse)
+        q.weight_scales.copy_(scales)
         return q
 
     @torch.no_grad()

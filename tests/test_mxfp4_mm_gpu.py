@@ -261,3 +261,15 @@ def test_offsets_past_32_bits(dev, m, n):
             last = min(n, first + (1 << 27))
             at = torch.arange(first, last, device=dev) % of_w
             assert torch.equal(got[r, first:last], row[at]), (r, first)
+
+
+def test_a_small_layer_is_saved_by_itself(dev, tmp_path):
+    """weights and scales in memory of their own each, whatever mxfp4_quant does with small answers"""
+    q = MXFP4Linear.from_fp16(torch.nn.Linear(64, 8, bias=False).half().to(dev))
+    assert q.weight.untyped_storage().data_ptr() != q.weight_scales.untyped_storage().data_ptr()
+    checkpoints = pytest.importorskip("safetensors.torch")
+    checkpoints.save_model(q, str(tmp_path / "layer.safetensors"))
+    other = MXFP4Linear(64, 8, device=dev)
+    checkpoints.load_model(other, str(tmp_path / "layer.safetensors"))
+    x = torch.randn(3, 64, device=dev).half()
+    assert torch.equal(other(x), q(x))

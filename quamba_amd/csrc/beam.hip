@@ -16,61 +16,48 @@ namespace {
 constexpr int kMaxBeams = 64, kMaxVocab = 1 << 20;
 constexpr int kMaxLoads = 16;              // chunks of a segment
 
-// A sum of exponentials is s 2^e e^m: e keeps s near 1 where the logits are, m is 0 unless they are further from 0 than kFarthest.
+// A sum of exponentials is s e^m, m the largest logit of what it covers: s is 1 at least, and 1 exactly where one logit has all of the weight.  Of nothing m is -inf and s 0, or
+// NaN where there was one.
 struct BeamPart {
     float m;
-    int e;
     double s;
 };
 
-// The sum of a part of a row, by one wave (all but s are the same in its lanes).  64 bits hold e^600 as well as e^-600, so where the first values are is good enough until one is
-// more than kReach above it.
+// The sum of a part of a row, by one wave (all but s are the same in its lanes).  64 bits hold e^600 as well as e^-600, so the first values' largest, m, is near enough until one is
+// more than kReach above it.  Terms are taken of the differences from it, which are exact: rows that differ by a number have the same terms.
 constexpr float kReach = 600.0f;
 constexpr int kSteps = 512;
-constexpr double kLn2Wide = 0.69314718055994531;
-constexpr int kNowhere = 1 << 29;          // below it there is no e of a sum
 __device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 struct WideSum {
-    float m;
-    int e;
     double s;
-    float limit, least;        // values above the one are seen from another place (-inf: none was seen yet), those below the other count as it
-    double round;
+    float m;                   // -inf: no value was seen yet
+    float limit, least;        // values above the one are seen from another place, those below the other count as it
     __device__ __forceinline__ void clear() {
-        m = 0.0f;
-        e = 0;
         s = 0.0;
-        limit = -__builtin_inff();
+        m = limit = -__builtin_inff();
         least = 0.0f;
-        round = 0.0;
     }
     // seen from where values up to `most` are
     __device__ __forceinline__ void place(float most) {
-        const float before_m = m;
-        const int before_e = e;
-        const bool near = fabsf(most) <= kFarthest;
-        m = uniform(near ? 0.0f : most);
-        e = __builtin_amdgcn_readfirstlane(near ? static_cast<int>(rintf(most * kLog2e)) : 0);
-        if (limit > -__builtin_inff()) s *= exp(fmax((static_cast<double>(before_m) - m) + (before_e - e) * kLn2Wide, -700.0));
-        const float here = near ? static_cast<float>(e) * kLn2 : m;
-        limit = uniform(here + kReach);
-        least = uniform(here - 700.0f);
-        // (1.5 * 2^52: the rounded multiple of a step is in the low word; less the steps of 2^e)
-        round = 6755399441055744.0 - static_cast<double>(e) * kSteps;
+        if (m > -__builtin_inff()) s *= exp(fmax(static_cast<double>(m) - most, -700.0));
+        m = uniform(most);
+        limit = uniform(most + kReach);
+        least = uniform(most - 700.0f);
     }
-    // e^d, d from -700 to kReach + some (a NaN stays one), added for B values d = v - m; powers those of kPowers.  In steps, so that the reads of the table are on
+    // e^d, d from -700 to kReach + some (a NaN stays one), added for B values to `to`; powers those of kPowers.  In steps, so that the reads of the table are on
     // their way together: one after the other they took 130 cycles a value, most of it waiting.
     template <int B>
-    __device__ __forceinline__ void add_exponentials(const double (&d)[B], const double* powers) {
-        constexpr double kPerUnit = 738.65986093514926, kStep = 0.0013538030870311431;     // 512 log2 e, ln 2 / 512
+    static __device__ __forceinline__ double exponentials(double to, const double (&d)[B], const double* powers) {
+        // 512 log2 e, ln 2 / 512; the rounded multiple of a step is in the low word of 1.5 * 2^52 and it
+        constexpr double kPerUnit = 738.65986093514926, kStep = 0.0013538030870311431, kRound = 6755399441055744.0;
         int n[B];
         double value[B], power[B];
 #pragma unroll
         for (int j = 0; j < B; ++j) {
-            const double shifted = __builtin_fma(d[j], kPerUnit, round);
+            const double shifted = __builtin_fma(d[j], kPerUnit, kRound);
             n[j] = static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, shifted)));
-            const double r = __builtin_fma(shifted - round, -kStep, d[j]);
+            const double r = __builtin_fma(shifted - kRound, -kStep, d[j]);
             value[j] = __builtin_fma(__builtin_fma(r, 0.5, 1.0), r, 1.0);
         }
 #pragma unroll
@@ -82,50 +69,46 @@ struct WideSum {
             uint32_t high;
             asm("v_lshl_add_u32 %0, %1, 11, %2" : "=v"(high) : "v"(n[j]), "v"(bits[1]));
             bits[1] = high;
-            s = __builtin_fma(value[j], __builtin_bit_cast(double, bits), s);
+            to = __builtin_fma(value[j], __builtin_bit_cast(double, bits), to);
         }
+        return to;
     }
     static_assert(kSteps == 1 << 9, "the shift into the exponent: 20 - 9");
     // values of which `most` is the largest of this lane's
     template <int B>
     __device__ __forceinline__ void add(const float (&v)[B], float most, const double* powers) {
         if (__builtin_amdgcn_ballot_w64(most > limit)) place(wave_max(most));
-        if (!(limit > -__builtin_inff())) {
+        if (!(m > -__builtin_inff())) {
             // (masked values alone, or NaNs)
 #pragma unroll
             for (int j = 0; j < B; ++j) s = v[j] == v[j] ? s : __builtin_nan("");
             return;
         }
         double d[B];
-        if (m == 0.0f) {
+        if (fabsf(m) <= kFarthest) {
 #pragma unroll
             for (int j = 0; j < B; ++j) {
                 float one;                                 // (the larger, a NaN if there is one)
                 asm("v_maximum3_f32 %0, %1, %2, %2" : "=v"(one) : "v"(v[j]), "v"(least));
-                d[j] = one;
+                d[j] = static_cast<double>(one) - m;
             }
         } else {
+            // (m - 700 is no number of 32 bits here)
 #pragma unroll
             for (int j = 0; j < B; ++j) {
                 d[j] = static_cast<double>(v[j]) - m;
                 d[j] = d[j] < -700.0 ? -700.0 : d[j];
             }
         }
-        add_exponentials(d, powers);
+        s = exponentials(s, d, powers);
+    }
+    // the wave's: `most` its largest value.  Divided by what its own term is, so that this one counts as 1 whatever the approximation is off by.
+    __device__ __forceinline__ BeamPart part(float most, const double* powers) const {
+        if (!(m > -__builtin_inff())) return {m, s};
+        const double d[1] = {static_cast<double>(most) - m};
+        return {most, s / exponentials(0.0, d, powers)};
     }
 };
-
-// Both sums as one, seen from the higher place.
-__device__ __forceinline__ BeamPart joined(BeamPart a, BeamPart b) {
-    if (a.s == 0.0 || b.s == 0.0) return a.s == 0.0 ? b : a;
-    if (a.m == 0.0f && b.m == 0.0f) {
-        const int e = max(a.e, b.e);
-        return {0.0f, e, ldexp(a.s, max(a.e - e, -2000)) + ldexp(b.s, max(b.e - e, -2000))};
-    }
-    const double apart = (static_cast<double>(b.m) - a.m) + (b.e - a.e) * kLn2Wide;
-    if (apart > 0.0) return {b.m, b.e, a.s * exp(fmax(-apart, -700.0)) + b.s};
-    return {a.m, a.e, a.s + b.s * exp(fmax(apart, -700.0))};
-}
 
 template <int MASK>
 __device__ __forceinline__ double across(double v, int lane) { return __builtin_bit_cast(double, lm::across<MASK>(__builtin_bit_cast(uint64_t, v), lane)); }
@@ -142,6 +125,21 @@ __device__ __forceinline__ void each_mask(int end, F&& f) {
 __device__ __forceinline__ double wave_sum(double s, int lane) {
     each_mask(64, [&](auto mask) { s += across<decltype(mask)::value>(s, lane); });
     return s;
+}
+
+// Both sums as one.
+__device__ __forceinline__ BeamPart joined(BeamPart a, BeamPart b) {
+    const BeamPart high = b.m > a.m ? b : a, low = b.m > a.m ? a : b;
+    return {high.m, low.s == 0.0 ? high.s : high.s + low.s * exp(static_cast<double>(low.m) - high.m)};
+}
+// The sums of `lanes` neighbouring lanes as one, in all of them: the largest first, then one exponential each, and their sum.
+__device__ __forceinline__ BeamPart joined_over(BeamPart r, int lanes, int lane) {
+    float m = r.m;
+    each_mask(lanes, [&](auto mask) { m = fmaxf(m, __uint_as_float(word_across<decltype(mask)::value>(__float_as_uint(m), lane))); });
+    r.s = r.s == 0.0 ? 0.0 : r.s * exp(static_cast<double>(r.m) - m);
+    each_mask(lanes, [&](auto mask) { r.s += across<decltype(mask)::value>(r.s, lane); });
+    r.m = m;
+    return r;
 }
 
 // powers[i] = 2^(i / kSteps), less i steps in the exponent's place: n steps added there, whatever n, make 2^(n / kSteps) of powers[n mod kSteps].  (Worked out by each
@@ -280,9 +278,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
     most = fmaxf(most, rest_v);
     if (segment == segments - 1 && wave == 0) r.add(one, rest_v, s_powers);
     r.s = wave_sum(r.s, lane);
-    if (lane == 0) s_part[wave] = {r.m, r.e, r.s};
 
     const float bound = bound_of_lanes(most, top, s_candidates, wave, lane);
+    const BeamPart mine = r.part(value_of_key(s_candidates.keys[wave][0]), s_powers);
+    if (lane == 0) s_part[wave] = mine;
     // (of chunks that are there, in bits)
     uint32_t hits = 0, there = (1u << max(loads, 0)) - 1;
     if (whole < loads && place(whole, threadIdx.x) >= vectors) there &= ~(1u << whole);
@@ -331,8 +330,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void beam_rows_kernel(QaBeamSearchP
     BeamPart* const parts = static_cast<BeamPart*>(p.workspace);
     Entry* const out = reinterpret_cast<Entry*>(parts + static_cast<int64_t>(p.batch) * p.beams * segments) + static_cast<int64_t>(blockIdx.x) * top;
     // (by the last wave, which has the fewest candidates to rank)
-    if (threadIdx.x == kThreads - 64) parts[blockIdx.x] = joined(joined(s_part[0], s_part[1]), joined(s_part[2], s_part[3]));
-    static_assert(W == 4, "a sum of each wave");
+    if (wave == W - 1) {
+        const BeamPart all = joined_over(s_part[lane % W], W, lane);
+        if (lane == 0) parts[blockIdx.x] = all;
+    }
     const int count = s_candidates.count;
     if (again <= kCandidates && count <= kCandidates - 8) {
         by_lanes(count, kThreads, [&](int i, int sub, int lanes) {
@@ -411,7 +412,7 @@ constexpr int kSlots = kMaxBeams * kMaxSegments + 1024;
 constexpr int join_lds(int entries) { return entries <= kKept ? kKept * 12 : kSlots * 8 + kMaxBeams * kMaxSegments * 2; }
 __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchParams p, int top, int segments) {
     static_assert(kMaxSegments <= 64 && kMaxTop <= 64, "a lane for each");
-    __shared__ double s_rest[kMaxBeams], s_base[kMaxBeams];        // of a beam: own score - ln s, -inf: it offers nothing; m + e ln 2
+    __shared__ double s_rest[kMaxBeams], s_base[kMaxBeams];        // of a beam: own score - ln s, -inf: it offers nothing; m
     __shared__ uint8_t s_done[kMaxBeams], s_beam[kOffers];
     __shared__ __attribute__((aligned(16))) uint64_t s_keys[kOffers + 8];
     __shared__ uint32_t s_at[kOffers], s_token[kOffers];
@@ -451,30 +452,17 @@ __global__ __launch_bounds__(kJoinThreads) void beam_join_kernel(QaBeamSearchPar
         const int64_t row = entry * p.beams + (there ? beam : 0);
         const double own = p.scores[row];
         const uint8_t end_reached = p.done ? p.done[row] : 0;
-        BeamPart r = {0.0f, 0, 0.0}, second = r;
+        BeamPart r = {-__builtin_inff(), 0.0}, second = r;
         if (there && part < segments) r = parts[beam * segments + part];
         if (there && part + share < segments) second = parts[beam * segments + part + share];
         const bool done = end_reached != 0;
         if (share < segments) r = joined(r, second);
         for (int i = part + 2 * share; there && i < segments; i += share) r = joined(r, parts[beam * segments + i]);
-        if (__builtin_amdgcn_ballot_w64(r.m != 0.0f) == 0) {
-            // one place for all of them, then their sum (bit for bit what joined gives: powers of two round nothing)
-            int e = r.s == 0.0 ? -kNowhere : r.e;
-            each_mask(share, [&](auto mask) { e = max(e, static_cast<int>(word_across<decltype(mask)::value>(static_cast<uint32_t>(e), lane))); });
-            r.s = ldexp(r.s, max((r.s == 0.0 ? e : r.e) - e, -2000));
-            r.e = e;
-            each_mask(share, [&](auto mask) { r.s += across<decltype(mask)::value>(r.s, lane); });
-        } else {
-            each_mask(share, [&](auto mask_c) {
-                constexpr int mask = decltype(mask_c)::value;
-                const BeamPart other = {__uint_as_float(word_across<mask>(__float_as_uint(r.m), lane)), static_cast<int>(word_across<mask>(static_cast<uint32_t>(r.e), lane)), across<mask>(r.s, lane)};
-                r = joined(r, other);
-            });
-        }
+        r = joined_over(r, share, lane);
         if (there && part == 0) {
             const bool offers = own > -__builtin_inf() && own < __builtin_inf() && (done || r.s > 0.0);
             s_rest[beam] = !offers ? -__builtin_inf() : done ? own : own - log(r.s);
-            s_base[beam] = done ? 0.0 : r.m + r.e * kLn2Wide;
+            s_base[beam] = done ? 0.0 : r.m;
             s_done[beam] = done;
         }
     }

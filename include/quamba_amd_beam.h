@@ -20,7 +20,9 @@ int qa_beam_abi_version(void);
 /*
  * Of each of `batch` entries the `count` best continuations of its beams.  Beam i offers every token v with the score
  *   scores[b, i] + l[b, i, v] - log sum_u exp l[b, i, u]
- * in 64 bits, rounded to fp32 as it is written; larger scores come first, of equal ones the lower beam's, then the lower token's.
+ * in 64 bits, rounded to fp32 as it is written; larger scores come first, of equal ones the lower beam's, then the lower token's.  The exponentials
+ * are good to 1e-14 of themselves, so scores of different beams that are nearer than that may come in either order; but a token that has all of its
+ * beam's weight has exactly the beam's score, tokens of equal logits share it evenly, and beams whose logits differ by one number have equal scores.
  * (Tokens of one beam whose logits differ by less than 64 bits of their scores show come in either order.)
  * A beam that is done offers itself once, with its score and the token -1, and its logits are not read.  A score of -inf is no offer: masked
  * tokens, and beams whose own score is that.  A beam offers nothing either where its logits are all -inf or hold a NaN or +inf, or where

@@ -4,8 +4,7 @@
 // workgroup for each entry of the batch joins the sums of its beams, turns the entries into scores and ranks those that reach a bound.
 //
 // Scores of different beams are compared, and which of two comes first is an answer in whole numbers.  So the sums are held in 64 bits and their terms are good to
-// some 1e-10: e^d is 2^(n / 512) from a table by e^r, |r| <= ln 2 / 1024, from a polynomial whose first missing term is r^3 / 6 < 6e-11.  Operations in 64 bits take 5.4
-// cycles of a wave and those in 32 some 4 to 5; thirteen of them a value are what a launch on many rows takes its time for.
+// 1e-14: e^d is 2^(n / 512) from a table by e^r, |r| <= ln 2 / 1024, from a polynomial whose first missing term is r^4 / 24 < 9e-15.
 #include "../../include/quamba_amd_beam.h"
 #include "logit_rows.hpp"
 
@@ -58,7 +57,7 @@ struct WideSum {
             const double shifted = __builtin_fma(d[j], kPerUnit, kRound);
             n[j] = static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, shifted)));
             const double r = __builtin_fma(shifted - kRound, -kStep, d[j]);
-            value[j] = __builtin_fma(__builtin_fma(r, 0.5, 1.0), r, 1.0);
+            value[j] = __builtin_fma(__builtin_fma(__builtin_fma(r, 1.0 / 6.0, 0.5), r, 1.0), r, 1.0);
         }
 #pragma unroll
         for (int j = 0; j < B; ++j) power[j] = powers[n[j] & (kSteps - 1)];

@@ -1018,8 +1018,8 @@ class BeamCandidates(NamedTuple):
 def beam_search_step(logits, scores, count, done=None):
     """The ``count`` best continuations of each entry's beams (qa_beam_search_step): beam i offers token v with the score
     scores[b, i] + log_softmax(logits[b, i])[v].  logits (batch, beams, vocab) fp16, bf16 or fp32, contiguous along the last dimension, up to 64
-    beams and 2^20 tokens; scores fp32 (batch, beams); 1 <= count <= 64.  Scores are compared in 64 bits; of equal ones the lower beam's
-    comes first, then the lower token's.  Returns BeamCandidates.
+    beams and 2^20 tokens; scores fp32 (batch, beams); 1 <= count <= 64.  Scores are compared in 64 bits (their exponentials good to
+    1e-14 of themselves); of equal ones the lower beam's comes first, then the lower token's.  Returns BeamCandidates.
 
     ``done`` bool (batch, beams): such a beam offers itself once, with its score and the token -1, whatever its logits.  A score of -inf is
     no candidate: masked tokens, and beams that are not there (the first step: one beam with 0, the others with -inf).  A beam offers nothing either if

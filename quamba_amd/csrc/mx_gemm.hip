@@ -8,11 +8,16 @@ namespace {
 constexpr int64_t kMaxPitch = 1 << 22;     // bytes of an operand's row: those of a tile in 32 bits
 constexpr int kMaxRows = 0x7fffffff - 255; // rows and columns: whole tiles of them in 32 bits
 
-int check(const QaMxGemmParams& p) {
+// (the workspace does not go by the output's type)
+int check_rows(const QaMxGemmParams& p) {
     if (p.m < 0 || p.n < 0 || p.k < 0) return QA_ERR_SHAPE;
-    if (!is_float_type(p.out_type) || (p.a_type != QA_LM_I8 && !is_float_type(p.a_type))) return QA_ERR_UNSUPPORTED;
+    if (p.a_type != QA_LM_I8 && !is_float_type(p.a_type)) return QA_ERR_UNSUPPORTED;
     if (p.k % kBlock != 0 || p.k / 2 > kMaxPitch || p.m > kMaxRows || p.n > kMaxRows) return QA_ERR_SHAPE;
     return QA_OK;
+}
+int check(const QaMxGemmParams& p) {
+    const int status = check_rows(p);
+    return status == QA_OK && !is_float_type(p.out_type) ? QA_ERR_UNSUPPORTED : status;
 }
 bool fused(const QaMxGemmParams& p) { return p.a_type != QA_LM_I8 && direct_takes_numbers(p); }
 int64_t code_bytes(const QaMxGemmParams& p) { return static_cast<int64_t>(p.m) * ((p.k / 2 + 15) / 16 * 16); }
@@ -25,7 +30,7 @@ int64_t workspace_bytes(const QaMxGemmParams& p, bool one_launch) { return p.a_t
 
 extern "C" int64_t qa_mxfp4_mm_workspace_bytes(const QaMxGemmParams* p) {
     using namespace qa::mx;
-    return p && check(*p) == QA_OK && p->m > 0 && p->n > 0 && p->k > 0 ? workspace_bytes(*p, fused(*p)) : 0;
+    return p && check_rows(*p) == QA_OK && p->m > 0 && p->n > 0 && p->k > 0 ? workspace_bytes(*p, fused(*p)) : 0;
 }
 
 extern "C" int qa_mxfp4_mm(const QaMxGemmParams* p, void* stream_) {

@@ -5,6 +5,8 @@
 //
 // Scores of different beams are compared, and which of two comes first is an answer in whole numbers.  So the sums are held in 64 bits and their terms are good to
 // 1e-14: e^d is 2^(n / 512) from a table by e^r, |r| <= ln 2 / 1024, from a polynomial whose first missing term is r^4 / 24 < 9e-15.
+// With the difference from the largest logit that makes thirteen instructions a value, nine of them in 64 bits (5.4 cycles of a wave each, those in 32 some 4 to 5): what a launch
+// on many rows takes its time for.
 #include "../../include/quamba_amd_beam.h"
 #include "logit_rows.hpp"
 
@@ -195,9 +197,10 @@ __device__ __forceinline__ int over_lanes(int v, int lanes, int lane) {
 
 // A workgroup has a segment of up to kMaxLoads chunks, one load a lane each; kAhead of them are under way while one is summed.  What each load's largest value is goes to LDS, and
 // when all were seen a bound says which loads have one of the best entries: their values are read once more, a lane each, and what reaches the bound is ranked (each
-// counts the others that are larger).  64 x 8 rows of 50280 bf16, count 16, take 20 us (2.6 TB/s): the loop 16, bound by the vector units (the loads alone 10), and the
-// selection of the last of a CU's four workgroups, which the others' hide behind their loops.  (Registers handed on from load to load, for which the compiler waits each time,
-// 26; entries kept on the way, as token_logprobs has them, 35; three to five loads ahead the same; six or eight workgroups a CU 26 and 28.)
+// counts the others that are larger).  64 x 8 rows of 50280 bf16, count 16, take 21.4 us (2.4 TB/s): the loop, bound by the vector units with 20 instructions a value in all (the
+// loads alone 10), and some 4 for the selection of the last of a CU's four workgroups, which the others' hide behind their loops.  (By terms of two instructions less, that do not
+// keep equal scores equal, 20; by those: registers handed on from load to load, for which the compiler waits each time, 26; entries kept on the way, as token_logprobs has
+// them, 35; three to five loads ahead the same; six or eight workgroups a CU 26 and 28.)
 constexpr int kAhead = 2;
 
 template <class T, bool WIDE>
@@ -402,8 +405,8 @@ __device__ __forceinline__ uint64_t bound_of_keys(uint64_t mine, int count, uint
 // An entry of the batch.  The lanes are shared out among the beams and join their segments' sums; meanwhile the lists are on their way.  Up to kKept entries, four a lane,
 // get their scores' keys at once: a bound, the `count`-th largest of what the lanes have best, leaves about as many offers, and those are ranked, each counting the
 // others that are larger.  Of more than that the first entry of each list alone says whether any of it counts: a bound that `count` firsts reach leaves
-// about as many lists, and a second one over their entries, a wave four lists at a time, about as many offers.  (us of this launch: 4 beams of 25 segments, count 8, 5.5,
-// lists first 7.6; 5 of 63, count 10, 8.3, all entries first, 13 a lane, 10.5; 30 of 28, count 60, 18, the lists' entries one after the other 27; all entries sorted, 64 at a
+// about as many lists, and a second one over their entries, a wave four lists at a time, about as many offers.  (us of this launch: 4 beams of 25 segments, count 8, 5.4,
+// lists first 7.6; 5 of 63, count 10, 7.9, all entries first, 13 a lane, 10.5; 30 of 28, count 60, 18.7, the lists' entries one after the other 27; all entries sorted, 64 at a
 // time, 8 and 26 for the first two; a wave eight or sixteen lists at a time 9 and 10.5 for the second.)  What is left are some ten waits, for memory and for LDS, one after the other.  Where more reach the bounds than there is room
 // for - equal scores, or as many places as lanes - each wave sorts what its lanes have.
 constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64, kOffers = 256, kFew = 48, kEach = 4, kKept = kEach * kJoinThreads;

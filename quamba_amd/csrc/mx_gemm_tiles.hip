@@ -7,8 +7,9 @@
 // each fragment while the two tiles last.
 //
 // Register-only loops of this instruction reach 7.0 PFLOP/s with random operands (9.0 with zeros: the clock follows the power) and those of 32x32x64 6.5
-// (9.5).  8192 x 10240 x 2560 takes 98 us, 4.4 PFLOP/s, and 125 where the power leaves a lower clock: the main loop 1.82 us a k tile of 256 x 256 outputs against 1.15 on
-// registers alone (LDS busy for more than half of it), the outputs 18 in all.  64 x 50280 x 2560 takes 13.5 us, its bytes at 5.5 TB/s.
+// (9.5).  8192 x 10240 x 2560 takes 125 us, 3.4 PFLOP/s, where calls follow each other, and 97 to 102 after a pause: 205 thousand cycles (2.0 GHz at 102 us, 2.45 with zeros as
+// operands, 86 us).  In the faster of the two the main loop is 1.82 us a k tile of 256 x 256 outputs against 1.15 on registers alone (LDS busy for more than half of
+// it), the outputs 18 in all.  64 x 50280 x 2560 takes 13.5 us, its bytes at 5.5 TB/s.
 #include "gemm_core.hpp"
 #include "mx_gemm.hpp"
 
@@ -173,7 +174,7 @@ struct TileCfg : Cfg<TM, TN, WGM, WGN, STAGES> {
     using Scales = ScaleLoader<Base::kBM, Base::kBN, Base::kWaves>;
     static constexpr int kScaleBuffers = 2;
     static constexpr int kLds = Base::kLdsBytes + kScaleBuffers * Scales::kBytes;
-    static_assert(STAGES <= 4, "a scale buffer is written again four tiles after it was read");
+    static_assert(5 - STAGES > 0, "group g's scales are last read in tile 2 g, and those of group g + 2 requested into their buffer in tile 2 g + 4 - (STAGES - 1)");
 };
 
 // MASKED: the last group has blocks behind K.  first: the output's tiles of 256 x 256 from that one on, in smaller ones; or -1: all of it.
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void mxfp4_tiles_kernel(QaMxGemmPar
     load_w.template init<WAVES>(0, columns, p.ldw, wave, lane);
     const Scales load_s = {p.a_scales + static_cast<int64_t>(m0) * 16, p.w_scales + static_cast<int64_t>(n0) * 16, p.a_scale_group_stride, p.w_scale_group_stride, rows, columns};
 
-    // Requests of a tile: its operands', and the scales' in front of them for the first tile of a group.  They go out one at a time, one per kPace multiplications counted
+    // Requests of a tile: its operands', and the scales' behind them for the first tile of a group.  They go out one at a time, one per kPace multiplications counted
     // from the barrier: those that fit behind it, whose stage it has just freed, for tile t + STAGES, the rest during the next tile.  Past the end of K every
     // lane is out of range and stores zeros.
     constexpr int kData = C::kAInstr + C::kWInstr, kMost = kData + Scales::kEach;

@@ -4,9 +4,10 @@
 // then writes them, so that no row is read after it was written and no copy is needed.  Rows that stay are neither read nor written, and a parent of several
 // rows comes from memory once and from the caches again.  One launch has up to kTensors tensors, with their addresses in its arguments.
 //
-// Bound by memory: 16 rows of 64 layers of 5120 x 16 fp32 states and their conv states, 479 MB of them read or written, take 81 us, 5.9 TB/s (one unit a thread 84).  States
-// that the last-level cache does not hold are written past it (89 us otherwise); those that it holds are read again soon (2 x 16 rows of 32 layers, 151 MB, 37 us, and 46
-// past it).  Rows of 2331 bytes, 256 of them in 64 tensors, take 15.6 us and of 2352 12.2 (a byte a lane 37).
+// Bound by memory: 4 x 4 rows of 64 layers of 5120 x 16 fp32 states and their int8 conv states, two launches that read and write 462 MB, take 99 us, 4.7 TB/s, where other states
+// were moved before, and 75 us again and again.  (2 x 16 rows of 32 layers of 4096, 434 MB: 87 and 73; one unit a thread 97 and 76, and 89 and 76.)  States that the last-level
+// cache does not hold are written past it (102 and 85 us otherwise, and 98 and 66); those that it holds are read again soon (2 x 16 rows of 32 layers of 2048, 143 MB, again and
+// again 32 us, 42 past it; after others 53 and 43).  Rows of 2331 bytes, 256 of them in 64 tensors, take 15.6 us and of 2352 12.2 (a byte a lane 37).
 #include "../../include/quamba_amd_beam.h"
 #include "lm_common.hpp"
 

@@ -404,7 +404,8 @@ class W4A8B8O8LinearParallel(_W4A8Base):
 # ------------------------------------------------------------------------------------------------
 class MXFP4Linear(nn.Module):
     """fp16, bf16 or fp32 in and out (``out_dtype``, by default the type of the input): x @ w.T with x and w in the format of ops.mxfp4_quant.
-    ``in_features`` is a multiple of 32, ``out_features`` anything."""
+    ``in_features`` is a multiple of 32, ``out_features`` anything.  A model's head, or a layer that a program calls by itself: the mixers take
+    their own int8 and W4A8 linears as projections."""
 
     def __init__(self, in_features, out_features, device=None, out_dtype=None):
         super().__init__()

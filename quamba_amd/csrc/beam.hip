@@ -25,7 +25,7 @@ struct BeamPart {
 };
 
 // The sum of a part of a row, by one wave (all but s are the same in its lanes).  64 bits hold e^600 as well as e^-600, so the first values' largest, m, is near enough until one is
-// more than kReach above it.  Terms are taken of the differences from it, which are exact: rows that differ by a number have the same terms.
+// more than kReach above it.  Terms are taken of the differences from it, exact in 64 bits (but for logits 2^29 times smaller than m): rows that differ by a number have the same terms.
 constexpr float kReach = 600.0f;
 constexpr int kSteps = 512;
 __device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
